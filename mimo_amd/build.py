@@ -15,7 +15,10 @@ INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 LIB_PATH = os.path.join(ROOT, "libmimo_hip.so")
 SOURCES = ["gemm_conv.hip", "hconv.hip", "thinconv.hip", "gemm_stream.hip", "ff_fused.hip", "ff_tail4.hip", "attention.hip", "norm.hip", "elementwise.hip", "image.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + INCLUDE, "-I" + CSRC]
+# no packed fp32 (v_pk_add / mul / fma_f32): hipcc makes them by itself from scalar float code, and some of their forms have given
+# wrong results on MI355X now and then.  Price: 0.4 % of a 512 x 512 clip (15.84 -> 15.77 frames/s, two interleaved runs each)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + INCLUDE, "-I" + CSRC,
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # ff_tail4.hip: one wave per SIMD — packed fp32 VALU (what the SLP vectoriser makes of adjacent scalar adds / fmas) is slow
 # beside MFMAs (MI355X_MICROARCH.md), the GEGLU there is written in scalar operations and must stay scalar
 EXTRA_FLAGS = {"ff_tail4.hip": ["-fno-slp-vectorize", "-Wno-inline-asm"]}
