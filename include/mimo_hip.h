@@ -375,6 +375,40 @@ int mimo_attention_fp8qk(int dtype, const void* q, int64_t ldq, const void* k, i
                          float scale, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * Attention of B images to the states of Be encoder rows (text tokens, image patches) of another length, and its gradients:
+ *   out[b, i, h] = sum_j softmax_j(scale q[b, i, h] . k[e, j, g]) v[e, j, g],   e = b / (B / Be), g = h / (heads / kv_heads)
+ *   replaces the attn2 call of BasicTransformerBlock.forward (src/models/attention.py:412-426) for encoder_hidden_states
+ *   [b, L, cross_dim] with L > 1 (L = 1 collapses to a bias: mimo_gemm's img_bias), including encoder_attention_mask.
+ *   q: half16 [B, Nq, heads d] with element strides q_batch, q_row; k, v: half16 [Be, Nk, kv_heads d] likewise; strides % 8 == 0
+ *   (0 is allowed: a broadcast axis), 16-byte aligned pointers, d % 8 == 0, d <= 160.  B % Be == 0: the images of a clip share
+ *   their encoder row, no copy.  kv_len int32 [Be] (nullable): keys [0, kv_len[e]) count (clamped to [0, Nk]).  mask uint8
+ *   [Be, mask_row] (nullable): keys with a nonzero byte count.  Both may be given.  What k and v hold at keys that do not count
+ *   (NaN included) has no effect.  A row without a key gives out = 0, lse = -inf and zero gradients.
+ *   out: half16 [B, Nq, heads d] contiguous.  lse: fp32 [B, heads, Nq] = ln sum exp (nullable).
+ *   backward: dout with strides dout_batch, dout_row; out, lse from the forward; dq [B, Nq, heads d], dk, dv [Be, Nk, kv_heads d]
+ *   half16 contiguous: dk / dv are summed over the images and query heads that share a key, in a fixed order (no atomics).
+ *   workspace: 16-byte aligned scratch of at least the size that the *_workspace call returns for the same params (0: none
+ *   needed); it holds nothing between calls.  Nq >= 1, Nk >= 0, B / Be * Nq * (heads / kv_heads) < 2^30, Be * kv_heads < 2^16.
+ * --------------------------------------------------------------------------------- */
+typedef struct mimo_cross_attention_params {
+  int B, Be, Nq, Nk, heads, kv_heads, d;
+  float scale;
+  int64_t q_batch, q_row, k_batch, k_row, v_batch, v_row;
+  int64_t dout_batch, dout_row;  /* backward only */
+  const int* kv_len;
+  const void* mask;
+  int64_t mask_row;
+} mimo_cross_attention_params;
+
+size_t mimo_cross_attention_workspace(const mimo_cross_attention_params* p);
+int mimo_cross_attention(int dtype, const void* q, const void* k, const void* v, void* out, float* lse,
+                         const mimo_cross_attention_params* p, void* workspace, size_t workspace_bytes, void* stream);
+size_t mimo_cross_attention_backward_workspace(const mimo_cross_attention_params* p);
+int mimo_cross_attention_backward(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out,
+                                  const float* lse, void* dq, void* dk, void* dv, const mimo_cross_attention_params* p,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Temporal attention over the frame axis without materialising '(b f) d c -> (b d) f c'
  *   replaces VersatileAttention.forward (src/models/motion_module.py:353-390).
  *   q,k,v: half16 [b*F, HW, ld*] (frame-major tokens); attention is over the F frames

@@ -1,0 +1,168 @@
+// cross_attention.hip.h — what the forward and the backward kernels of the cross attention share: arguments, the flat query
+// rows, the masked staging of key / value rows, transposed LDS fragments (gfx950, MFMA 32x32x16).
+//
+// Work is laid out per (encoder row e, key head g).  The queries that see these keys are the images [e G, (e + 1) G), their Nq
+// tokens and the hg query heads of the key head: R = G Nq hg FLAT ROWS, f = (image, token, head) with the head fastest.  A wave
+// takes 32 of them as the 32 columns of a matrix tile, so 24 single-token frames or 8 grouped heads of one token fill a tile
+// as well as 32 neighbouring tokens do.
+#pragma once
+#include "common.hip.h"
+
+namespace mimo_xattn {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// n / d for n < 2^31: (n * mul) >> (31 + shift), mul = floor(2^(31 + shift) / d) + 1, shift = ceil(log2 d); exact, because
+// mul d exceeds 2^(31 + shift) by at most d <= 2^shift and n < 2^31.
+struct FastDiv {
+  uint32_t d, mul;
+  int shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  while ((1ull << f.shift) < d) ++f.shift;
+  f.mul = (uint32_t)((1ull << (31 + f.shift)) / d + 1);
+  return f;
+}
+__device__ __forceinline__ uint32_t div_fast(uint32_t n, const FastDiv& f) {
+  return f.d == 1u ? n : (uint32_t)(((uint64_t)n * f.mul) >> (31 + f.shift));
+}
+
+struct Args {
+  const uint16_t *q, *k, *v;
+  const uint16_t *o, *dout;      // backward: the forward's output and its gradient
+  const float* lse_in;           // backward
+  uint16_t *out, *dk, *dv;       // out: the forward's output, or dq
+  float *lse, *delta;            // [B, heads, Nq]
+  float* ws;                     // partial results of a split launch
+  const int* kv_len;             // [Be] or null
+  const uint8_t* mask;           // [Be, Nk] or null
+  int64_t sqb, sqr, skb, skr, svb, svr, sob, sor, sdb, sdr, smb;  // element strides: batch, row (o / dout: sob.., sdb..)
+  int Be, G, Nq, Nk, kvh, hg, d, R;
+  FastDiv by_hg, by_nq;
+  float c;                       // scale * log2(e): scores leave the matrix unit unscaled
+  float scale;
+  int nb;                        // blocks per (e, g)
+  int nsplit;                    // parts the keys (forward, dq) or the flat rows (dk / dv) are cut into
+};
+
+// (image, token, head) of a flat row
+__device__ __forceinline__ void flat_row(const Args& a, int f, int& img, int& qi, int& hh) {
+  const uint32_t t = div_fast((uint32_t)f, a.by_hg);
+  hh = f - (int)t * a.hg;
+  img = (int)div_fast(t, a.by_nq);
+  qi = (int)t - img * a.Nq;
+}
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }  // arguments <= ~0: flushing is fine
+
+__device__ __forceinline__ int valid_len(const Args& a, int e) {
+  if (!a.kv_len) return a.Nk;
+  const int n = a.kv_len[e];
+  return n < 0 ? 0 : (n > a.Nk ? a.Nk : n);
+}
+__device__ __forceinline__ bool key_valid(const Args& a, int e, int len, int key) {
+  return key < len && (!a.mask || a.mask[(int64_t)e * a.smb + key]);
+}
+
+// A operand of a 32x32x16 MFMA from a row-major LDS tile with rows = the contraction index: lane (h2, i = lane & 31) gets
+// column c0 + i of rows {r0 + 4 h2 + 0..3, r0 + 8 + 4 h2 + 0..3} — the k-slot order in which a 32x32 accumulator tile holds its
+// 16 consecutive rows, so that packed accumulators are the B operand without a lane exchange.  Two hardware-transposed reads:
+// inside a 16-lane group lane m points at row (m >> 2), columns 4 (m & 3).., lane i receives column i of the four rows.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+__device__ __forceinline__ uint4 read_tr(const uint16_t* tile, int pitch, int r0, int c0, int lane) {
+  const int m = lane & 15, cg = (lane >> 4) & 1, h2 = lane >> 5;
+  const uint16_t* p = tile + (r0 + 4 * h2 + (m >> 2)) * pitch + c0 + 16 * cg + 4 * (m & 3);
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 8 * pitch));
+  const uint2 lo = __builtin_bit_cast(uint2, a), hi = __builtin_bit_cast(uint2, b);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
+// eight packed accumulator rows [8 u, 8 u + 8) of a 32x32 tile = the k-step u of the product that contracts over its rows
+template <int DT>
+__device__ __forceinline__ uint4 pack_k(const f32x16& s, int u) {
+  return make_uint4(pack2<DT>(s[8 * u], s[8 * u + 1]), pack2<DT>(s[8 * u + 2], s[8 * u + 3]),
+                    pack2<DT>(s[8 * u + 4], s[8 * u + 5]), pack2<DT>(s[8 * u + 6], s[8 * u + 7]));
+}
+
+// stores 32 channels (tile dt) of the flat rows a 32x32 accumulator tile holds as columns: the two lane halves exchange
+// quadruples so that a lane writes 16 bytes.  p = the row's first channel; live = the row exists.
+template <int DT>
+__device__ __forceinline__ void store_tile(const f32x16& o, float f, uint16_t* p, bool live, int dt, int d, int h2) {
+#pragma unroll
+  for (int c = 0; c < 4; c += 2) {
+    const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(o[4 * c] * f, o[4 * c + 1] * f),
+                                                    pack2<DT>(o[4 * c + 4] * f, o[4 * c + 5] * f), false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(pack2<DT>(o[4 * c + 2] * f, o[4 * c + 3] * f),
+                                                    pack2<DT>(o[4 * c + 6] * f, o[4 * c + 7] * f), false, false);
+    const int d0 = 32 * dt + 8 * c + 8 * h2;
+    if (live && d0 < d) *reinterpret_cast<uint4*>(p + d0) = make_uint4(x[0], y[0], x[1], y[1]);
+  }
+}
+
+// fragments of one row: lane (h2, .) holds channels 16 s + 8 h2 .. + 8.  Channels >= d repeat channel 0 (the partner operand
+// is zero there); rows that do not exist are the caller's to drop.
+template <int KS>
+__device__ __forceinline__ void load_row(uint4 (&f)[KS], const uint16_t* p, int d, int h2) {
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int kk = 16 * s + 8 * h2;
+    f[s] = *reinterpret_cast<const uint4*>(p + (kk < d ? kk : 0));
+  }
+}
+
+// Key and value rows [key0, key0 + n) of (e, g) into row-major LDS tiles of pitch 16 KS + 8 halfs (an odd number of 16-byte
+// units: a 16-lane group of b128 row reads covers all banks).  Rows the mask drops and channels >= d are ZERO whatever memory
+// holds there (NaN included); bias[i] = 0 or -inf is added to their scores.
+template <int KS, int THREADS>
+__device__ __forceinline__ void stage_kv(const Args& a, int e, int g, int len, int key0, int n, uint16_t* ks, uint16_t* vs,
+                                         float* bias, int tid) {
+  constexpr int P = 16 * KS + 8, CH = 2 * KS;
+  const uint16_t* kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
+  const uint16_t* vb = a.v + (int64_t)e * a.svb + (int64_t)g * a.d;
+  for (int i = tid; i < n * CH; i += THREADS) {
+    const int row = i / CH, cc = (i - row * CH) * 8, key = key0 + row;
+    uint4 kv = make_uint4(0, 0, 0, 0), vv = make_uint4(0, 0, 0, 0);
+    if (cc < a.d && key_valid(a, e, len, key)) {
+      kv = *reinterpret_cast<const uint4*>(kb + (int64_t)key * a.skr + cc);
+      vv = *reinterpret_cast<const uint4*>(vb + (int64_t)key * a.svr + cc);
+    }
+    *reinterpret_cast<uint4*>(ks + row * P + cc) = kv;
+    *reinterpret_cast<uint4*>(vs + row * P + cc) = vv;
+  }
+  for (int i = tid; i < n; i += THREADS) bias[i] = key_valid(a, e, len, key0 + i) ? 0.f : -INFINITY;
+}
+
+// bytes of LDS that n staged keys take (+ the transposed reads of the last row's last tile, which run up to 16 halfs past it)
+constexpr int kv_lds(int ks, int n) { return 2 * n * (16 * ks + 8) * 2 + n * 4 + 64; }
+
+inline int cu_count() {
+  static const int cus = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    return n;
+  }();
+  return cus;
+}
+
+// the padded head widths that have kernels: 16 KS halfs, KS = 2 3 4 5 6 8 10
+inline int k_steps(int d) { return d <= 32 ? 2 : d <= 48 ? 3 : d <= 64 ? 4 : d <= 80 ? 5 : d <= 96 ? 6 : d <= 128 ? 8 : 10; }
+
+#define MIMO_XATTN_DISPATCH(ks, CALL) \
+  switch (ks) {                       \
+    case 2: CALL(2); break;           \
+    case 3: CALL(3); break;           \
+    case 4: CALL(4); break;           \
+    case 5: CALL(5); break;           \
+    case 6: CALL(6); break;           \
+    case 8: CALL(8); break;           \
+    default: CALL(10); break;         \
+  }
+
+// fills the geometry; MIMO_OK or an error.  Strides are those of the header's mimo_cross_attention_params.
+int fill(Args& a, const mimo_cross_attention_params* p);
+
+}  // namespace mimo_xattn

@@ -41,6 +41,12 @@ class CompositeParams(ctypes.Structure):  # mimo_composite_params
                                                                  "w_min", "h_min", "mh", "mw", "H", "W")]
 
 
+class CrossAttentionParams(ctypes.Structure):  # mimo_cross_attention_params
+    _fields_ = [(n, c_i) for n in ("B", "Be", "Nq", "Nk", "heads", "kv_heads", "d")] + [("scale", c_f)] + \
+               [(n, c_i64) for n in ("q_batch", "q_row", "k_batch", "k_row", "v_batch", "v_row", "dout_batch", "dout_row")] + \
+               [("kv_len", c_vp), ("mask", c_vp), ("mask_row", c_i64)]
+
+
 # name -> argtypes, mirrors include/mimo_hip.h one to one
 SIGNATURES = {
     "mimo_version": [],
@@ -75,6 +81,10 @@ SIGNATURES = {
                               c_vp, c_i64, c_vp, c_i64, c_i64, c_i, c_vp, c_vp],
     "mimo_block_head_fused": [c_i, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_f, c_vp, c_i64, c_i,
                               c_vp, c_i64, c_vp, c_i64, c_i64, c_i, c_vp],
+    "mimo_cross_attention_workspace": [ctypes.POINTER(CrossAttentionParams)],
+    "mimo_cross_attention": [c_i, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.POINTER(CrossAttentionParams), c_vp, c_sz, c_vp],
+    "mimo_cross_attention_backward_workspace": [ctypes.POINTER(CrossAttentionParams)],
+    "mimo_cross_attention_backward": [c_i] + [c_vp] * 9 + [ctypes.POINTER(CrossAttentionParams), c_vp, c_sz, c_vp],
     "mimo_temporal_attention": [c_i, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i, c_i, c_i64, c_i, c_i, c_f, c_vp],
     "mimo_softmax_rows": [c_i, c_vp, c_i64, c_vp, c_i64, c_i64, c_i, c_f, c_vp],
     "mimo_ncfhw_to_tokens": [c_vp, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_vp, c_i, c_i, c_i64, c_i, c_vp, c_vp],
@@ -99,7 +109,8 @@ class MimoHipError(RuntimeError):
 _lib = None
 
 
-RESTYPES = {"mimo_workspace_bytes": c_sz}  # every other entry point returns int (0 or an error code)
+RESTYPES = {"mimo_workspace_bytes": c_sz, "mimo_cross_attention_workspace": c_sz,
+            "mimo_cross_attention_backward_workspace": c_sz}  # every other entry point returns int (0 or an error code)
 
 
 def load():

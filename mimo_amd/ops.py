@@ -817,6 +817,122 @@ def attention(q, k, v, heads, *, k2=None, v2=None, seg2_first_batch=0, scale=Non
     return out
 
 
+def _require(ok, what):
+    if not ok:
+        raise L.MimoHipError(what)
+
+
+class _on_device:
+    """The launch happens on the tensors' own device, whatever the current one is."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+        return False
+
+
+def _stride(t, i):
+    """Element stride of axis i, 0 where the axis has one entry (its stride is then arbitrary)."""
+    return t.stride(i) if t.shape[i] > 1 else 0
+
+
+def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
+    """Checks the operands of a cross attention and lays their geometry down for the C-ABI."""
+    dt_code(q.dtype)
+    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v: [batch, tokens, channels]")
+    B, Nq, C = q.shape
+    Be, Nk, Ck = k.shape
+    kv_heads = heads if kv_heads is None else kv_heads
+    _require(heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and C % heads == 0, f"{C} channels in {heads} heads over {kv_heads} key heads")
+    d = C // heads
+    _require(d % 8 == 0 and 8 <= d <= 160, f"head width {d}: a multiple of 8 up to 160")
+    _require(Ck == kv_heads * d and v.shape == k.shape, f"k {tuple(k.shape)}, v {tuple(v.shape)}: [encoder rows, keys, {kv_heads * d}]")
+    _require(Be > 0 and B % Be == 0, f"{B} images over {Be} encoder rows")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _require(t.device == q.device and t.dtype == q.dtype, f"{name}: {t.dtype} on {t.device}, q is {q.dtype} on {q.device}")
+        _rows_ok(t, name)
+    scale = d ** -0.5 if scale is None else float(scale)
+    _require(0.0 < scale < float("inf"), f"scale {scale}")
+    p = L.CrossAttentionParams(B, Be, Nq, Nk, heads, kv_heads, d, scale, _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
+                               _stride(v, 0), _stride(v, 1))
+    if kv_len is not None:
+        _require(kv_len.device == q.device and kv_len.dtype == torch.int32 and kv_len.shape == (Be,) and kv_len.is_contiguous(),
+                 f"kv_len: contiguous int32 [{Be}] on {q.device}")
+        p.kv_len = kv_len.data_ptr()
+    if mask is not None:
+        _require(mask.device == q.device and mask.dtype in (torch.bool, torch.uint8) and mask.shape == (Be, Nk) and
+                 (Nk <= 1 or mask.stride(1) == 1), f"mask: bool or uint8 [{Be}, {Nk}] on {q.device}, True where the key counts")
+        p.mask, p.mask_row = mask.data_ptr(), _stride(mask, 0)
+    _chk(q, "q")
+    return p
+
+
+def _rows_ok(t, name):
+    """Rows of whole 16-byte chunks: what the kernels' wide loads need."""
+    _require(t.stride(-1) == 1 or t.shape[-1] <= 1 or t.numel() == 0, f"{name}: the last axis is contiguous")
+    _require(t.data_ptr() % 16 == 0 and all(_stride(t, i) % 8 == 0 for i in range(t.dim() - 1)),
+             f"{name}: 16-byte aligned rows (strides {t.stride()})")
+
+
+def cross_attention(q, k, v, heads, *, kv_heads=None, kv_len=None, mask=None, scale=None, want_lse=False):
+    """Attention of B images to the states of Be encoder rows of another length (text tokens, image patches): half [B, Nq, heads d].
+
+    q: half [B, Nq, heads d]; k, v: half [Be, Nk, kv_heads d] views (any strides of whole 16-byte chunks, the last axis contiguous),
+    B % Be == 0: image b reads encoder row b // (B // Be) — the frames of a clip share theirs without a copy — and query head h reads
+    key head h // (heads // kv_heads).  d a multiple of 8 up to 160; Nq = 1 and long Nk split the keys over the chip.
+    kv_len: int32 [Be] device tensor, only keys below it count; mask: bool / uint8 [Be, Nk], only nonzero keys count (both may be
+    given; what k and v hold elsewhere, NaN included, has no effect).  A query without any key gives zeros.
+    want_lse: returns (out, lse), lse fp32 [B, heads, Nq] = ln sum exp(scale q.k) (-inf without a key), for the backward."""
+    p = _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale)
+    with _on_device(q.device):
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty((p.B, heads, p.Nq), device=q.device, dtype=torch.float32) if want_lse else None
+        if out.numel():
+            fl = 4 * p.B * p.Nq * p.Nk * q.shape[2]
+            _count(fl)
+            nb = L.load().mimo_cross_attention_workspace(ctypes.byref(p))
+            ws = torch.empty((nb // 4,), device=q.device, dtype=torch.float32) if nb else None
+            with _Bracket("attn_kernel", fl, _nbytes(q, k, v, out)):
+                L.call("mimo_cross_attention", dt_code(q.dtype), q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(), _ptr(lse),
+                       ctypes.byref(p), _ptr(ws), nb, _stream())
+    return (out, lse) if want_lse else out
+
+
+def cross_attention_backward(dout, q, k, v, out, lse, heads, *, kv_heads=None, kv_len=None, mask=None, scale=None):
+    """(dq, dk, dv) of cross_attention, half and contiguous, from its operands, its output and its lse (want_lse=True) and the
+    gradient dout [B, Nq, heads d] (any strides of whole 16-byte chunks).  dk and dv are summed over the images and query heads that
+    share a key, in a fixed order: the same bits on every run.  Keys that do not count get zeros."""
+    p = _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale)
+    _require(dout.shape == q.shape and dout.dtype == q.dtype and dout.device == q.device, f"dout {tuple(dout.shape)}: as q")
+    _rows_ok(dout, "dout")
+    _require(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.is_contiguous() and
+             out.data_ptr() % 16 == 0, "out: the forward's output")
+    _require(lse.shape == (p.B, heads, p.Nq) and lse.dtype == torch.float32 and lse.device == q.device and lse.is_contiguous(),
+             "lse: the forward's fp32 [B, heads, Nq]")
+    p.dout_batch, p.dout_row = _stride(dout, 0), _stride(dout, 1)
+    with _on_device(q.device):
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        if not dq.numel():
+            return dq, torch.zeros(k.shape, device=q.device, dtype=q.dtype), torch.zeros(v.shape, device=q.device, dtype=q.dtype)
+        dk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        dv = torch.empty(v.shape, device=q.device, dtype=q.dtype)
+        fl = 10 * p.B * p.Nq * p.Nk * q.shape[2]
+        _count(fl)
+        nb = L.load().mimo_cross_attention_backward_workspace(ctypes.byref(p))
+        ws = torch.empty((nb // 4,), device=q.device, dtype=torch.float32)
+        with _Bracket("attn_kernel", fl, _nbytes(dout, q, k, v, out, dq, dk, dv)):
+            L.call("mimo_cross_attention_backward", dt_code(q.dtype), dout.data_ptr(), q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(),
+                   lse.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dv), ctypes.byref(p), ws.data_ptr(), nb, _stream())
+    return dq, dk, dv
+
+
 def temporal_attention(q, k, v, b, F, HW, heads, *, scale=None):
     """Attention over the F frames of each (batch, pixel, head); q/k/v: [b*F*HW, C] views (last stride 1)."""
     _chk(q, "q")
