@@ -13,7 +13,7 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 LIB_PATH = os.path.join(ROOT, "libmimo_hip.so")
-SOURCES = ["gemm_conv.hip", "hconv.hip", "thinconv.hip", "gemm_stream.hip", "ff_fused.hip", "ff_tail4.hip", "attention.hip", "cross_attention.hip", "cross_attention_bwd.hip",
+SOURCES = ["gemm_conv.hip", "adapter.hip", "hconv.hip", "thinconv.hip", "gemm_stream.hip", "ff_fused.hip", "ff_tail4.hip", "attention.hip", "cross_attention.hip", "cross_attention_bwd.hip",
            "norm.hip", "elementwise.hip", "image.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # no packed fp32 (v_pk_add / mul / fma_f32): hipcc makes them by itself from scalar float code, and some of their forms have given
@@ -43,7 +43,7 @@ def build(force: bool = False, verbose: bool = False, tune: bool = False) -> str
     os.makedirs(objdir, exist_ok=True)
     flags = FLAGS + (["-DMIMO_TUNE"] if tune else [])
     lib_path = TUNE_LIB_PATH if tune else LIB_PATH
-    headers = [os.path.join(CSRC, h) for h in ("common.hip.h", "gemm_stream.hip.h", "thinconv.hip.h", "ff_fused.hip.h", "cross_attention.hip.h")] + [os.path.join(INCLUDE, "mimo_hip.h")]
+    headers = [os.path.join(CSRC, h) for h in ("common.hip.h", "gemm_core.hip.h", "gemm_stream.hip.h", "thinconv.hip.h", "ff_fused.hip.h", "cross_attention.hip.h")] + [os.path.join(INCLUDE, "mimo_hip.h")]
     jobs = []
     objs = []
     for s in SOURCES:

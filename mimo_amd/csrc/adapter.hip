@@ -1,0 +1,638 @@
+// adapter.hip — low-rank adapters of many requests beside a shared projection, and their gradients (gfx950).
+//
+//   out[m] = a[m].W^T + bias + residual[m] + u[m].up[i]^T,   u[m] = scale[i] a[m].down[i]^T,   i = index[m / rows_per_index]
+//
+// The shared projection is one GEMM over all rows, whatever their adapters; u is a thin product in front of it (adapter_low_*:
+// it reads `a` once, a stream) and u.up^T is added to the accumulators of the GEMM's tiles before their epilogue
+// (tile_adapter): the result is written once and no intermediate is wider than the rank.  A tile walks the DISTINCT adapters of
+// its rows, usually one; a row never takes part in another row's adapter (values are selected, not multiplied by zero, so a NaN
+// in one adapter stays in its requests).
+// u is kept as a rounded 16-bit value where the result is 16 bit, and as hi + lo halves (22 / 16 mantissa bits) where the
+// result is fp32 or gradients are to be taken.
+//
+// Backward of the same call, W frozen: t[m] = scale[i] dy[m].up[i];  da = dy.W + t.down (the same kernels on W^T and transposed
+// adapters);  ddown[i] = sum_m t[m]^T a[m];  dup[i] = sum_m dy[m]^T u[m] (adapter_outer_kernel: rows stream through LDS, both
+// operands by transposed reads; parts of the rows joined in a fixed order, no atomics).
+#include "gemm_core.hip.h"
+
+namespace {
+
+inline int cu_count() {
+  static const int cus = [] {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    return n;
+  }();
+  return cus;
+}
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// which adapter a row has
+struct Rows {
+  const int* index;
+  int64_t M, rpi;
+  int n;
+};
+__device__ __forceinline__ int adapter_of(const Rows& r, int64_t m) {
+  if (m >= r.M) return -1;
+  const int i = r.index[r.rpi == 1 ? m : m / r.rpi];
+  return (unsigned)i < (unsigned)r.n ? i : -1;
+}
+
+// the adapter of the first row that is still to do (rows: `n` per-lane values, done or none = -1), or -1
+template <int N>
+__device__ __forceinline__ int next_adapter(const int (&ad)[N]) {
+  int cur = -1;
+#pragma unroll
+  for (int i = N - 1; i >= 0; --i) {
+    const unsigned long long b = __builtin_amdgcn_ballot_w64(ad[i] >= 0);
+    if (b != 0ull) cur = __builtin_amdgcn_readlane(ad[i], (int)__builtin_ctzll(b));
+  }
+  return cur;
+}
+
+}  // namespace
+
+namespace {
+
+template <int DT, int NR, int MT>
+__device__ __forceinline__ void tile_adapter(const GemmArgs& g, f32x4 (&acc)[NR][MT], const int64_t M0, const int N0, const int wm,
+                                             const int wn, const int lg, const int li) {
+  int ad[MT];
+#pragma unroll
+  for (int mi = 0; mi < MT; ++mi) {
+    const int64_t m = M0 + (wm * MT + mi) * 16 + li;
+    int i = -1;
+    if (m < g.M) i = g.ad_index[g.ad_rpi == 1 ? m + g.ad_row0 : (m + g.ad_row0) / g.ad_rpi];
+    ad[mi] = (unsigned)i < (unsigned)g.ad_n ? i : -1;
+  }
+  const uint16_t* low = g.ad_low + (M0 + wm * MT * 16 + li) * g.ad_ld;
+  for (int cur = next_adapter<MT>(ad); cur >= 0; cur = next_adapter<MT>(ad)) {
+    const uint16_t* up = g.ad_up + ((int64_t)cur * g.N + N0 + wn * 16 * NR + li) * g.ad_rank;
+    for (int k0 = 0; k0 < g.ad_cols; k0 += 32) {
+      const int kk = k0 + 8 * lg, ku = kk < g.ad_rank ? kk : kk - g.ad_rank;  // (the lo halves meet the same weights)
+      uint4 fb[NR];
+#pragma unroll
+      for (int ni = 0; ni < NR; ++ni) {
+        fb[ni] = make_uint4(0, 0, 0, 0);
+        if (kk < g.ad_cols && N0 + (wn * NR + ni) * 16 + li < g.N)
+          fb[ni] = *reinterpret_cast<const uint4*>(up + (int64_t)ni * 16 * g.ad_rank + ku);
+      }
+#pragma unroll
+      for (int mi = 0; mi < MT; ++mi) {
+        const bool mine = ad[mi] == cur;
+        const unsigned long long b = __builtin_amdgcn_ballot_w64(mine);
+        if (b == 0ull) continue;
+        uint4 fu = make_uint4(0, 0, 0, 0);
+        if (mine && kk < g.ad_cols) fu = *reinterpret_cast<const uint4*>(low + (int64_t)mi * 16 * g.ad_ld + kk);
+        if (b == ~0ull) {
+#pragma unroll
+          for (int ni = 0; ni < NR; ++ni) acc[ni][mi] = HT<DT>::mfma16(fb[ni], fu, acc[ni][mi]);
+        } else {
+#pragma unroll
+          for (int ni = 0; ni < NR; ++ni) {
+            const f32x4 v = HT<DT>::mfma16(fb[ni], fu, acc[ni][mi]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[ni][mi][r] = mine ? v[r] : acc[ni][mi][r];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) ad[mi] = ad[mi] == cur ? -1 : ad[mi];
+  }
+}
+
+struct LowArgs {
+  const uint16_t *X, *down;  // [M, ldx], [n, r, K]
+  const float* scale;        // [n] or null
+  uint16_t* low;             // [M, ld]: hi, and lo behind it when split
+  int64_t ldx;
+  Rows rows;
+  int K, r, ld, split;
+};
+
+__device__ __forceinline__ float scale_of(const LowArgs& a, int ad) { return ad < 0 ? 0.f : a.scale ? a.scale[ad] : 1.f; }
+
+// u for rows by the 32 (MFMA 16x16x32, down as the row operand: a lane ends with four consecutive ranks of one row).
+// KSPLIT: the block's four waves share 32 rows and take every fourth k-step, joined in LDS in wave order — few rows; else
+// each wave has 32 rows of its own.  Bound by the stream of X; the adapter's k-steps come from L1 / L2.
+template <int DT, int RT, bool KSPLIT>
+__global__ __launch_bounds__(256) void adapter_low_kernel(const LowArgs a) {
+  __shared__ f32x4 part[KSPLIT ? 4 * RT * 2 * 64 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lg = lane >> 4, li = lane & 15;
+  const int64_t m0 = KSPLIT ? (int64_t)blockIdx.x * 32 : ((int64_t)blockIdx.x * 4 + wave) * 32;
+  if (m0 >= a.rows.M) return;
+  int ad[2], todo[2];
+  const uint16_t* x[2];
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi) {
+    const int64_t m = m0 + 16 * mi + li;
+    ad[mi] = todo[mi] = adapter_of(a.rows, m);
+    x[mi] = a.X + (m < a.rows.M ? m : m0) * a.ldx;
+  }
+  f32x4 res[RT][2];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) res[t][0] = res[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int cur = next_adapter<2>(todo); cur >= 0; cur = next_adapter<2>(todo)) {
+    f32x4 acc[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t][0] = acc[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const uint16_t* dn = a.down + (int64_t)cur * a.r * a.K;
+    const int steps = (a.K + 31) / 32;
+#pragma unroll 4
+    for (int s = KSPLIT ? wave : 0; s < steps; s += KSPLIT ? 4 : 1) {
+      const int kk = 32 * s + 8 * lg;
+      uint4 fx[2], fa[RT];
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi) fx[mi] = kk < a.K ? *reinterpret_cast<const uint4*>(x[mi] + kk) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        fa[t] = (kk < a.K && 16 * t + li < a.r) ? *reinterpret_cast<const uint4*>(dn + (int64_t)(16 * t + li) * a.K + kk)
+                                               : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int mi = 0; mi < 2; ++mi) acc[t][mi] = HT<DT>::mfma16(fa[t], fx[mi], acc[t][mi]);
+    }
+#pragma unroll
+    for (int mi = 0; mi < 2; ++mi) {
+      const bool mine = todo[mi] == cur;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) res[t][mi][i] = mine ? acc[t][mi][i] : res[t][mi][i];
+      todo[mi] = mine ? -1 : todo[mi];
+    }
+  }
+  if constexpr (KSPLIT) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi) part[((wave * RT + t) * 2 + mi) * 64 + lane] = res[t][mi];
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi) {
+        f32x4 v = part[(t * 2 + mi) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += part[((w * RT + t) * 2 + mi) * 64 + lane];
+        res[t][mi] = v;
+      }
+  }
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi) {
+    const int64_t m = m0 + 16 * mi + li;
+    const float sc = scale_of(a, ad[mi]);
+    if (m >= a.rows.M) continue;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (KSPLIT && (2 * t + mi) % 4 != wave) continue;
+      const int j = 16 * t + 4 * lg;
+      if (j >= a.r) continue;
+      f32x4 v = res[t][mi] * sc;
+      if (ad[mi] < 0) v = (f32x4){0.f, 0.f, 0.f, 0.f};
+      uint16_t* p = a.low + m * a.ld + j;
+      const uint2 hi = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
+      *reinterpret_cast<uint2*>(p) = hi;
+      if (a.split) {
+        f32x4 h;
+        h[0] = HT<DT>::to_f((uint16_t)(hi.x & 0xffffu)); h[1] = HT<DT>::to_f((uint16_t)(hi.x >> 16));
+        h[2] = HT<DT>::to_f((uint16_t)(hi.y & 0xffffu)); h[3] = HT<DT>::to_f((uint16_t)(hi.y >> 16));
+        v -= h;
+        *reinterpret_cast<uint2*>(p + a.r) = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
+      }
+    }
+  }
+}
+
+// u for rows that each have an adapter of their own: one block per row, a wave per rank in turn, lanes along K
+template <int DT>
+__global__ __launch_bounds__(256) void adapter_low_row_kernel(const LowArgs a) {
+  const int64_t m = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int ad = adapter_of(a.rows, m);
+  const float sc = scale_of(a, ad);
+  const uint16_t* x = a.X + m * a.ldx;
+#pragma unroll 4
+  for (int j = wave; j < a.r; j += 4) {
+    float s = 0.f;
+    if (ad >= 0) {
+      const uint16_t* dn = a.down + ((int64_t)ad * a.r + j) * a.K;
+      for (int k = 8 * lane; k < a.K; k += 512) {
+        float p[8], q[8];
+        unpack8<DT>(*reinterpret_cast<const uint4*>(x + k), p);
+        unpack8<DT>(*reinterpret_cast<const uint4*>(dn + k), q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(p[i], q[i], s);
+      }
+      s = wave_sum(s) * sc;
+    }
+    if (lane == 0) {
+      const uint16_t hi = HT<DT>::from_f(s);
+      a.low[m * a.ld + j] = hi;
+      if (a.split) a.low[m * a.ld + a.r + j] = HT<DT>::from_f(s - HT<DT>::to_f(hi));
+    }
+  }
+}
+
+// [n, R, C] -> [n, C, R] of two stacks in one launch (blockIdx.z = which): 32 x 32 tiles through LDS
+struct TransposeArgs {
+  const uint16_t* in[2];
+  uint16_t* out[2];
+  int R[2], C[2];
+};
+__global__ __launch_bounds__(256) void adapter_transpose_kernel(const TransposeArgs a) {
+  __shared__ uint16_t tile[32][33];
+  const int z = blockIdx.z, R = a.R[z], C = a.C[z];
+  const int tc = (C + 31) / 32, tr = (R + 31) / 32;
+  const uint16_t* in = a.in[z] + (int64_t)blockIdx.y * R * C;
+  uint16_t* out = a.out[z] + (int64_t)blockIdx.y * R * C;
+  for (int t = blockIdx.x; t < tc * tr; t += gridDim.x) {
+    const int r0 = t / tc * 32, c0 = t % tc * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    for (int i = y; i < 32; i += 8)
+      if (r0 + i < R && c0 + x < C) tile[i][x] = in[(int64_t)(r0 + i) * C + c0 + x];
+    __syncthreads();
+    for (int i = y; i < 32; i += 8)
+      if (c0 + i < C && r0 + x < R) out[(int64_t)(c0 + i) * R + r0 + x] = tile[x][i];
+    __syncthreads();
+  }
+}
+
+// sum over the rows of adapter blockIdx.y of low[m]^T x[m], for two pairs in one launch: (t, a) -> ddown and (u, dy) -> dup.
+// A block owns 128 columns of x and all ranks; tiles of 64 rows pass through LDS row-major, both operands are read transposed
+// (a row that is not this adapter's is staged as zeros on BOTH sides); the hi and lo halves of low meet in the same fp32
+// accumulators.  Rows: only [first, last] of the adapter, cut into gridDim.z parts.
+struct OuterArgs {
+  const uint16_t *x[2], *low[2];
+  float* part[2];  // [parts][n][r][C]
+  int64_t ldx[2];
+  int C[2];
+  Rows rows;
+  int r, ld, ct0;  // ct0: column tiles of the first pair
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+// operand of a 16x16x32 MFMA whose contraction index runs over LDS rows [r0, r0 + 32): lane (lg, i) gets column c0 + i of rows
+// r0 + 8 lg .. + 8
+__device__ __forceinline__ uint4 read_tr16(const uint16_t* tile, int pitch, int r0, int c0, int lane) {
+  const int m = lane & 15, lg = lane >> 4;
+  const uint16_t* p = tile + (r0 + 8 * lg + (m >> 2)) * pitch + c0 + 4 * (m & 3);
+  const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p));
+  const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * pitch)));
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+template <int DT, int RT>
+__global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
+  constexpr int MR = 64, XP = 128 + 8, LP = 32 * RT + 24;  // (the lo half of a rank of 8 is read up to column 8 + 16)
+  constexpr int NX = 4, NL = RT;                          // 16-byte chunks a thread stages per tile
+  __shared__ __attribute__((aligned(16))) uint16_t xs[MR * XP];
+  __shared__ __attribute__((aligned(16))) uint16_t ls[MR * LP];
+  __shared__ int range[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  const int z = (int)blockIdx.x >= a.ct0;
+  const int c0 = ((int)blockIdx.x - (z ? a.ct0 : 0)) * 128, C = a.C[z], who = blockIdx.y;
+  // rows of this adapter
+  if (tid == 0) {
+    range[0] = 0x7fffffff;
+    range[1] = -1;
+  }
+  __syncthreads();
+  const int64_t G = (a.rows.M + a.rows.rpi - 1) / a.rows.rpi;
+  int lo = 0x7fffffff, hi = -1;
+  for (int64_t i = tid; i < G; i += 256)
+    if (a.rows.index[i] == who) {
+      lo = lo < (int)i ? lo : (int)i;
+      hi = (int)i;
+    }
+  if (hi >= 0) {
+    atomicMin(&range[0], lo);
+    atomicMax(&range[1], hi);
+  }
+  for (int i = tid; i < MR * LP / 2; i += 256) reinterpret_cast<uint32_t*>(ls)[i] = 0u;  // columns behind 2 r are never staged
+  __syncthreads();
+  f32x4 acc[RT][2];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) acc[t][0] = acc[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (range[1] >= 0) {
+    const int64_t m_lo = (int64_t)range[0] * a.rows.rpi;
+    int64_t m_hi = ((int64_t)range[1] + 1) * a.rows.rpi;
+    if (m_hi > a.rows.M) m_hi = a.rows.M;
+    const int64_t tiles = (m_hi - m_lo + MR - 1) / MR, per = (tiles + gridDim.z - 1) / gridDim.z;
+    const int64_t t_lo = blockIdx.z * per, t_hi = t_lo + per < tiles ? t_lo + per : tiles;
+    const int lc = 2 * a.r / 8;  // 16-byte chunks of a row of low
+    uint4 xr[NX], lr[NL];
+    auto fetch = [&](int64_t t) {
+      const int64_t m0 = m_lo + t * MR;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int id = tid + 256 * i, c = c0 + (id & 15) * 8;
+        const int64_t m = m0 + (id >> 4);
+        xr[i] = make_uint4(0, 0, 0, 0);
+        if (c < C && adapter_of(a.rows, m) == who) xr[i] = *reinterpret_cast<const uint4*>(a.x[z] + m * a.ldx[z] + c);
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int id = tid + 256 * i, row = id / lc;
+        const int64_t m = m0 + row;
+        lr[i] = make_uint4(0, 0, 0, 0);
+        if (row < MR && adapter_of(a.rows, m) == who) lr[i] = *reinterpret_cast<const uint4*>(a.low[z] + m * a.ld + (id - row * lc) * 8);
+      }
+    };
+    if (t_lo < t_hi) fetch(t_lo);
+    for (int64_t t = t_lo; t < t_hi; ++t) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int id = tid + 256 * i;
+        *reinterpret_cast<uint4*>(xs + (id >> 4) * XP + (id & 15) * 8) = xr[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int id = tid + 256 * i, row = id / lc;
+        if (row < MR) *reinterpret_cast<uint4*>(ls + row * LP + (id - row * lc) * 8) = lr[i];
+      }
+      __syncthreads();
+      if (t + 1 < t_hi) fetch(t + 1);
+#pragma unroll
+      for (int k0 = 0; k0 < MR; k0 += 32) {
+        uint4 fx[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) fx[c] = read_tr16(xs, XP, k0, wave * 32 + 16 * c, lane);
+#pragma unroll
+        for (int q = 0; q < RT; ++q) {
+          const uint4 fh = read_tr16(ls, LP, k0, 16 * q, lane), fl = read_tr16(ls, LP, k0, a.r + 16 * q, lane);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[q][c] = HT<DT>::mfma16(fl, fx[c], HT<DT>::mfma16(fh, fx[c], acc[q][c]));
+        }
+      }
+    }
+  }
+  // lane: column c0 + .. + li, ranks 16 q + 4 lg + i
+  float* out = a.part[z] + ((int64_t)blockIdx.z * gridDim.y + who) * a.r * C;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int col = c0 + wave * 32 + 16 * c + li;
+    if (col >= C) continue;
+#pragma unroll
+    for (int q = 0; q < RT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 16 * q + 4 * lg + i;
+        if (j < a.r) out[(int64_t)j * C + col] = acc[q][c][i];
+      }
+  }
+}
+
+// the sum of the parts in order: ddown [n, r, K] as it lies, dup [n, N, r] transposed
+__global__ __launch_bounds__(256) void adapter_join_kernel(const float* p0, const float* p1, float* ddown, float* dup, int n, int r, int K,
+                                                           int N, int parts) {
+  const int64_t s0 = (int64_t)n * r * K, s1 = (int64_t)n * r * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < s0 + s1; i += (int64_t)gridDim.x * 256) {
+    const bool first = i < s0;
+    const int64_t at = first ? i : i - s0, plane = first ? s0 : s1;
+    const float* p = (first ? p0 : p1) + at;
+    float s = p[0];
+    for (int q = 1; q < parts; ++q) s += p[(int64_t)q * plane];
+    if (first) {
+      ddown[at] = s;
+    } else {
+      const int64_t row = at / N;  // (adapter, rank)
+      dup[(row / r * N + (at - row * N)) * r + row % r] = s;
+    }
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------------------------------------
+template <int DT>
+int launch_low(const LowArgs& a, hipStream_t st) {
+  // few rows with an adapter each: a matrix tile would run once per row, a block per row reads what the row needs
+  if (a.rows.rpi == 1 && a.rows.M <= 256 && a.rows.n > 1) {
+    hipLaunchKernelGGL((adapter_low_row_kernel<DT>), dim3((unsigned)a.rows.M), dim3(256), 0, st, a);
+    MIMO_LAUNCH_CHECK();
+    return MIMO_OK;
+  }
+  const int rt = (a.r + 15) / 16;
+  const int64_t m32 = (a.rows.M + 31) / 32;
+  const bool ksplit = m32 < 4 * (int64_t)cu_count();  // one wave per 32 rows would leave SIMDs empty
+  const int64_t nwg = ksplit ? m32 : (m32 + 3) / 4;
+  if (nwg > 0x7fffffff) return MIMO_EINVAL;
+#define LOW(RT)                                                                                                                  \
+  do {                                                                                                                           \
+    if (ksplit) hipLaunchKernelGGL((adapter_low_kernel<DT, RT, true>), dim3((unsigned)nwg), dim3(256), 0, st, a);                \
+    else hipLaunchKernelGGL((adapter_low_kernel<DT, RT, false>), dim3((unsigned)nwg), dim3(256), 0, st, a);                      \
+  } while (0)
+  if (rt == 1) LOW(1);
+  else if (rt == 2) LOW(2);
+  else if (rt <= 4) LOW(4);
+  else LOW(8);
+#undef LOW
+  MIMO_LAUNCH_CHECK();
+  return MIMO_OK;
+}
+
+template <int DT, int NR>
+int launch_tiles(GemmArgs& g, hipStream_t st) {
+  // the tile choice of mimo_gemm (gemm_conv.hip launch_nr), without split-K
+  const int cus = cu_count();
+  const int64_t m256 = (g.M + 255) / 256;
+  const int tn_s = (g.N + 32 * NR - 1) / (32 * NR), tn_xl = (g.N + 64 * NR - 1) / (64 * NR);
+  if (g.N > 32 * NR && m256 * tn_xl >= 160) {
+    g.tiles_n = tn_xl;
+    auto cost = [&](int bm) { return ((((g.M + bm - 1) / bm) * tn_xl + cus - 1) / cus) * (int64_t)(bm + 24); };
+    int bm = 256;
+    if (cost(192) < cost(bm)) bm = 192;
+    if (cost(128) < cost(bm)) bm = 128;
+    const int64_t nwg = ((g.M + bm - 1) / bm) * tn_xl;
+    if (nwg > 0x7fffffff) return MIMO_EINVAL;
+    if (NR == 5 && bm == 256 && nwg >= 3 * (int64_t)cus && g.nkt >= 2 && g.nkt <= 20) {
+      g.ntiles = (unsigned)nwg;
+      hipLaunchKernelGGL((gemm_dense_persist_kernel<DT, NR, 2, 4, 8, 3>), dim3((unsigned)cus), dim3(512), 0, st, g);
+    } else if (bm == 256) {
+      hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 4, 2, 8, 3>), dim3((unsigned)nwg), dim3(512), 0, st, g);
+    } else if (bm == 192) {
+      hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 4, 2, 6, 3>), dim3((unsigned)nwg), dim3(512), 0, st, g);
+    } else {
+      hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 4, 2, 4, 3>), dim3((unsigned)nwg), dim3(512), 0, st, g);
+    }
+  } else {
+    g.tiles_n = tn_s;
+    const int64_t nwg = ((g.M + 127) / 128) * tn_s;
+    if (nwg > 0x3fffffff) return MIMO_EINVAL;
+    if (nwg <= cus) {
+      const int64_t nwg64 = ((g.M + 63) / 64) * tn_s;
+      hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 2, 2, 2, 3>), dim3((unsigned)nwg64), dim3(256), 0, st, g);
+    } else {
+      hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 2, 2, 4, 3>), dim3((unsigned)nwg), dim3(256), 0, st, g);
+    }
+  }
+  MIMO_LAUNCH_CHECK();
+  return MIMO_OK;
+}
+
+template <int DT>
+int launch_gemm(GemmArgs g, hipStream_t st) {
+  // operands are addressed with 32-bit byte offsets: more rows than that go in several launches
+  const int64_t M = g.M, most = g.lda > 0 ? (0x7fffffffLL / (2 * g.lda) - 1) / 256 * 256 : M;
+  const bool of32 = g.flags & MIMO_EPI_OUT_F32, rf32 = g.flags & MIMO_EPI_RES_F32;
+  for (int64_t r0 = 0; r0 < M; r0 += most) {
+    GemmArgs c = g;
+    c.M = M - r0 < most ? M - r0 : most;
+    c.A = g.A + r0 * g.lda;
+    c.out = (char*)g.out + r0 * g.ldo * (of32 ? 4 : 2);
+    if (g.res) c.res = (const char*)g.res + r0 * g.ldr * (rf32 ? 4 : 2);
+    c.ad_row0 = r0;
+    c.ad_low = g.ad_low + r0 * g.ad_ld;
+    c.a_bytes = (unsigned)(((c.M - 1) * c.lda + c.K) * 2);
+    const int64_t tn8 = (c.N + 255) / 256, nt8 = ((c.M + 255) / 256) * tn8;
+    int rc;
+    if ((c.K % 128) == 0 && tn8 * 256 - c.N <= c.N / 12 && nt8 >= 128 && nt8 <= 0x7fffffff) {
+      c.tiles_n = (int)tn8;
+      c.ntiles = (unsigned)G8_GM;
+      hipLaunchKernelGGL((gemm8_kernel<DT, 3>), dim3((unsigned)nt8), dim3(512), 0, st, c);
+      const hipError_t e = hipGetLastError();
+      rc = e == hipSuccess ? MIMO_OK : (int)e;
+    } else {
+      rc = c.N % 160 == 0 ? launch_tiles<DT, 5>(c, st) : launch_tiles<DT, 4>(c, st);
+    }
+    if (rc) return rc;
+  }
+  return MIMO_OK;
+}
+
+// checks shared by both entries
+int check(const mimo_adapter_params* p, int64_t M, int N, int K) {
+  if (!p || M <= 0 || M >= 0x7fffffffLL || N <= 0 || K <= 0 || (N & 7) || (K & 7) || (int64_t)N * K >= 0x40000000LL) return MIMO_EINVAL;
+  if (!p->down || !p->up || !p->index || p->count <= 0 || p->rank <= 0 || p->rank > 128 || (p->rank & 7) || p->rows_per_index <= 0)
+    return MIMO_EINVAL;
+  if (p->count > 65535 || !aligned16(p->down) || !aligned16(p->up) || (reinterpret_cast<uintptr_t>(p->index) & 3u)) return MIMO_EINVAL;
+  return MIMO_OK;
+}
+
+GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t ldo, int64_t M, int N, int K, const Rows& rows,
+                   const uint16_t* low, int ld, int cols, const uint16_t* up, int rank) {
+  GemmArgs g{};
+  g.A = (const uint16_t*)A; g.W = (const uint16_t*)W; g.out = out;
+  g.lda = lda; g.ldw = K; g.ldo = ldo; g.M = M; g.N = N; g.K = K; g.out_scale = 1.f;
+  g.rows_per_img = 1; g.ldib = N; g.ln_rows_per_frame = 1; g.ln_pe_frames = 1;
+  g.nkt = (K + BK - 1) / BK;
+  g.w_bytes = (unsigned)((int64_t)N * K * 2);
+  g.flags = F_STAGGER;
+  g.ad_index = rows.index; g.ad_rpi = rows.rpi; g.ad_n = rows.n;
+  g.ad_low = low; g.ad_up = up; g.ad_rank = rank; g.ad_cols = cols; g.ad_ld = ld;
+  return g;
+}
+
+template <int DT>
+int forward(GemmArgs g, const LowArgs& la, hipStream_t st) {
+  if (const int rc = launch_low<DT>(la, st)) return rc;
+  return launch_gemm<DT>(g, st);
+}
+
+// workspace of the backward, in bytes: t [M, 2 r] | up^T | down^T | parts of ddown | parts of dup
+struct BackwardPlan {
+  int parts;
+  size_t t, upt, downt, p0, p1, total;
+};
+BackwardPlan backward_plan(const mimo_adapter_params* p, int64_t M, int N, int K) {
+  BackwardPlan b{};
+  const int64_t n = p->count, r = p->rank;
+  const int64_t blocks = n * ((N + 127) / 128 + (K + 127) / 128), tiles = (M + 63) / 64;
+  int64_t parts = (2 * (int64_t)cu_count() + blocks - 1) / blocks;  // two blocks per CU; a part keeps at least four row tiles
+  if (parts > tiles / 4) parts = tiles / 4;
+  if (parts > 256) parts = 256;
+  b.parts = parts < 1 ? 1 : (int)parts;
+  auto up16 = [](size_t x) { return (x + 15) / 16 * 16; };
+  b.t = up16((size_t)M * 2 * r * 2);
+  b.upt = up16((size_t)n * r * N * 2);
+  b.downt = up16((size_t)n * r * K * 2);
+  b.p0 = up16((size_t)b.parts * n * r * K * 4);
+  b.p1 = up16((size_t)b.parts * n * r * N * 4);
+  b.total = b.t + b.upt + b.downt + b.p0 + b.p1;
+  return b;
+}
+
+template <int DT>
+int backward(const void* dY, int64_t ldy, const void* A, int64_t lda, const void* Wt, void* dA, int64_t ldda, int64_t M, int N, int K,
+             const mimo_adapter_params* p, const void* low, float* ddown, float* dup, char* ws, hipStream_t st) {
+  const BackwardPlan b = backward_plan(p, M, N, K);
+  const int n = p->count, r = p->rank;
+  uint16_t* t = (uint16_t*)ws;
+  uint16_t* upt = (uint16_t*)(ws + b.t);
+  uint16_t* downt = (uint16_t*)(ws + b.t + b.upt);
+  float* p0 = (float*)(ws + b.t + b.upt + b.downt);
+  float* p1 = (float*)((char*)p0 + b.p0);
+  const Rows rows{p->index, M, p->rows_per_index, n};
+  TransposeArgs ta{{(const uint16_t*)p->up, (const uint16_t*)p->down}, {upt, downt}, {N, r}, {r, K}};
+  const int tiles = ((N > K ? N : K) + 31) / 32 * ((r + 31) / 32);
+  hipLaunchKernelGGL(adapter_transpose_kernel, dim3((unsigned)tiles, (unsigned)n, 2u), dim3(256), 0, st, ta);
+  MIMO_LAUNCH_CHECK();
+  const LowArgs la{(const uint16_t*)dY, upt, p->scale, t, ldy, rows, N, r, 2 * r, 1};
+  if (const int rc = launch_low<DT>(la, st)) return rc;
+  if (dA) {
+    GemmArgs g = gemm_args(dY, ldy, Wt, dA, ldda, M, K, N, rows, t, 2 * r, r, downt, r);
+    if (const int rc = launch_gemm<DT>(g, st)) return rc;
+  }
+  OuterArgs oa{{(const uint16_t*)A, (const uint16_t*)dY}, {t, (const uint16_t*)low}, {p0, p1}, {lda, ldy}, {K, N}, rows, r, 2 * r,
+               (K + 127) / 128};
+  const dim3 grid((unsigned)((K + 127) / 128 + (N + 127) / 128), (unsigned)n, (unsigned)b.parts);
+  const int rt = (r + 15) / 16;
+  if (rt == 1) hipLaunchKernelGGL((adapter_outer_kernel<DT, 1>), grid, dim3(256), 0, st, oa);
+  else if (rt == 2) hipLaunchKernelGGL((adapter_outer_kernel<DT, 2>), grid, dim3(256), 0, st, oa);
+  else if (rt <= 4) hipLaunchKernelGGL((adapter_outer_kernel<DT, 4>), grid, dim3(256), 0, st, oa);
+  else hipLaunchKernelGGL((adapter_outer_kernel<DT, 8>), grid, dim3(256), 0, st, oa);
+  MIMO_LAUNCH_CHECK();
+  const int64_t total = (int64_t)n * r * (N + K), nwg = (total + 255) / 256;
+  hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)(nwg > 2048 ? 2048 : nwg)), dim3(256), 0, st, p0, p1, ddown, dup, n, r, K, N,
+                     b.parts);
+  MIMO_LAUNCH_CHECK();
+  return MIMO_OK;
+}
+
+}  // namespace
+
+extern "C" int mimo_adapter_gemm(int dtype, const void* A, int64_t lda, const void* W, void* out, int64_t ldo, int64_t M, int N, int K,
+                                 const float* bias, const void* residual, int64_t ldr, unsigned flags, const mimo_adapter_params* p,
+                                 void* low, int low_split, void* stream) {
+  if (const int rc = check(p, M, N, K)) return rc;
+  if (!A || !W || !out || !low || (lda & 7) || (ldo & 3) || (residual && (ldr & 3)) || !aligned16(A) || !aligned16(W) || !aligned16(out) ||
+      !aligned16(low) || lda < 0 || lda > 0x100000)
+    return MIMO_EINVAL;
+  if (flags & ~(MIMO_EPI_OUT_F32 | MIMO_EPI_RES_F32)) return MIMO_EINVAL;
+  const bool of32 = flags & MIMO_EPI_OUT_F32;
+  if (of32 && !low_split) return MIMO_EINVAL;
+  const Rows rows{p->index, M, p->rows_per_index, p->count};
+  const int ld = low_split ? 2 * p->rank : p->rank;
+  GemmArgs g = gemm_args(A, lda, W, out, ldo, M, N, K, rows, (const uint16_t*)low, ld, of32 ? 2 * p->rank : p->rank,
+                         (const uint16_t*)p->up, p->rank);
+  g.bias = bias; g.res = residual; g.ldr = ldr;
+  g.flags |= flags;
+  const LowArgs la{(const uint16_t*)A, (const uint16_t*)p->down, p->scale, (uint16_t*)low, lda, rows, K, p->rank, ld, low_split ? 1 : 0};
+  if (dtype == MIMO_F16) return forward<MIMO_F16>(g, la, (hipStream_t)stream);
+  if (dtype == MIMO_BF16) return forward<MIMO_BF16>(g, la, (hipStream_t)stream);
+  return MIMO_EDTYPE;
+}
+
+extern "C" size_t mimo_adapter_gemm_backward_workspace(const mimo_adapter_params* p, int64_t M, int N, int K) {
+  return check(p, M, N, K) == MIMO_OK ? backward_plan(p, M, N, K).total : 0;
+}
+
+extern "C" int mimo_adapter_gemm_backward(int dtype, const void* dY, int64_t ldy, const void* A, int64_t lda, const void* Wt, void* dA,
+                                          int64_t ldda, int64_t M, int N, int K, const mimo_adapter_params* p, const void* low,
+                                          float* ddown, float* dup, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check(p, M, N, K)) return rc;
+  if (!dY || !A || !low || !ddown || !dup || !workspace || (dA && !Wt) || (ldy & 7) || (lda & 7) || (ldda & 3) || lda < 0 || ldy < 0 || ldy > 0x100000 ||
+      !aligned16(dY) || !aligned16(A) || !aligned16(Wt) || !aligned16(dA) || !aligned16(low) || !aligned16(ddown) || !aligned16(dup) ||
+      !aligned16(workspace) || workspace_bytes < backward_plan(p, M, N, K).total)
+    return MIMO_EINVAL;
+  if (dtype == MIMO_F16)
+    return backward<MIMO_F16>(dY, ldy, A, lda, Wt, dA, ldda, M, N, K, p, low, ddown, dup, (char*)workspace, (hipStream_t)stream);
+  if (dtype == MIMO_BF16)
+    return backward<MIMO_BF16>(dY, ldy, A, lda, Wt, dA, ldda, M, N, K, p, low, ddown, dup, (char*)workspace, (hipStream_t)stream);
+  return MIMO_EDTYPE;
+}

@@ -47,6 +47,10 @@ class CrossAttentionParams(ctypes.Structure):  # mimo_cross_attention_params
                [("kv_len", c_vp), ("mask", c_vp), ("mask_row", c_i64)]
 
 
+class AdapterParams(ctypes.Structure):  # mimo_adapter_params
+    _fields_ = [("down", c_vp), ("up", c_vp), ("scale", c_vp), ("index", c_vp), ("rows_per_index", c_i64), ("count", c_i), ("rank", c_i)]
+
+
 # name -> argtypes, mirrors include/mimo_hip.h one to one
 SIGNATURES = {
     "mimo_version": [],
@@ -57,6 +61,11 @@ SIGNATURES = {
                   c_sz, c_vp],
     "mimo_gemm_ext": [c_i, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i, c_i, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_f, c_u,
                       c_vp, c_sz, ctypes.POINTER(EpilogueExt), c_vp],
+    "mimo_adapter_gemm": [c_i, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i, c_i, c_vp, c_vp, c_i64, c_u, ctypes.POINTER(AdapterParams),
+                          c_vp, c_i, c_vp],
+    "mimo_adapter_gemm_backward_workspace": [ctypes.POINTER(AdapterParams), c_i64, c_i, c_i],
+    "mimo_adapter_gemm_backward": [c_i, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i, c_i, ctypes.POINTER(AdapterParams),
+                                   c_vp, c_vp, c_vp, c_vp, c_sz, c_vp],
     "mimo_conv2d": [c_i, c_vp, c_vp, c_vp, c_vp, ctypes.POINTER(ConvParams), c_vp, c_vp, c_vp, c_f, c_u, c_vp, c_sz, c_vp],
     "mimo_conv2d_ext": [c_i, c_vp, c_vp, c_vp, c_vp, ctypes.POINTER(ConvParams), c_vp, c_vp, c_vp, c_f, c_u, c_vp, c_sz,
                         ctypes.POINTER(EpilogueExt), c_vp],
@@ -110,7 +119,7 @@ _lib = None
 
 
 RESTYPES = {"mimo_workspace_bytes": c_sz, "mimo_cross_attention_workspace": c_sz,
-            "mimo_cross_attention_backward_workspace": c_sz}  # every other entry point returns int (0 or an error code)
+            "mimo_cross_attention_backward_workspace": c_sz, "mimo_adapter_gemm_backward_workspace": c_sz}  # every other entry point returns int (0 or an error code)
 
 
 def load():

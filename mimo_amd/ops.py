@@ -327,6 +327,134 @@ def gemm(a, w, *, bias=None, img_bias=None, rows_per_img=0, residual=None, out_f
     return out, ln_out
 
 
+def _require(ok, what):
+    if not ok:
+        raise L.MimoHipError(what)
+
+
+class _on_device:
+    """The launch happens on the tensors' own device, whatever the current one is."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+        return False
+
+
+def _stride(t, i):
+    """Element stride of axis i, 0 where the axis has one entry (its stride is then arbitrary)."""
+    return t.stride(i) if t.shape[i] > 1 else 0
+
+
+def _ld(t):
+    """Row pitch of a matrix in elements (0: every row is the same one)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows_ok(t, name):
+    """Rows of whole 16-byte chunks: what the kernels' wide loads need."""
+    _require(t.stride(-1) == 1 or t.shape[-1] <= 1 or t.numel() == 0, f"{name}: the last axis is contiguous")
+    _require(t.data_ptr() % 16 == 0 and all(_stride(t, i) % 8 == 0 for i in range(t.dim() - 1)),
+             f"{name}: 16-byte aligned rows (strides {t.stride()})")
+
+
+def _adapter_params(a, w, down, up, index, rows_per_index, scale, w_shape):
+    """Checks the operands of an adapter product and lays the adapters down for the C-ABI; returns (params, tensors they point at)."""
+    dt_code(a.dtype)
+    _require(a.dim() == 2 and w.dim() == 2 and down.dim() == 3 and up.dim() == 3, "a [M, K], w [N, K], down [S, r, K], up [S, N, r]")
+    M, K = a.shape
+    S, r, _ = down.shape
+    N = up.shape[1]
+    _require(down.shape == (S, r, K) and up.shape == (S, N, r) and w.shape == w_shape(N, K),
+             f"a {tuple(a.shape)}, w {tuple(w.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)} do not fit together")
+    _require(S > 0 and 0 < r <= 128 and r % 8 == 0, f"{S} adapters of rank {r}: ranks are multiples of 8 up to 128 (packing.pack_adapters pads)")
+    _require(N % 8 == 0 and K % 8 == 0 and N > 0 and K > 0 and N * K < 1 << 30, f"widths {N}, {K}: multiples of 8")
+    for t, name in ((a, "a"), (w, "w"), (down, "down"), (up, "up")):
+        _require(t.device == a.device and t.dtype == a.dtype, f"{name}: {t.dtype} on {t.device}, a is {a.dtype} on {a.device}")
+    for t, name in ((w, "w"), (down, "down"), (up, "up")):
+        _require(t.is_contiguous() and t.data_ptr() % 16 == 0, f"{name}: contiguous, 16-byte aligned")
+    _rows_ok(a, "a")
+    rows_per_index = int(rows_per_index)
+    _require(rows_per_index > 0, f"rows_per_index {rows_per_index}")
+    _require(index.dim() == 1 and index.dtype == torch.int32 and index.device == a.device and index.is_contiguous() and
+             index.numel() >= (M + rows_per_index - 1) // rows_per_index,
+             f"index: contiguous int32 on {a.device}, an entry per {rows_per_index} of {M} rows")
+    if scale is not None:
+        _require(scale.shape == (S,) and scale.dtype == torch.float32 and scale.device == a.device and scale.is_contiguous(),
+                 f"scale: contiguous fp32 [{S}] on {a.device}")
+    _chk(a, "a")
+    return L.AdapterParams(down.data_ptr(), up.data_ptr(), _ptr(scale), index.data_ptr(), rows_per_index, S, r)
+
+
+def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=None, residual=None, out_f32=False, want_low=False):
+    """out[M, N] = a @ w^T + bias + residual + (scale[i] a @ down[i]^T) @ up[i]^T, i = index[m // rows_per_index]: a shared projection
+    with the low-rank adapter of each row's request added in the same pass over the output.
+
+    a: half [M, K], row-strided allowed; w: half [N, K]; down: half [S, r, K], up: half [S, N, r] (r a multiple of 8 up to 128:
+    packing.pack_adapters pads and stacks checkpoints of any rank); index: int32 device tensor, one entry per rows_per_index
+    consecutive rows, in any order; an entry outside [0, S) (use -1) means no adapter.  scale: fp32 [S] (None: 1); bias: fp32 [N];
+    residual: fp32 or half [M, N].  Returns half, or fp32 with out_f32.
+    want_low: returns (out, low), low half [M, 2 r] = the rows' scaled low-rank values as hi | lo halves, for the backward."""
+    p = _adapter_params(a, w, down, up, index, rows_per_index, scale, lambda N, K: (N, K))
+    M, K = a.shape
+    N, r = w.shape[0], p.rank
+    if bias is not None:
+        _require(bias.shape == (N,) and bias.dtype == torch.float32 and bias.device == a.device and bias.is_contiguous(), f"bias: fp32 [{N}]")
+    if residual is not None:
+        _require(residual.shape == (M, N) and residual.device == a.device and residual.dtype in (torch.float32, a.dtype) and
+                 (residual.stride(1) == 1 or N == 1) and _stride(residual, 0) % 4 == 0 and residual.data_ptr() % 16 == 0,
+                 f"residual: fp32 or {a.dtype} [{M}, {N}], 16-byte aligned rows")
+    split = bool(want_low or out_f32)
+    with _on_device(a.device):
+        out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_f32 else a.dtype)
+        low = torch.empty((M, 2 * r if split else r), device=a.device, dtype=a.dtype)
+        if M:
+            fl = 2 * M * N * K + 2 * M * r * (N + K)
+            _count(fl)
+            flags = (L.EPI_OUT_F32 if out_f32 else 0) | (L.EPI_RES_F32 if residual is not None and residual.dtype == torch.float32 else 0)
+            with _Bracket("gemm_kernel", fl, _nbytes(a, w, out, residual, down, up), f"adapter_gemm M{M} N{N} K{K} r{r}"):
+                L.call("mimo_adapter_gemm", dt_code(a.dtype), a.data_ptr(), _ld(a), w.data_ptr(), out.data_ptr(), N, M, N, K,
+                       _ptr(bias), _ptr(residual), 0 if residual is None else _ld(residual), flags, ctypes.byref(p), low.data_ptr(),
+                       int(split), _stream())
+    return (out, low) if want_low else out
+
+
+def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=1, scale=None, want_da=True):
+    """(da, ddown, dup) of adapter_gemm with w frozen, from the gradient dout half [M, N] of its result (row-strided allowed), its
+    operands, w_t = the transposed weight [K, N] (contiguous, laid out once) and its low (want_low=True).  da: half [M, K] (None
+    with want_da=False); ddown fp32 [S, r, K] and dup fp32 [S, N, r] are summed over the rows of each adapter in a fixed order:
+    the same bits on every run, zeros for an adapter without rows.  (The residual's gradient is dout, the bias's its column sum.)"""
+    p = _adapter_params(a, w_t, down, up, index, rows_per_index, scale, lambda N, K: (K, N))
+    M, K = a.shape
+    N, r, S = up.shape[1], p.rank, p.count
+    _require(dout.shape == (M, N) and dout.dtype == a.dtype and dout.device == a.device, f"dout: {a.dtype} [{M}, {N}]")
+    _rows_ok(dout, "dout")
+    _require(low.shape == (M, 2 * r) and low.dtype == a.dtype and low.device == a.device and low.is_contiguous() and
+             low.data_ptr() % 16 == 0, f"low: the forward's [{M}, {2 * r}] (want_low=True)")
+    with _on_device(a.device):
+        da = torch.empty((M, K), device=a.device, dtype=a.dtype) if want_da else None
+        if not M:
+            return da, torch.zeros(down.shape, device=a.device), torch.zeros(up.shape, device=a.device)
+        ddown = torch.empty((S, r, K), device=a.device, dtype=torch.float32)
+        dup = torch.empty((S, N, r), device=a.device, dtype=torch.float32)
+        fl = (2 * M * N * K if want_da else 0) + 2 * M * r * (2 * N + 2 * K)
+        _count(fl)
+        nb = L.load().mimo_adapter_gemm_backward_workspace(ctypes.byref(p), M, N, K)
+        ws = torch.empty(((nb + 3) // 4,), device=a.device, dtype=torch.float32)
+        with _Bracket("gemm_kernel", fl, _nbytes(dout, a, w_t, da, ddown, dup), f"adapter_gemm_backward M{M} N{N} K{K} r{r}"):
+            L.call("mimo_adapter_gemm_backward", dt_code(a.dtype), dout.data_ptr(), _ld(dout), a.data_ptr(), _ld(a),
+                   w_t.data_ptr(), _ptr(da), K, M, N, K, ctypes.byref(p), low.data_ptr(), ddown.data_ptr(), dup.data_ptr(), ws.data_ptr(),
+                   nb, _stream())
+    return da, ddown, dup
+
+
 # The fused feed-forward kernel exists for the 320-wide level only (its K = 320 operand lives in registers).  Like every
 # kernel choice of this package the decision depends on the layer's width and on a fixed row threshold, never on how many
 # images share the launch beyond it (FF_FUSED_MIN_ROWS: below it the panel count cannot fill the chip).
@@ -817,32 +945,6 @@ def attention(q, k, v, heads, *, k2=None, v2=None, seg2_first_batch=0, scale=Non
     return out
 
 
-def _require(ok, what):
-    if not ok:
-        raise L.MimoHipError(what)
-
-
-class _on_device:
-    """The launch happens on the tensors' own device, whatever the current one is."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-        return False
-
-
-def _stride(t, i):
-    """Element stride of axis i, 0 where the axis has one entry (its stride is then arbitrary)."""
-    return t.stride(i) if t.shape[i] > 1 else 0
-
-
 def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
     """Checks the operands of a cross attention and lays their geometry down for the C-ABI."""
     dt_code(q.dtype)
@@ -872,13 +974,6 @@ def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
         p.mask, p.mask_row = mask.data_ptr(), _stride(mask, 0)
     _chk(q, "q")
     return p
-
-
-def _rows_ok(t, name):
-    """Rows of whole 16-byte chunks: what the kernels' wide loads need."""
-    _require(t.stride(-1) == 1 or t.shape[-1] <= 1 or t.numel() == 0, f"{name}: the last axis is contiguous")
-    _require(t.data_ptr() % 16 == 0 and all(_stride(t, i) % 8 == 0 for i in range(t.dim() - 1)),
-             f"{name}: 16-byte aligned rows (strides {t.stride()})")
 
 
 def cross_attention(q, k, v, heads, *, kv_heads=None, kv_len=None, mask=None, scale=None, want_lse=False):

@@ -171,3 +171,20 @@ def pack_block_head_stream(proj_w, qkv_w, dtype):
     accumulator registers)."""
     assert proj_w.shape[0] == proj_w.shape[1] and qkv_w.shape == (3 * proj_w.shape[0], proj_w.shape[1])
     return torch.cat([pack_rows_tail(proj_w, dtype), pack_ff2_kperm(qkv_w, dtype)], 0).contiguous()
+
+
+def pack_adapters(adapters, dtype, device=None):
+    """Low-rank adapters of one projection for ops.adapter_gemm: adapters = [(down [r_i, K], up [N, r_i], alpha_i), ...] of any ranks
+    up to 128 (alpha None: alpha = r, i.e. scale 1) -> dict(down [S, r, K], up [S, N, r] in `dtype`, scale fp32 [S] = alpha_i / r_i)
+    with r the largest rank rounded up to a multiple of 8, zeros behind each adapter's own."""
+    assert len(adapters) > 0
+    ranks = [d.shape[0] for d, _, _ in adapters]
+    r = (max(ranks) + 7) // 8 * 8
+    K, N = adapters[0][0].shape[1], adapters[0][1].shape[0]
+    assert 0 < min(ranks) and r <= 128 and all(d.shape == (q, K) and u.shape == (N, q) for (d, u, _), q in zip(adapters, ranks))
+    pad = torch.nn.functional.pad
+    down = torch.stack([pad(d.detach().float(), (0, 0, 0, r - d.shape[0])) for d, _, _ in adapters]).to(dtype)
+    up = torch.stack([pad(u.detach().float(), (0, r - u.shape[1])) for _, u, _ in adapters]).to(dtype)
+    scale = torch.tensor([1.0 if al is None else float(al) / q for (_, _, al), q in zip(adapters, ranks)], dtype=torch.float32)
+    device = down.device if device is None else device
+    return dict(down=down.to(device).contiguous(), up=up.to(device).contiguous(), scale=scale.to(device))
