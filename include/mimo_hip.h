@@ -140,12 +140,13 @@ int mimo_gemm_ext(int dtype, const void* A, int64_t lda, const void* W, void* ou
  * feed-forward projections of src/models/attention.py:321-345,429 with an adapter per request):
  *   out[m] = A[m].W^T + bias + residual[m] + u[m].up[i]^T,   u[m] = scale[i] A[m].down[i]^T,   i = index[m / rows_per_index]
  *   A: half16 [M, lda]; W: half16 [N, K]; out: half16 or (MIMO_EPI_OUT_F32) fp32 [M, ldo]; bias fp32 [N], residual half16 or
- *   (MIMO_EPI_RES_F32) fp32 [M, ldr], both nullable; flags: those two only.  N % 8 == 0, K % 8 == 0, N K < 2^30, M < 2^31.
+ *   (MIMO_EPI_RES_F32) fp32 [M, ldr], both nullable; flags: those two only.  N % 8 == 0, K % 8 == 0, N K < 2^30,
+ *   N, K < 2^23, M < 2^31.
  *   down: half16 [count, rank, K], up: half16 [count, N, rank], rank % 8 == 0, rank <= 128 (pad a smaller one with zeros);
  *   scale: fp32 [count] or NULL (1); index: int32 device array of ceil(M / rows_per_index) entries, in any order and number; an
  *   entry outside [0, count) means no adapter.
- *   low: caller's half16 [M, rank] (low_split = 0) or [M, 2 rank] (low_split != 0: hi | lo halves of u, needed for a fp32 result
- *   and for the backward); it is written by the call and holds u afterwards.
+ *   low: caller's half16 [M, rank] (low_split = 0) or [M, P rank] (low_split != 0: u as P = 2 (fp16) | 3 (bf16) planes, value and
+ *   remainders, needed for a fp32 result and for the backward); it is written by the call and holds u afterwards.
  *   backward, W frozen: dA [M, ldda] half16 (nullable: not wanted) = dY.W + t.down with t = scale dY.up, from Wt = W^T, half16 [K, N];
  *   ddown fp32 [count, rank, K] = sum_m t[m]^T A[m], dup fp32 [count, N, rank] = sum_m dY[m]^T u[m], summed in a fixed order (no
  *   atomics; zeros for an adapter without rows).  low: the forward's split form.  workspace: 16-byte aligned, the size the
@@ -162,7 +163,7 @@ typedef struct mimo_adapter_params {
 int mimo_adapter_gemm(int dtype, const void* A, int64_t lda, const void* W, void* out, int64_t ldo, int64_t M, int N, int K,
                       const float* bias, const void* residual, int64_t ldr, unsigned flags, const mimo_adapter_params* p,
                       void* low, int low_split, void* stream);
-size_t mimo_adapter_gemm_backward_workspace(const mimo_adapter_params* p, int64_t M, int N, int K);
+size_t mimo_adapter_gemm_backward_workspace(int dtype, const mimo_adapter_params* p, int64_t M, int N, int K);
 int mimo_adapter_gemm_backward(int dtype, const void* dY, int64_t ldy, const void* A, int64_t lda, const void* Wt, void* dA,
                                int64_t ldda, int64_t M, int N, int K, const mimo_adapter_params* p, const void* low, float* ddown,
                                float* dup, void* workspace, size_t workspace_bytes, void* stream);

@@ -7,8 +7,8 @@
 // (tile_adapter): the result is written once and no intermediate is wider than the rank.  A tile walks the DISTINCT adapters of
 // its rows, usually one; a row never takes part in another row's adapter (values are selected, not multiplied by zero, so a NaN
 // in one adapter stays in its requests).
-// u is kept as a rounded 16-bit value where the result is 16 bit, and as hi + lo halves (22 / 16 mantissa bits) where the
-// result is fp32 or gradients are to be taken.
+// u is kept as one rounded 16-bit value where the result is 16 bit, and as PLANES of 16-bit values (value | remainder: fp16 2, bf16
+// 3, i.e. at least 22 mantissa bits) where the result is fp32 or gradients are to be taken: [M, planes rank].
 //
 // Backward of the same call, W frozen: t[m] = scale[i] dy[m].up[i];  da = dy.W + t.down (the same kernels on W^T and transposed
 // adapters);  ddown[i] = sum_m t[m]^T a[m];  dup[i] = sum_m dy[m]^T u[m] (adapter_outer_kernel: rows stream through LDS, both
@@ -28,15 +28,19 @@ inline int cu_count() {
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+constexpr int planes_of(int dt) { return dt == MIMO_F16 ? 2 : 3; }
+constexpr float T_SCALE = 2048.f;  // on the remainder plane of t in fp16: gradients are small, 2^-25 is not small beside them
+
 // which adapter a row has
 struct Rows {
   const int* index;
-  int64_t M, rpi;
+  int64_t M;
+  unsigned rpi;
   int n;
 };
 __device__ __forceinline__ int adapter_of(const Rows& r, int64_t m) {
   if (m >= r.M) return -1;
-  const int i = r.index[r.rpi == 1 ? m : m / r.rpi];
+  const int i = r.index[r.rpi == 1u ? (unsigned)m : (unsigned)m / r.rpi];
   return (unsigned)i < (unsigned)r.n ? i : -1;
 }
 
@@ -52,66 +56,31 @@ __device__ __forceinline__ int next_adapter(const int (&ad)[N]) {
   return cur;
 }
 
-}  // namespace
-
-namespace {
-
-template <int DT, int NR, int MT>
-__device__ __forceinline__ void tile_adapter(const GemmArgs& g, f32x4 (&acc)[NR][MT], const int64_t M0, const int N0, const int wm,
-                                             const int wn, const int lg, const int li) {
-  int ad[MT];
-#pragma unroll
-  for (int mi = 0; mi < MT; ++mi) {
-    const int64_t m = M0 + (wm * MT + mi) * 16 + li;
-    int i = -1;
-    if (m < g.M) i = g.ad_index[g.ad_rpi == 1 ? m + g.ad_row0 : (m + g.ad_row0) / g.ad_rpi];
-    ad[mi] = (unsigned)i < (unsigned)g.ad_n ? i : -1;
-  }
-  const uint16_t* low = g.ad_low + (M0 + wm * MT * 16 + li) * g.ad_ld;
-  for (int cur = next_adapter<MT>(ad); cur >= 0; cur = next_adapter<MT>(ad)) {
-    const uint16_t* up = g.ad_up + ((int64_t)cur * g.N + N0 + wn * 16 * NR + li) * g.ad_rank;
-    for (int k0 = 0; k0 < g.ad_cols; k0 += 32) {
-      const int kk = k0 + 8 * lg, ku = kk < g.ad_rank ? kk : kk - g.ad_rank;  // (the lo halves meet the same weights)
-      uint4 fb[NR];
-#pragma unroll
-      for (int ni = 0; ni < NR; ++ni) {
-        fb[ni] = make_uint4(0, 0, 0, 0);
-        if (kk < g.ad_cols && N0 + (wn * NR + ni) * 16 + li < g.N)
-          fb[ni] = *reinterpret_cast<const uint4*>(up + (int64_t)ni * 16 * g.ad_rank + ku);
-      }
-#pragma unroll
-      for (int mi = 0; mi < MT; ++mi) {
-        const bool mine = ad[mi] == cur;
-        const unsigned long long b = __builtin_amdgcn_ballot_w64(mine);
-        if (b == 0ull) continue;
-        uint4 fu = make_uint4(0, 0, 0, 0);
-        if (mine && kk < g.ad_cols) fu = *reinterpret_cast<const uint4*>(low + (int64_t)mi * 16 * g.ad_ld + kk);
-        if (b == ~0ull) {
-#pragma unroll
-          for (int ni = 0; ni < NR; ++ni) acc[ni][mi] = HT<DT>::mfma16(fb[ni], fu, acc[ni][mi]);
-        } else {
-#pragma unroll
-          for (int ni = 0; ni < NR; ++ni) {
-            const f32x4 v = HT<DT>::mfma16(fb[ni], fu, acc[ni][mi]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[ni][mi][r] = mine ? v[r] : acc[ni][mi][r];
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int mi = 0; mi < MT; ++mi) ad[mi] = ad[mi] == cur ? -1 : ad[mi];
-  }
-}
-
 struct LowArgs {
   const uint16_t *X, *down;  // [M, ldx], [n, r, K]
   const float* scale;        // [n] or null
-  uint16_t* low;             // [M, ld]: hi, and lo behind it when split
+  uint16_t* low;             // [M, planes r]
   int64_t ldx;
   Rows rows;
-  int K, r, ld, split;
+  int K, r, planes;
+  float lo_scale;            // a power of two on the remainder plane (fp16: small values keep their precision)
 };
+
+// the planes of four consecutive ranks of a row
+template <int DT>
+__device__ __forceinline__ void store_planes(const LowArgs& a, uint16_t* p, f32x4 v) {
+  float scale = a.lo_scale;
+  for (int q = 0;; ++q) {
+    const uint2 h = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
+    *reinterpret_cast<uint2*>(p + q * a.r) = h;
+    if (q + 1 >= a.planes) break;
+    v[0] = (v[0] - HT<DT>::to_f((uint16_t)(h.x & 0xffffu))) * scale;
+    v[1] = (v[1] - HT<DT>::to_f((uint16_t)(h.x >> 16))) * scale;
+    v[2] = (v[2] - HT<DT>::to_f((uint16_t)(h.y & 0xffffu))) * scale;
+    v[3] = (v[3] - HT<DT>::to_f((uint16_t)(h.y >> 16))) * scale;
+    scale = 1.f;
+  }
+}
 
 __device__ __forceinline__ float scale_of(const LowArgs& a, int ad) { return ad < 0 ? 0.f : a.scale ? a.scale[ad] : 1.f; }
 
@@ -195,21 +164,12 @@ __global__ __launch_bounds__(256) void adapter_low_kernel(const LowArgs a) {
       if (j >= a.r) continue;
       f32x4 v = res[t][mi] * sc;
       if (ad[mi] < 0) v = (f32x4){0.f, 0.f, 0.f, 0.f};
-      uint16_t* p = a.low + m * a.ld + j;
-      const uint2 hi = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
-      *reinterpret_cast<uint2*>(p) = hi;
-      if (a.split) {
-        f32x4 h;
-        h[0] = HT<DT>::to_f((uint16_t)(hi.x & 0xffffu)); h[1] = HT<DT>::to_f((uint16_t)(hi.x >> 16));
-        h[2] = HT<DT>::to_f((uint16_t)(hi.y & 0xffffu)); h[3] = HT<DT>::to_f((uint16_t)(hi.y >> 16));
-        v -= h;
-        *reinterpret_cast<uint2*>(p + a.r) = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
-      }
+      store_planes<DT>(a, a.low + m * a.planes * a.r + j, v);
     }
   }
 }
 
-// u for rows that each have an adapter of their own: one block per row, a wave per rank in turn, lanes along K
+// u for rows that each have an adapter of their own: one block per row, a wave per four ranks in turn, lanes along K
 template <int DT>
 __global__ __launch_bounds__(256) void adapter_low_row_kernel(const LowArgs a) {
   const int64_t m = blockIdx.x;
@@ -217,25 +177,25 @@ __global__ __launch_bounds__(256) void adapter_low_row_kernel(const LowArgs a) {
   const int ad = adapter_of(a.rows, m);
   const float sc = scale_of(a, ad);
   const uint16_t* x = a.X + m * a.ldx;
-#pragma unroll 4
-  for (int j = wave; j < a.r; j += 4) {
-    float s = 0.f;
+  for (int j = 4 * wave; j < a.r; j += 16) {
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (ad >= 0) {
       const uint16_t* dn = a.down + ((int64_t)ad * a.r + j) * a.K;
+#pragma unroll 3
       for (int k = 8 * lane; k < a.K; k += 512) {
         float p[8], q[8];
         unpack8<DT>(*reinterpret_cast<const uint4*>(x + k), p);
-        unpack8<DT>(*reinterpret_cast<const uint4*>(dn + k), q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(p[i], q[i], s);
+        for (int n = 0; n < 4; ++n) {
+          unpack8<DT>(*reinterpret_cast<const uint4*>(dn + (int64_t)n * a.K + k), q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[n] = fmaf(p[i], q[i], s[n]);
+        }
       }
-      s = wave_sum(s) * sc;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) s[n] = wave_sum(s[n]) * sc;
     }
-    if (lane == 0) {
-      const uint16_t hi = HT<DT>::from_f(s);
-      a.low[m * a.ld + j] = hi;
-      if (a.split) a.low[m * a.ld + a.r + j] = HT<DT>::from_f(s - HT<DT>::to_f(hi));
-    }
+    if (lane == 0) store_planes<DT>(a, a.low + m * a.planes * a.r + j, s);
   }
 }
 
@@ -264,15 +224,16 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(const TransposeA
 
 // sum over the rows of adapter blockIdx.y of low[m]^T x[m], for two pairs in one launch: (t, a) -> ddown and (u, dy) -> dup.
 // A block owns 128 columns of x and all ranks; tiles of 64 rows pass through LDS row-major, both operands are read transposed
-// (a row that is not this adapter's is staged as zeros on BOTH sides); the hi and lo halves of low meet in the same fp32
-// accumulators.  Rows: only [first, last] of the adapter, cut into gridDim.z parts.
+// (a row that is not this adapter's is staged as zeros on BOTH sides); the planes of low meet the same columns (fp16: the remainder
+// plane has accumulators of its own, its scale comes off at the end).  Rows: only [first, last] of the adapter, cut into gridDim.z parts.
 struct OuterArgs {
   const uint16_t *x[2], *low[2];
   float* part[2];  // [parts][n][r][C]
   int64_t ldx[2];
   int C[2];
+  float lo_scale[2];  // what the remainder plane has to be multiplied with
   Rows rows;
-  int r, ld, ct0;  // ct0: column tiles of the first pair
+  int r, ct0;      // ct0: column tiles of the first pair
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -289,8 +250,9 @@ __device__ __forceinline__ uint4 read_tr16(const uint16_t* tile, int pitch, int 
 
 template <int DT, int RT>
 __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
-  constexpr int MR = 64, XP = 128 + 8, LP = 32 * RT + 24;  // (the lo half of a rank of 8 is read up to column 8 + 16)
-  constexpr int NX = 4, NL = RT;                          // 16-byte chunks a thread stages per tile
+  constexpr int NP = planes_of(DT), NA = DT == MIMO_F16 ? 2 : 1;
+  constexpr int MR = 64, XP = 128 + 8, LP = NP * 16 * RT + 8;
+  constexpr int NX = 4, NL = (NP * RT + 1) / 2;  // 16-byte chunks a thread stages per tile
   __shared__ __attribute__((aligned(16))) uint16_t xs[MR * XP];
   __shared__ __attribute__((aligned(16))) uint16_t ls[MR * LP];
   __shared__ int range[2];
@@ -314,18 +276,20 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     atomicMin(&range[0], lo);
     atomicMax(&range[1], hi);
   }
-  for (int i = tid; i < MR * LP / 2; i += 256) reinterpret_cast<uint32_t*>(ls)[i] = 0u;  // columns behind 2 r are never staged
+  for (int i = tid; i < MR * LP / 2; i += 256) reinterpret_cast<uint32_t*>(ls)[i] = 0u;  // columns behind the planes are never staged
   __syncthreads();
-  f32x4 acc[RT][2];
+  f32x4 acc[NA][RT][2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) acc[t][0] = acc[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < NA; ++p)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[p][t][0] = acc[p][t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if (range[1] >= 0) {
     const int64_t m_lo = (int64_t)range[0] * a.rows.rpi;
     int64_t m_hi = ((int64_t)range[1] + 1) * a.rows.rpi;
     if (m_hi > a.rows.M) m_hi = a.rows.M;
     const int64_t tiles = (m_hi - m_lo + MR - 1) / MR, per = (tiles + gridDim.z - 1) / gridDim.z;
     const int64_t t_lo = blockIdx.z * per, t_hi = t_lo + per < tiles ? t_lo + per : tiles;
-    const int lc = 2 * a.r / 8;  // 16-byte chunks of a row of low
+    const int lc = NP * a.r / 8;  // 16-byte chunks of a row of low
     uint4 xr[NX], lr[NL];
     auto fetch = [&](int64_t t) {
       const int64_t m0 = m_lo + t * MR;
@@ -341,7 +305,7 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
         const int id = tid + 256 * i, row = id / lc;
         const int64_t m = m0 + row;
         lr[i] = make_uint4(0, 0, 0, 0);
-        if (row < MR && adapter_of(a.rows, m) == who) lr[i] = *reinterpret_cast<const uint4*>(a.low[z] + m * a.ld + (id - row * lc) * 8);
+        if (row < MR && adapter_of(a.rows, m) == who) lr[i] = *reinterpret_cast<const uint4*>(a.low[z] + m * NP * a.r + (id - row * lc) * 8);
       }
     };
     if (t_lo < t_hi) fetch(t_lo);
@@ -366,9 +330,12 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
         for (int c = 0; c < 2; ++c) fx[c] = read_tr16(xs, XP, k0, wave * 32 + 16 * c, lane);
 #pragma unroll
         for (int q = 0; q < RT; ++q) {
-          const uint4 fh = read_tr16(ls, LP, k0, 16 * q, lane), fl = read_tr16(ls, LP, k0, a.r + 16 * q, lane);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) acc[q][c] = HT<DT>::mfma16(fl, fx[c], HT<DT>::mfma16(fh, fx[c], acc[q][c]));
+          for (int p = 0; p < NP; ++p) {
+            const uint4 fl = read_tr16(ls, LP, k0, p * a.r + 16 * q, lane);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) acc[p % NA][q][c] = HT<DT>::mfma16(fl, fx[c], acc[p % NA][q][c]);
+          }
         }
       }
     }
@@ -384,7 +351,7 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = 16 * q + 4 * lg + i;
-        if (j < a.r) out[(int64_t)j * C + col] = acc[q][c][i];
+        if (j < a.r) out[(int64_t)j * C + col] = NA == 1 ? acc[0][q][c][i] : fmaf(acc[NA - 1][q][c][i], a.lo_scale[z], acc[0][q][c][i]);
       }
   }
 }
@@ -438,7 +405,7 @@ int launch_low(const LowArgs& a, hipStream_t st) {
 
 template <int DT, int NR>
 int launch_tiles(GemmArgs& g, hipStream_t st) {
-  // the tile choice of mimo_gemm (gemm_conv.hip launch_nr), without split-K
+  // the tile choice of mimo_gemm (gemm_conv.hip launch_nr), without split-K and persistent blocks
   const int cus = cu_count();
   const int64_t m256 = (g.M + 255) / 256;
   const int tn_s = (g.N + 32 * NR - 1) / (32 * NR), tn_xl = (g.N + 64 * NR - 1) / (64 * NR);
@@ -450,10 +417,7 @@ int launch_tiles(GemmArgs& g, hipStream_t st) {
     if (cost(128) < cost(bm)) bm = 128;
     const int64_t nwg = ((g.M + bm - 1) / bm) * tn_xl;
     if (nwg > 0x7fffffff) return MIMO_EINVAL;
-    if (NR == 5 && bm == 256 && nwg >= 3 * (int64_t)cus && g.nkt >= 2 && g.nkt <= 20) {
-      g.ntiles = (unsigned)nwg;
-      hipLaunchKernelGGL((gemm_dense_persist_kernel<DT, NR, 2, 4, 8, 3>), dim3((unsigned)cus), dim3(512), 0, st, g);
-    } else if (bm == 256) {
+    if (bm == 256) {
       hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 4, 2, 8, 3>), dim3((unsigned)nwg), dim3(512), 0, st, g);
     } else if (bm == 192) {
       hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 4, 2, 6, 3>), dim3((unsigned)nwg), dim3(512), 0, st, g);
@@ -478,7 +442,7 @@ int launch_tiles(GemmArgs& g, hipStream_t st) {
 template <int DT>
 int launch_gemm(GemmArgs g, hipStream_t st) {
   // operands are addressed with 32-bit byte offsets: more rows than that go in several launches
-  const int64_t M = g.M, most = g.lda > 0 ? (0x7fffffffLL / (2 * g.lda) - 1) / 256 * 256 : M;
+  const int64_t M = g.M, wide = g.lda > g.ad_ld ? g.lda : g.ad_ld, most = (0x7fffffffLL / (2 * wide) - 1) / 256 * 256;
   const bool of32 = g.flags & MIMO_EPI_OUT_F32, rf32 = g.flags & MIMO_EPI_RES_F32;
   for (int64_t r0 = 0; r0 < M; r0 += most) {
     GemmArgs c = g;
@@ -491,7 +455,7 @@ int launch_gemm(GemmArgs g, hipStream_t st) {
     c.a_bytes = (unsigned)(((c.M - 1) * c.lda + c.K) * 2);
     const int64_t tn8 = (c.N + 255) / 256, nt8 = ((c.M + 255) / 256) * tn8;
     int rc;
-    if ((c.K % 128) == 0 && tn8 * 256 - c.N <= c.N / 12 && nt8 >= 128 && nt8 <= 0x7fffffff) {
+    if ((c.K % 64) == 0 && tn8 * 256 - c.N <= c.N / 12 && nt8 >= 128 && nt8 <= 0x7fffffff) {
       c.tiles_n = (int)tn8;
       c.ntiles = (unsigned)G8_GM;
       hipLaunchKernelGGL((gemm8_kernel<DT, 3>), dim3((unsigned)nt8), dim3(512), 0, st, c);
@@ -507,11 +471,17 @@ int launch_gemm(GemmArgs g, hipStream_t st) {
 
 // checks shared by both entries
 int check(const mimo_adapter_params* p, int64_t M, int N, int K) {
-  if (!p || M <= 0 || M >= 0x7fffffffLL || N <= 0 || K <= 0 || (N & 7) || (K & 7) || (int64_t)N * K >= 0x40000000LL) return MIMO_EINVAL;
+  if (!p || M <= 0 || M >= 0x7fffffffLL || N <= 0 || K <= 0 || (N & 7) || (K & 7) || (int64_t)N * K >= 0x40000000LL ||
+      N >= 0x800000 || K >= 0x800000)
+    return MIMO_EINVAL;
   if (!p->down || !p->up || !p->index || p->count <= 0 || p->rank <= 0 || p->rank > 128 || (p->rank & 7) || p->rows_per_index <= 0)
     return MIMO_EINVAL;
   if (p->count > 65535 || !aligned16(p->down) || !aligned16(p->up) || (reinterpret_cast<uintptr_t>(p->index) & 3u)) return MIMO_EINVAL;
   return MIMO_OK;
+}
+
+Rows rows_of(const mimo_adapter_params* p, int64_t M) {
+  return Rows{p->index, M, (unsigned)(p->rows_per_index < 0x7fffffff ? p->rows_per_index : 0x7fffffff), p->count};
 }
 
 GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t ldo, int64_t M, int N, int K, const Rows& rows,
@@ -534,12 +504,12 @@ int forward(GemmArgs g, const LowArgs& la, hipStream_t st) {
   return launch_gemm<DT>(g, st);
 }
 
-// workspace of the backward, in bytes: t [M, 2 r] | up^T | down^T | parts of ddown | parts of dup
+// workspace of the backward, in bytes: t [M, planes r] | up^T | down^T | parts of ddown | parts of dup
 struct BackwardPlan {
   int parts;
   size_t t, upt, downt, p0, p1, total;
 };
-BackwardPlan backward_plan(const mimo_adapter_params* p, int64_t M, int N, int K) {
+BackwardPlan backward_plan(int dtype, const mimo_adapter_params* p, int64_t M, int N, int K) {
   BackwardPlan b{};
   const int64_t n = p->count, r = p->rank;
   const int64_t blocks = n * ((N + 127) / 128 + (K + 127) / 128), tiles = (M + 63) / 64;
@@ -548,7 +518,7 @@ BackwardPlan backward_plan(const mimo_adapter_params* p, int64_t M, int N, int K
   if (parts > 256) parts = 256;
   b.parts = parts < 1 ? 1 : (int)parts;
   auto up16 = [](size_t x) { return (x + 15) / 16 * 16; };
-  b.t = up16((size_t)M * 2 * r * 2);
+  b.t = up16((size_t)M * planes_of(dtype) * r * 2);
   b.upt = up16((size_t)n * r * N * 2);
   b.downt = up16((size_t)n * r * K * 2);
   b.p0 = up16((size_t)b.parts * n * r * K * 4);
@@ -560,25 +530,27 @@ BackwardPlan backward_plan(const mimo_adapter_params* p, int64_t M, int N, int K
 template <int DT>
 int backward(const void* dY, int64_t ldy, const void* A, int64_t lda, const void* Wt, void* dA, int64_t ldda, int64_t M, int N, int K,
              const mimo_adapter_params* p, const void* low, float* ddown, float* dup, char* ws, hipStream_t st) {
-  const BackwardPlan b = backward_plan(p, M, N, K);
+  const BackwardPlan b = backward_plan(DT, p, M, N, K);
   const int n = p->count, r = p->rank;
   uint16_t* t = (uint16_t*)ws;
   uint16_t* upt = (uint16_t*)(ws + b.t);
   uint16_t* downt = (uint16_t*)(ws + b.t + b.upt);
   float* p0 = (float*)(ws + b.t + b.upt + b.downt);
   float* p1 = (float*)((char*)p0 + b.p0);
-  const Rows rows{p->index, M, p->rows_per_index, n};
+  const Rows rows = rows_of(p, M);
   TransposeArgs ta{{(const uint16_t*)p->up, (const uint16_t*)p->down}, {upt, downt}, {N, r}, {r, K}};
   const int tiles = ((N > K ? N : K) + 31) / 32 * ((r + 31) / 32);
   hipLaunchKernelGGL(adapter_transpose_kernel, dim3((unsigned)tiles, (unsigned)n, 2u), dim3(256), 0, st, ta);
   MIMO_LAUNCH_CHECK();
-  const LowArgs la{(const uint16_t*)dY, upt, p->scale, t, ldy, rows, N, r, 2 * r, 1};
+  constexpr int NP = planes_of(DT);
+  constexpr float up2 = DT == MIMO_F16 ? T_SCALE : 1.f;
+  const LowArgs la{(const uint16_t*)dY, upt, p->scale, t, ldy, rows, N, r, NP, up2};
   if (const int rc = launch_low<DT>(la, st)) return rc;
   if (dA) {
-    GemmArgs g = gemm_args(dY, ldy, Wt, dA, ldda, M, K, N, rows, t, 2 * r, r, downt, r);
+    GemmArgs g = gemm_args(dY, ldy, Wt, dA, ldda, M, K, N, rows, t, NP * r, r, downt, r);
     if (const int rc = launch_gemm<DT>(g, st)) return rc;
   }
-  OuterArgs oa{{(const uint16_t*)A, (const uint16_t*)dY}, {t, (const uint16_t*)low}, {p0, p1}, {lda, ldy}, {K, N}, rows, r, 2 * r,
+  OuterArgs oa{{(const uint16_t*)A, (const uint16_t*)dY}, {t, (const uint16_t*)low}, {p0, p1}, {lda, ldy}, {K, N}, {1.f / up2, 1.f}, rows, r,
                (K + 127) / 128};
   const dim3 grid((unsigned)((K + 127) / 128 + (N + 127) / 128), (unsigned)n, (unsigned)b.parts);
   const int rt = (r + 15) / 16;
@@ -606,20 +578,19 @@ extern "C" int mimo_adapter_gemm(int dtype, const void* A, int64_t lda, const vo
   if (flags & ~(MIMO_EPI_OUT_F32 | MIMO_EPI_RES_F32)) return MIMO_EINVAL;
   const bool of32 = flags & MIMO_EPI_OUT_F32;
   if (of32 && !low_split) return MIMO_EINVAL;
-  const Rows rows{p->index, M, p->rows_per_index, p->count};
-  const int ld = low_split ? 2 * p->rank : p->rank;
-  GemmArgs g = gemm_args(A, lda, W, out, ldo, M, N, K, rows, (const uint16_t*)low, ld, of32 ? 2 * p->rank : p->rank,
+  const Rows rows = rows_of(p, M);
+  if (dtype != MIMO_F16 && dtype != MIMO_BF16) return MIMO_EDTYPE;
+  const int planes = low_split ? planes_of(dtype) : 1;
+  GemmArgs g = gemm_args(A, lda, W, out, ldo, M, N, K, rows, (const uint16_t*)low, planes * p->rank, of32 ? planes * p->rank : p->rank,
                          (const uint16_t*)p->up, p->rank);
   g.bias = bias; g.res = residual; g.ldr = ldr;
   g.flags |= flags;
-  const LowArgs la{(const uint16_t*)A, (const uint16_t*)p->down, p->scale, (uint16_t*)low, lda, rows, K, p->rank, ld, low_split ? 1 : 0};
-  if (dtype == MIMO_F16) return forward<MIMO_F16>(g, la, (hipStream_t)stream);
-  if (dtype == MIMO_BF16) return forward<MIMO_BF16>(g, la, (hipStream_t)stream);
-  return MIMO_EDTYPE;
+  const LowArgs la{(const uint16_t*)A, (const uint16_t*)p->down, p->scale, (uint16_t*)low, lda, rows, K, p->rank, planes, 1.f};
+  return dtype == MIMO_F16 ? forward<MIMO_F16>(g, la, (hipStream_t)stream) : forward<MIMO_BF16>(g, la, (hipStream_t)stream);
 }
 
-extern "C" size_t mimo_adapter_gemm_backward_workspace(const mimo_adapter_params* p, int64_t M, int N, int K) {
-  return check(p, M, N, K) == MIMO_OK ? backward_plan(p, M, N, K).total : 0;
+extern "C" size_t mimo_adapter_gemm_backward_workspace(int dtype, const mimo_adapter_params* p, int64_t M, int N, int K) {
+  return check(p, M, N, K) == MIMO_OK ? backward_plan(dtype, p, M, N, K).total : 0;
 }
 
 extern "C" int mimo_adapter_gemm_backward(int dtype, const void* dY, int64_t ldy, const void* A, int64_t lda, const void* Wt, void* dA,
@@ -628,7 +599,7 @@ extern "C" int mimo_adapter_gemm_backward(int dtype, const void* dY, int64_t ldy
   if (const int rc = check(p, M, N, K)) return rc;
   if (!dY || !A || !low || !ddown || !dup || !workspace || (dA && !Wt) || (ldy & 7) || (lda & 7) || (ldda & 3) || lda < 0 || ldy < 0 || ldy > 0x100000 ||
       !aligned16(dY) || !aligned16(A) || !aligned16(Wt) || !aligned16(dA) || !aligned16(low) || !aligned16(ddown) || !aligned16(dup) ||
-      !aligned16(workspace) || workspace_bytes < backward_plan(p, M, N, K).total)
+      !aligned16(workspace) || workspace_bytes < backward_plan(dtype, p, M, N, K).total)
     return MIMO_EINVAL;
   if (dtype == MIMO_F16)
     return backward<MIMO_F16>(dY, ldy, A, lda, Wt, dA, ldda, M, N, K, p, low, ddown, dup, (char*)workspace, (hipStream_t)stream);

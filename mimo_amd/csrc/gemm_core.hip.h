@@ -57,9 +57,10 @@ struct GemmArgs {
   float a_eps;
   // low-rank adapters (EPI 3): row m (counted from ad_row0) belongs to adapter ad_index[(ad_row0 + m) / ad_rpi], none if outside [0, ad_n)
   const int* ad_index;
-  const uint16_t* ad_low;    // half16 [M, ad_ld]: the rows' low-rank values in ad_cols columns, rounded (rank) or as hi | lo halves (2 rank)
+  const uint16_t* ad_low;    // half16 [M, ad_ld]: the rows' low-rank values in ad_cols columns = planes of ad_rank (value, remainder, ..)
   const uint16_t* ad_up;     // half16 [ad_n, N, ad_rank]
-  int64_t ad_row0, ad_rpi;
+  int64_t ad_row0;
+  unsigned ad_rpi;
   int ad_n, ad_rank, ad_cols, ad_ld;
   unsigned long long* dbg;  // MIMO_TUNE builds: cycle-counter trace of block 0 (null otherwise)
 };
@@ -776,15 +777,101 @@ __device__ __forceinline__ void tile_epilogue_ln(const GemmArgs& g, f32x4 (&acc)
   }
 }
 
-// acc += low . up^T for the rows of the tile, each with its own adapter (adapter.hip)
+// ---- EPI 3: out += low . up^T, every row with the adapter of its request ----
+// Where all rows of a tile have one adapter (most tiles: requests are longer than tiles) the low-rank product is the tile's last
+// K-tiles: the same ring, the operands come from `low` and from that adapter's `up`, nothing waits.  A tile with several adapters
+// takes tile_adapter behind the K loop instead.
+// adapters of rows M0 + lane, M0 + 64 + lane, ... (rows that do not exist: -2, no adapter: -1)
+template <int N>
+__device__ __forceinline__ void adapter_rows(const GemmArgs& g, const int64_t M0, const int lane, int (&ad)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int64_t m = M0 + 64 * i + lane;
+    ad[i] = -2;
+    if (m < g.M) {
+      const unsigned x = (unsigned)(m + g.ad_row0);
+      const int a = g.ad_index[g.ad_rpi == 1u ? x : x / g.ad_rpi];
+      ad[i] = (unsigned)a < (unsigned)g.ad_n ? a : -1;
+    }
+  }
+}
+// the one adapter (or -1: none) of all rows, -2 where they differ.  The same value in every wave.
+template <int N>
+__device__ __forceinline__ int adapter_vote(const int (&ad)[N]) {
+  const int first = __builtin_amdgcn_readfirstlane(ad[0]);
+  bool same = true;
+#pragma unroll
+  for (int i = 0; i < N; ++i) same &= (ad[i] == first) | (ad[i] == -2);
+  return __builtin_amdgcn_ballot_w64(!same) == 0ull ? first : -2;
+}
+// rank index of column kk of `low`
+__device__ __forceinline__ int adapter_rank_of(const GemmArgs& g, int kk) {
+  while (kk >= g.ad_rank) kk -= g.ad_rank;
+  return kk;
+}
+
+// A tile with several adapters: for each of them in turn, its rows' low values meet its weights on the matrix unit; results are
+// SELECTED into the rows that have it (a zero operand would let a NaN of one adapter into the other requests' rows).  Fragments
+// straight from L2: acc keeps most of the registers.
 template <int DT, int NR, int MT>
 __device__ __forceinline__ void tile_adapter(const GemmArgs& g, f32x4 (&acc)[NR][MT], const int64_t M0, const int N0, const int wm,
-                                             const int wn, const int lg, const int li);
+                                             const int wn, int lg, int li) {
+  asm volatile("" : "+v"(lg), "+v"(li));  // nothing of this is computed ahead of the K loop
+  constexpr unsigned OOB = 0xFFFFFFF0u;
+  int ad[MT];
+#pragma unroll
+  for (int mi = 0; mi < MT; ++mi) {
+    int one[1];
+    adapter_rows<1>(g, M0 + (wm * MT + mi) * 16, li, one);
+    ad[mi] = one[0];
+  }
+  const int64_t rows = g.M - M0;
+  const __amdgpu_buffer_rsrc_t r_low = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)const_cast<uint16_t*>(g.ad_low + M0 * g.ad_ld), 0, (int)((rows < 256 ? rows : 256) * g.ad_ld * 2), 0x00020000);
+  for (;;) {
+    int cur = -1;  // the adapter of the first row that is still to do
+#pragma unroll
+    for (int mi = MT - 1; mi >= 0; --mi) {
+      const unsigned long long b = __builtin_amdgcn_ballot_w64(ad[mi] >= 0);
+      if (b != 0ull) cur = __builtin_amdgcn_readlane(ad[mi], (int)__builtin_ctzll(b));
+    }
+    if (cur < 0) break;
+    const __amdgpu_buffer_rsrc_t r_up = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)const_cast<uint16_t*>(g.ad_up + (int64_t)cur * g.N * g.ad_rank), 0, g.N * g.ad_rank * 2, 0x00020000);
+    for (int k0 = 0; k0 < g.ad_cols; k0 += 32) {
+      const int kk = k0 + 8 * lg, ku = adapter_rank_of(g, kk);
+      const bool kok = kk < g.ad_cols;
+      uint4 fb[NR];
+#pragma unroll
+      for (int ni = 0; ni < NR; ++ni) {
+        const int n = N0 + (wn * NR + ni) * 16 + li;
+        fb[ni] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               r_up, kok && n < g.N ? (unsigned)(n * g.ad_rank + ku) * 2u : OOB, 0, 0));
+      }
+#pragma unroll
+      for (int mi = 0; mi < MT; ++mi) {
+        const bool mine = ad[mi] == cur;
+        if (__builtin_amdgcn_ballot_w64(mine) == 0ull) continue;
+        const uint4 fu = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                       r_low, mine && kok ? (unsigned)(((wm * MT + mi) * 16 + li) * g.ad_ld + kk) * 2u : OOB, 0, 0));
+#pragma unroll
+        for (int ni = 0; ni < NR; ++ni) {
+          const f32x4 v = HT<DT>::mfma16(fb[ni], fu, acc[ni][mi]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[ni][mi][r] = mine ? v[r] : acc[ni][mi][r];
+        }
+      }
+    }
+#pragma unroll
+    for (int mi = 0; mi < MT; ++mi) ad[mi] = ad[mi] == cur ? -1 : ad[mi];
+  }
+}
 
 // MODE 0: dense GEMM; 1: convolution gather; 2: convolution gather through a nearest-neighbour upsampling
 // EPI 0: ordinary epilogue (+ GroupNorm column statistics when g.colstats is set); 1: + fused LayerNorm second output
+// (EPI 3 on four waves: two blocks per CU have to be asked for, the mixed-tile path would otherwise take the registers of both)
 template <int DT, int NR, int MODE, int WM, int WN, int NSTAGE, int MT, int EPI = 0>
-__global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_kernel(const GemmArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, (EPI == 3 && WM * WN == 4) ? 2 : (WM * WN) / 4) void gemm_kernel(const GemmArgs g) {
   constexpr bool CONV = MODE != 0;
   constexpr int THREADS = 64 * WM * WN;
   constexpr int BM = 16 * MT * WM;
@@ -881,7 +968,10 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_kernel(const
   // split-K: gridDim.y blocks share one output tile, block y reduces K-tiles [kt_lo, kt_hi) into its own fp32
   // partial (the launcher points g.out at the workspace); gridDim.y == 1 is the ordinary case
   const int kt_lo = (int)(((int64_t)g.nkt * blockIdx.y) / gridDim.y);
-  const int kt_hi = (int)(((int64_t)g.nkt * (blockIdx.y + 1)) / gridDim.y);
+  int kt_hi = (int)(((int64_t)g.nkt * (blockIdx.y + 1)) / gridDim.y);
+  // EPI 3: the K-tiles behind g.nkt are the low-rank product of the tile's one adapter
+  [[maybe_unused]] int ad_rows[(BM + 63) / 64], tile_ad = -1;
+  if constexpr (EPI == 3) adapter_rows<(BM + 63) / 64>(g, M0, lane, ad_rows);
 
   // MODE 2 loader (the nearest-neighbour gather needs a per-tap source coordinate): issue the LOADS DMAs of K-tile kt
   // into ring slot `slot` (kt >= kt_hi: all-zero DMAs keep the counts uniform)
@@ -1016,6 +1106,16 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_kernel(const
         soffW = (unsigned)(ntaps * g.Cin) * 2u + soffA;
         ragged_now = ragged2 && ld_chunk == g.chunks2 - 1;
       }
+    } else if (EPI == 3 && ld_kt >= g.nkt) {  // (uniform) the low-rank K-tiles
+      const int kk = (ld_kt - g.nkt) * BK + sc * 8, ku = adapter_rank_of(g, kk);
+      const bool ok = kk < g.ad_cols;
+      seg2 = true;
+      soffA = soffW = 0;
+      ragged_now = false;
+#pragma unroll
+      for (int j = 0; j < NAJ; ++j) offA[j] = ok && a_ok[j] ? (unsigned)((M0 + srow + PASS * j) * g.ad_ld + kk) * 2u : OOBA;
+#pragma unroll
+      for (int j = 0; j < NBJ; ++j) offB[j] = ok && fb_base[j] != OOBA ? (unsigned)((N0 + srow + PASS * j) * g.ad_rank + ku) * 2u : OOBA;
     } else {
 #pragma unroll
       for (int j = 0; j < NAJ; ++j) offA[j] = a_base[j];
@@ -1036,11 +1136,12 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_kernel(const
       for (int j = 0; j < NBJ; ++j) offB[j] = OOBA;
     }
     const unsigned slot_base = smem_base + 16u * (unsigned)(slot * STAGE);
-    const i32x4 rsel = seg2 ? rA2 : rA1;
+    const i32x4 rsel = EPI == 3 && seg2 ? make_rsrc(g.ad_low, (unsigned)(g.M * g.ad_ld * 2)) : seg2 ? rA2 : rA1;
+    const i32x4 rwsel = EPI == 3 && seg2 ? make_rsrc(g.ad_up + (int64_t)tile_ad * g.N * g.ad_rank, (unsigned)(g.N * g.ad_rank * 2)) : rW;
 #pragma unroll
     for (int j = 0; j < NAJ; ++j) dma_s(rsel, offA[j], soffA, slot_base + 16u * ((wave_u * 8 + PASS * j) * 8));
 #pragma unroll
-    for (int j = 0; j < NBJ; ++j) dma_s(rW, offB[j], soffW, slot_base + 16u * ((BM + b_row0[j]) * 8));
+    for (int j = 0; j < NBJ; ++j) dma_s(rwsel, offB[j], soffW, slot_base + 16u * ((BM + b_row0[j]) * 8));
     // advance the cursor
     ++ld_kt;
     if (CONV) {
@@ -1120,6 +1221,10 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_kernel(const
       row_stats_finish(g, BM, BN, tid, rsq, csq, mr, mr + 2 * BM);
     }
   }
+  if constexpr (EPI == 3) {  // (requested before K-tile 0, whose arrival the first step waits for anyway)
+    tile_ad = adapter_vote<(BM + 63) / 64>(ad_rows);
+    if (tile_ad >= 0) kt_hi += (g.ad_cols + BK - 1) / BK;
+  }
   for (int kt = kt_lo; kt < kt_hi; kt += NSTAGE) {
     step(IC<0>{}, kt);
     if (kt + 1 < kt_hi) step(IC<1 % NSTAGE>{}, kt + 1);
@@ -1131,7 +1236,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_kernel(const
   if constexpr (EPI == 1) {
     tile_epilogue_ln<DT, NR, MT, BM, WN>(g, acc, M0, wm, wn, lg, li, reinterpret_cast<float*>(&smem[NSTAGE * STAGE]));
   } else if constexpr (EPI == 3) {
-    tile_adapter<DT, NR, MT>(g, acc, M0, N0, wm, wn, lg, li);
+    if (tile_ad == -2) tile_adapter<DT, NR, MT>(g, acc, M0, N0, wm, wn, lg, li);
     tile_epilogue<DT, NR, MT, BM, true>(g, acc, M0, N0, wm, wn, lg, li, 0u);
   } else if constexpr (EPI == 2) {  // LayerNorm folded into the consumer: the instantiations that carry its two halves
     if (g.a_row_stats) {
@@ -1319,7 +1424,6 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void gemm_dense_persis
     if constexpr (EPI == 1) {
       tile_epilogue_ln<DT, NR, MT, BM, WN>(g, acc, M0, wm, wn, lg_, li_, reinterpret_cast<float*>(&smem[2 * STAGE]));
     } else {
-      if constexpr (EPI == 3) tile_adapter<DT, NR, MT>(g, acc, M0, N0, wm, wn, lg_, li_);
       tile_epilogue<DT, NR, MT, BM, (WM * WN <= 8)>(g, acc, M0, N0, wm, wn, lg_, li_, 0u);
     }
     MIMO_TRACE(g, tr, 6);
@@ -1375,7 +1479,9 @@ __global__ __launch_bounds__(512, 2) void gemm8_kernel(const GemmArgs g) {
   }
   const int64_t M0 = (int64_t)tile_m * BM;
   const int N0 = (int)tile_n * BN;
-  const int nkt = g.nkt;  // even (host)
+  int nkt = g.nkt;  // even (host; EPI 3: any)
+  [[maybe_unused]] int ad_rows[4], tile_ad = -1;
+  if constexpr (EPI == 3) adapter_rows<4>(g, M0, lane, ad_rows);
   [[maybe_unused]] u32x4 rsq[EPI == 2 ? ROW_STAT_LOADS : 1], csq;
   if constexpr (EPI == 2) row_stats_issue(g, M0, N0, BM, BN, tid, rsq, csq);   // (all out of range without a_row_stats)
 
@@ -1409,6 +1515,20 @@ __global__ __launch_bounds__(512, 2) void gemm8_kernel(const GemmArgs g) {
   };
   // half-tile (operand o, half h) of K-tile kt into parity d: two DMAs per thread
   auto stage = [&](int o, int h, int kt, int d) {
+    if constexpr (EPI == 3) {
+      if (kt >= g.nkt && kt < nkt) {  // (uniform) a low-rank K-tile: rows of low, of the adapter's up
+        const int kk = (kt - g.nkt) * BK + (int)lc * 8, ku = adapter_rank_of(g, kk);
+        const int64_t first = (o ? (int64_t)N0 : M0) + 128 * h, rows = (o ? (int64_t)g.N : g.M) - first;
+        const int pitch = o ? g.ad_rank : g.ad_ld;
+        const i32x4 x = make_rsrc((o ? g.ad_up + (int64_t)tile_ad * g.N * g.ad_rank : g.ad_low) + first * pitch,
+                                  rows > 0 ? (unsigned)((rows < 128 ? rows : 128) * pitch * 2) : 0u);
+        const unsigned v = kk < g.ad_cols ? (unsigned)((int)srow * pitch + (o ? ku : kk)) * 2u : 0x80000000u;
+        const unsigned base = smem_base + (unsigned)(((d * 2 + o) * 2 + h) * HTB) + wave_u * 1024u;
+        dma(x, v, 0u, base);
+        dma(x, v + (unsigned)(pitch * 128), 0u, base + 8192u);
+        return;
+      }
+    }
     i32x4 r = o ? rB[h] : rA[h];
     r.z = kt < nkt ? r.z : 0;  // past the end: zero fill keeps the DMA counts uniform
     const unsigned soff = kt < nkt ? (unsigned)kt * 128u : 0u;
@@ -1480,6 +1600,10 @@ __global__ __launch_bounds__(512, 2) void gemm8_kernel(const GemmArgs g) {
       row_stats_finish(g, BM, BN, tid, rsq, csq, mr, mr + 2 * BM);
     }
   }
+  if constexpr (EPI == 3) {
+    tile_ad = adapter_vote<4>(ad_rows);
+    if (tile_ad >= 0) nkt += (g.ad_cols + BK - 1) / BK;
+  }
   stage(0, 0, 1, 1); stage(0, 1, 1, 1);
   asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
   if (wr == 1) asm volatile("s_barrier" ::: "memory");  // group 1 runs one barrier behind group 0 from here on
@@ -1515,11 +1639,13 @@ __global__ __launch_bounds__(512, 2) void gemm8_kernel(const GemmArgs g) {
   };
   for (int t = 0; t < nkt; t += 2) {
     ktile(IC<0>{}, t);
-    ktile(IC<1>{}, t + 1);
+    if (EPI != 3 || t + 1 < nkt) ktile(IC<1>{}, t + 1);
   }
   if (wr == 0) asm volatile("s_barrier" ::: "memory");
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the trailing zero-fill DMAs must not outlive the block's LDS
-  if constexpr (EPI == 3) tile_adapter<DT, NR, MT>(g, acc, M0, N0, wr, wc, lg, li);
+  if constexpr (EPI == 3) {
+    if (tile_ad == -2) tile_adapter<DT, NR, MT>(g, acc, M0, N0, wr, wc, lg, li);
+  }
   if constexpr (EPI == 2) {
     if (g.a_row_stats) {
       const float* mr = reinterpret_cast<const float*>(lds + 8 * HTB);

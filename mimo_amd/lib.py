@@ -63,7 +63,7 @@ SIGNATURES = {
                       c_vp, c_sz, ctypes.POINTER(EpilogueExt), c_vp],
     "mimo_adapter_gemm": [c_i, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i, c_i, c_vp, c_vp, c_i64, c_u, ctypes.POINTER(AdapterParams),
                           c_vp, c_i, c_vp],
-    "mimo_adapter_gemm_backward_workspace": [ctypes.POINTER(AdapterParams), c_i64, c_i, c_i],
+    "mimo_adapter_gemm_backward_workspace": [c_i, ctypes.POINTER(AdapterParams), c_i64, c_i, c_i],
     "mimo_adapter_gemm_backward": [c_i, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i, c_i, ctypes.POINTER(AdapterParams),
                                    c_vp, c_vp, c_vp, c_vp, c_sz, c_vp],
     "mimo_conv2d": [c_i, c_vp, c_vp, c_vp, c_vp, ctypes.POINTER(ConvParams), c_vp, c_vp, c_vp, c_f, c_u, c_vp, c_sz, c_vp],

@@ -393,6 +393,10 @@ def _adapter_params(a, w, down, up, index, rows_per_index, scale, w_shape):
     return L.AdapterParams(down.data_ptr(), up.data_ptr(), _ptr(scale), index.data_ptr(), rows_per_index, S, r)
 
 
+# the low-rank values of adapter_gemm with nothing lost: value + remainder planes of the operand type (fp16 22, bf16 24 mantissa bits)
+LOW_PLANES = {torch.float16: 2, torch.bfloat16: 3}
+
+
 def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=None, residual=None, out_f32=False, want_low=False):
     """out[M, N] = a @ w^T + bias + residual + (scale[i] a @ down[i]^T) @ up[i]^T, i = index[m // rows_per_index]: a shared projection
     with the low-rank adapter of each row's request added in the same pass over the output.
@@ -401,7 +405,7 @@ def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=No
     packing.pack_adapters pads and stacks checkpoints of any rank); index: int32 device tensor, one entry per rows_per_index
     consecutive rows, in any order; an entry outside [0, S) (use -1) means no adapter.  scale: fp32 [S] (None: 1); bias: fp32 [N];
     residual: fp32 or half [M, N].  Returns half, or fp32 with out_f32.
-    want_low: returns (out, low), low half [M, 2 r] = the rows' scaled low-rank values as hi | lo halves, for the backward."""
+    want_low: returns (out, low), low half [M, LOW_PLANES r] = the rows' scaled low-rank values, value and remainders, for the backward."""
     p = _adapter_params(a, w, down, up, index, rows_per_index, scale, lambda N, K: (N, K))
     M, K = a.shape
     N, r = w.shape[0], p.rank
@@ -414,7 +418,7 @@ def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=No
     split = bool(want_low or out_f32)
     with _on_device(a.device):
         out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_f32 else a.dtype)
-        low = torch.empty((M, 2 * r if split else r), device=a.device, dtype=a.dtype)
+        low = torch.empty((M, LOW_PLANES[a.dtype] * r if split else r), device=a.device, dtype=a.dtype)
         if M:
             fl = 2 * M * N * K + 2 * M * r * (N + K)
             _count(fl)
@@ -436,8 +440,8 @@ def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=
     N, r, S = up.shape[1], p.rank, p.count
     _require(dout.shape == (M, N) and dout.dtype == a.dtype and dout.device == a.device, f"dout: {a.dtype} [{M}, {N}]")
     _rows_ok(dout, "dout")
-    _require(low.shape == (M, 2 * r) and low.dtype == a.dtype and low.device == a.device and low.is_contiguous() and
-             low.data_ptr() % 16 == 0, f"low: the forward's [{M}, {2 * r}] (want_low=True)")
+    _require(low.shape == (M, LOW_PLANES[a.dtype] * r) and low.dtype == a.dtype and low.device == a.device and low.is_contiguous() and
+             low.data_ptr() % 16 == 0, f"low: the forward's [{M}, {LOW_PLANES[a.dtype] * r}] (want_low=True)")
     with _on_device(a.device):
         da = torch.empty((M, K), device=a.device, dtype=a.dtype) if want_da else None
         if not M:
@@ -446,7 +450,7 @@ def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=
         dup = torch.empty((S, N, r), device=a.device, dtype=torch.float32)
         fl = (2 * M * N * K if want_da else 0) + 2 * M * r * (2 * N + 2 * K)
         _count(fl)
-        nb = L.load().mimo_adapter_gemm_backward_workspace(ctypes.byref(p), M, N, K)
+        nb = L.load().mimo_adapter_gemm_backward_workspace(dt_code(a.dtype), ctypes.byref(p), M, N, K)
         ws = torch.empty(((nb + 3) // 4,), device=a.device, dtype=torch.float32)
         with _Bracket("gemm_kernel", fl, _nbytes(dout, a, w_t, da, ddown, dup), f"adapter_gemm_backward M{M} N{N} K{K} r{r}"):
             L.call("mimo_adapter_gemm_backward", dt_code(a.dtype), dout.data_ptr(), _ld(dout), a.data_ptr(), _ld(a),

@@ -2,8 +2,9 @@
 the formulas in 64 bits, element by element, under bounds that count the kernels' own roundings.
 
 With u = eps / 2 of the operand type: a 16-bit result rounds the low-rank values once and the result once, so
-|error| <= u (sum_j |low_j up_j| + |out|); where the low-rank values are kept as hi + lo halves they are off by u^2 (and 2^-25
-absolutely where an fp16 half is below its normal range).  Sums are fp32: n terms are off by at most n 2^-24 of the sum of their
+|error| <= u (sum_j |low_j up_j| + |out|); where the low-rank values are kept as planes they are off by u^2 (fp16: two planes) or
+u^3 (bf16: three), and by 2^-25 absolutely where an fp16 remainder is below its normal range (2^-36 in the gradient's t, whose
+remainder plane is scaled by 2^11).  Sums are fp32: n terms are off by at most n 2^-24 of the sum of their
 magnitudes, taken here as sqrt(n) + 8 steps, which a random walk of that many roundings does not pass (each is at most half a
 step of the running sum)."""
 import ctypes
@@ -44,6 +45,7 @@ def reference(a, w, down, up, who, scale, bias, residual, out_f32, dout=None):
     absbase = A.abs() @ W.t().abs()
     low, lowabs = (torch.zeros((M, r), dtype=torch.float64, device=a.device) for _ in range(2))
     add, addabs, addlow = (torch.zeros((M, N), dtype=torch.float64, device=a.device) for _ in range(3))
+    p = u * u if dt == torch.float16 else u ** 3
     res = {}
     if dout is not None:
         dY = dout.double()
@@ -60,7 +62,7 @@ def reference(a, w, down, up, who, scale, bias, residual, out_f32, dout=None):
         lowabs[at] = s * A[at].abs() @ D[i].t().abs()
         add[at] = low[at] @ U[i].t()
         addabs[at] = low[at].abs() @ U[i].t().abs()
-        elow = acc(K) * lowabs[at] + (u * u * low[at].abs() + tiny if out_f32 else u * low[at].abs() + tiny)
+        elow = acc(K) * lowabs[at] + (p * low[at].abs() + tiny if out_f32 else u * low[at].abs() + tiny)
         addlow[at] = elow @ U[i].t().abs()
         if dout is None:
             continue
@@ -69,8 +71,8 @@ def reference(a, w, down, up, who, scale, bias, residual, out_f32, dout=None):
         da[at] = t[at] @ D[i]
         dalow[at] = (u * t[at].abs() + tiny + acc(N) * tabs[at]) @ D[i].abs()
         daabs[at] = t[at].abs() @ D[i].abs()
-        e_t = acc(N) * tabs[at] + u * u * t[at].abs() + tiny     # hi + lo halves
-        e_u = acc(K) * lowabs[at] + u * u * low[at].abs() + tiny
+        e_t = acc(N) * tabs[at] + p * t[at].abs() + tiny * 2.0 ** -11
+        e_u = acc(K) * lowabs[at] + p * low[at].abs() + tiny
         n = acc(at.numel())
         ddown[i] = t[at].t() @ A[at]
         eddown[i] = (e_t + n * t[at].abs()).t() @ A[at].abs()
@@ -340,7 +342,7 @@ def test_c_entry_refuses_what_it_cannot_run():
     for kw in (dict(down=None), dict(up=4100), dict(index=None), dict(index=4098), dict(rows_per_index=0), dict(count=0), dict(count=70000),
                dict(rank=0), dict(rank=12), dict(rank=136)):
         assert fwd(params(**kw)) == -1 and bwd(params(**kw)) == -1, kw
-        assert L.mimo_adapter_gemm_backward_workspace(ctypes.byref(params(**kw)), 8, 64, 64) == 0
+        assert L.mimo_adapter_gemm_backward_workspace(lib.F16, ctypes.byref(params(**kw)), 8, 64, 64) == 0
     for kw in (dict(M=0), dict(N=60), dict(K=12), dict(N=1 << 16, K=1 << 16)):
         assert fwd(**kw) == -1 and bwd(**kw) == -1, kw
     assert fwd(A=None) == -1 and fwd(A=4104) == -1 and fwd(lda=68) == -1 and fwd(ldo=66) == -1 and fwd(res=4096, ldr=2) == -1
