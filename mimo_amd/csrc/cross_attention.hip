@@ -42,63 +42,76 @@ struct IC {
   static constexpr int value = V;
 };
 
-constexpr int CH = 64;          // keys per streamed buffer
-constexpr int RES_LDS = 80000;  // resident keys: two blocks per CU
+// keys per streamed buffer: what a thread can hold on its way
+constexpr int stream_keys(int ks, int nw) { return ks >= 8 || (nw == 1 && ks > 4) ? 32 : 64; }
 
-inline int lds_of(int ks, bool resident, int nk) { return resident ? kv_lds(ks, (nk + 31) / 32 * 32) : 2 * kv_lds(ks, CH); }
+constexpr float LAG = 8.f;  // log2 units by which a row's maximum may pass its reference before the row is rescaled
 
-template <int DT, int KS, bool RESIDENT, int NW>
-__global__ __launch_bounds__(64 * NW, KS <= 4 ? 3 : 2) void xattn_kernel(const Args a) {
+// RESIDENT: all keys of (e, g) staged once; NW = 4 (two or more blocks per CU) or 8 (one).  Else: streamed in chunks of CHK keys
+// through two buffers, NW = 4 or 1 waves that share them.
+template <int DT, int KS, bool RESIDENT, int NW, int CHK>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS <= 3 && NW > 1) || KS == 2 || (KS == 4 && RESIDENT) ? 3 : 2) void xattn_kernel(const Args a) {
   constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h2 = lane >> 5, li = lane & 31;
-  // consecutive blocks of an XCD are the key heads of the same query rows: they read the same lines of q
+  // consecutive blocks of an XCD are the key heads of the same query rows: they share the lines of q and out; then come the encoder
+  // rows, whose lengths differ: every XCD gets some of each
   const unsigned L = xcd_remap(blockIdx.x, gridDim.x);
   const int g = (int)(L % (unsigned)a.kvh);
-  const int j = (int)(L / (unsigned)a.kvh) % a.nb, e = (int)(L / (unsigned)a.kvh) / a.nb;
+  const int e = (int)(L / (unsigned)a.kvh) % a.Be, j = (int)(L / (unsigned)a.kvh) / a.Be;
   const int len = valid_len(a, e);
   const int T = (a.R + 31) >> 5;  // query tiles of this (e, g)
   // keys of this part
-  const int per = ((len + CH - 1) / CH + a.nsplit - 1) / a.nsplit * CH;
+  const int per = ((len + CHK - 1) / CHK + a.nsplit - 1) / a.nsplit * CHK;
   const int k_lo = min(len, (int)blockIdx.y * per), k_hi = min(len, k_lo + per);
-  const int nkeys = k_hi - k_lo;
+  const bool ones = (a.d & 31) != 0;  // the last channel tile has a row to spare: the sum of P comes with the product
 
-  const int npad = RESIDENT ? (a.Nk + 31) / 32 * 32 : CH;
-  uint16_t* const ks0 = reinterpret_cast<uint16_t*>(smem);
-  uint16_t* const vs0 = ks0 + npad * P;
-  float* const bias0 = reinterpret_cast<float*>(smem + 2 * npad * P * 2 + 64);
+  const int npad = RESIDENT ? (a.Nk + 31) / 32 * 32 : CHK;
   const int stride = kv_lds(KS, npad);  // bytes between the two streamed buffers
+  auto ks_of = [&](int b) { return reinterpret_cast<uint16_t*>(smem + b * stride); };
+  auto vs_of = [&](int b) { return reinterpret_cast<uint16_t*>(smem + b * stride) + npad * P; };
+  auto bias_of = [&](int b) { return reinterpret_cast<float*>(smem + b * stride + 2 * npad * P * 2 + 64); };
 
+  Stager<KS, THREADS, CHK> stager;
+  stager.open(a, e, g);
   if constexpr (RESIDENT) {
-    stage_kv<KS, THREADS>(a, e, g, len, 0, (len + 31) / 32 * 32, ks0, vs0, bias0, tid);
+    stage_all<DT, KS, THREADS>(a, e, g, len, ks_of(0), vs_of(0), bias_of(0), ones, tid);
     __syncthreads();
   }
-  // a streamed block's waves share its key buffers: all of them walk the same number of tiles
   const int step = a.nb * NW;
   int t = j * NW + wave;
-  const int rounds = RESIDENT ? 0 : (T - j * NW + step - 1) / step;
+  // a streamed block's waves share its key buffers: all of them walk the same number of tiles
+  const int rounds = (T - j * NW + step - 1) / step;
 
-  uint4 qf[KS], qn[KS];
-  auto query = [&](int tt, uint4 (&f)[KS]) {
+  uint4 qf[KS], qn[RESIDENT ? KS : 1];
+  auto query = [&](int tt, auto& f) {
     int img, qi, hh;
     flat_row(a, min(32 * tt + li, a.R - 1), img, qi, hh);
     load_row<KS>(f, a.q + ((int64_t)e * a.G + img) * a.sqb + (int64_t)qi * a.sqr + (int64_t)(g * a.hg + hh) * a.d, a.d, h2);
   };
-  if (t < T) query(t, qn);
+  if constexpr (RESIDENT) {
+    if (t < T) query(t, qn);
+  }
 
   for (int round = 0; RESIDENT ? t < T : round < rounds; t += step, ++round) {
+    if constexpr (RESIDENT) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = qn[s];
-    if (t + step < T) query(t + step, qn);
+      for (int s = 0; s < KS; ++s) qf[s] = qn[s];
+      if (t + step < T) query(t + step, qn);
+    } else {
+      query(min(t, T - 1), qf);
+    }
     f32x16 ot[OT];
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) ot[i][r] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
+    // m_ref: the maximum that P is taken against.  It follows the running maximum only when that passes it by LAG (P then stays
+    // below 2^LAG: the same arithmetic, far fewer rescalings); sum: this lane's half of the keys
+    float m_ref = -INFINITY, sum = 0.f;
 
-    // two 32-key tiles at LDS rows kr.. (n = how many of them hold keys)
+    // two or one 32-key tiles at LDS rows kr..
     auto tiles = [&](const uint16_t* ks, const uint16_t* vs, const float* bias, int kr, auto n_c, bool masked) {
       constexpr int n = decltype(n_c)::value;
       f32x16 st[n];
@@ -126,27 +139,29 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 ? 3 : 2) void xattn_kernel(const A
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[u][r]);
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-      const float m_new = fmaxf(m_run, mt);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // nothing but masked keys so far: exp2(-inf) below
-      if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0ull) {
-        const float alpha = fast_exp2((m_run - m_use) * a.c);
-        l_run *= alpha;
+      const bool move = mt > m_ref + a.lag;  // (m_ref = -inf: any finite maximum)
+      if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
+        const float alpha = move ? fast_exp2((m_ref - mt) * a.c) : 1.f;  // m_ref = -inf: 0
+        m_ref = move ? mt : m_ref;
+        sum *= alpha;
 #pragma unroll
         for (int i = 0; i < OT; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) ot[i][r] *= alpha;
       }
-      m_run = m_new;
-      const float mc = -m_use * a.c;
-      float ps = 0.f;
+      const float mc = m_ref == -INFINITY ? 0.f : -m_ref * a.c;  // nothing but masked keys so far: exp2(-inf)
 #pragma unroll
       for (int u = 0; u < n; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          st[u][r] = fast_exp2(fmaf(st[u][r], a.c, mc));
-          ps += st[u][r];
-        }
-      l_run += ps;  // this lane's half of the keys; the halves meet at the end
+        for (int r = 0; r < 16; ++r) st[u][r] = fast_exp2(fmaf(st[u][r], a.c, mc));
+      if (!ones || a.lse) {
+        float ps = 0.f;
+#pragma unroll
+        for (int u = 0; u < n; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) ps += st[u][r];
+        sum += ps;
+      }
 #pragma unroll
       for (int u = 0; u < 2 * n; ++u) {
         const uint4 pf = pack_k<DT>(st[u >> 1], u & 1);
@@ -156,34 +171,42 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 ? 3 : 2) void xattn_kernel(const A
     };
     if constexpr (RESIDENT) {
       int kr = 0;
-      for (; kr + 32 < len; kr += 64) tiles(ks0, vs0, bias0, kr, IC<2>{}, a.mask || kr + 64 > len);
-      if (kr < len) tiles(ks0, vs0, bias0, kr, IC<1>{}, a.mask || kr + 32 > len);
+      for (; kr + 32 < len; kr += 64) tiles(ks_of(0), vs_of(0), bias_of(0), kr, IC<2>{}, a.mask || kr + 64 > len);
+      if (kr < len) tiles(ks_of(0), vs_of(0), bias_of(0), kr, IC<1>{}, a.mask || kr + 32 > len);
     } else {
-      // buffer b holds chunk i (i & 1 == b); the other one is filled while this one is used, one barrier per chunk
-      const int chunks = (nkeys + CH - 1) / CH;
-      __syncthreads();  // the previous round's last chunk is read
-      if (chunks > 0) stage_kv<KS, THREADS>(a, e, g, k_hi, k_lo, CH, ks0, vs0, bias0, tid);
+      // chunk i is in buffer i & 1; while it is used the next one is on its way into registers and then into the other buffer:
+      // one barrier per chunk
+      const int chunks = (k_hi - k_lo + CHK - 1) / CHK;
+      if (chunks > 0) {
+        stager.issue(a, e, k_hi, k_lo, tid);
+        if (round > 0) __syncthreads();  // the previous round's last chunk is read
+        stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), ones, tid);
+        if (chunks > 1) stager.issue(a, e, k_hi, k_lo + CHK, tid);
+      }
       for (int i = 0; i < chunks; ++i) {
         __syncthreads();
-        const int off = (i & 1) * stride, nxt = ((i + 1) & 1) * stride;
-        auto at = [&](const void* p, int o) { return (unsigned char*)p + o; };
-        if (i + 1 < chunks)
-          stage_kv<KS, THREADS>(a, e, g, k_hi, k_lo + (i + 1) * CH, CH, (uint16_t*)at(ks0, nxt), (uint16_t*)at(vs0, nxt),
-                                (float*)at(bias0, nxt), tid);
-        if (t < T)
-          tiles((const uint16_t*)at(ks0, off), (const uint16_t*)at(vs0, off), (const float*)at(bias0, off), 0, IC<2>{},
-                a.mask || (i + 1) * CH > nkeys);
+        const int b = i & 1;
+        if (t < T) tiles(ks_of(b), vs_of(b), bias_of(b), 0, IC<CHK / 32>{}, a.mask || k_lo + (i + 1) * CHK > k_hi);
+        if (i + 1 < chunks) {
+          stager.template commit<DT>(a, ks_of(b ^ 1), vs_of(b ^ 1), bias_of(b ^ 1), ones, tid);
+          if (i + 2 < chunks) stager.issue(a, e, k_hi, k_lo + (i + 2) * CHK, tid);
+        }
       }
     }
     if (t >= T) continue;
-    l_run += __shfl_xor(l_run, 32, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    float l = sum;  // what the output is divided by: the sum of the P that were multiplied, where it came with them
+    if (ones) {
+      const int r = (a.d & 31) >> 3;  // row d of O^T: register 4 r of the last tile, lanes 0..31
+      l = __shfl(r == 1 ? ot[OT - 1][4] : r == 2 ? ot[OT - 1][8] : ot[OT - 1][12], li, 64);
+    }
     const int f = 32 * t + li;
     const bool live = f < a.R;
     int img, qi, hh;
     flat_row(a, min(f, a.R - 1), img, qi, hh);
     const int head = g * a.hg + hh;
     const int64_t b = (int64_t)e * a.G + img;
-    if (a.nsplit > 1) {  // partial: unnormalised rows, then (reference maximum in log2 units, sum)
+    if (a.nsplit > 1) {  // partial: unnormalised rows, then (reference maximum in log2 units, divisor, sum)
       const int64_t row = (((int64_t)blockIdx.y * a.Be + e) * a.kvh + g) * a.R + f;
       float* po = a.ws + row * a.d;
       if (live) {
@@ -194,103 +217,130 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 ? 3 : 2) void xattn_kernel(const A
             const int d0 = 32 * i + 8 * c + 4 * h2;
             if (d0 < a.d) *reinterpret_cast<f32x4*>(po + d0) = (f32x4){ot[i][4 * c], ot[i][4 * c + 1], ot[i][4 * c + 2], ot[i][4 * c + 3]};
           }
-        if (h2 == 0) {
-          float* ml = a.ws + (int64_t)a.nsplit * a.Be * a.kvh * a.R * a.d + 2 * row;
-          ml[0] = m_run * a.c;
-          ml[1] = l_run;
-        }
+        if (h2 == 0)
+          *reinterpret_cast<f32x4*>(a.ws + (int64_t)a.nsplit * a.Be * a.kvh * a.R * a.d + 4 * row) = (f32x4){m_ref * a.c, l, sum, 0.f};
       }
       continue;
     }
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
     uint16_t* p = a.out + b * a.sob + (int64_t)qi * a.sor + (int64_t)head * a.d;
 #pragma unroll
     for (int i = 0; i < OT; ++i) store_tile<DT>(ot[i], inv, p, live, i, a.d, h2);
     if (a.lse && live && h2 == 0)
-      a.lse[(b * a.kvh * a.hg + head) * a.Nq + qi] = l_run > 0.f ? m_run * a.scale + logf(l_run) : -INFINITY;
+      a.lse[(b * a.kvh * a.hg + head) * a.Nq + qi] = sum > 0.f ? m_ref * a.scale + logf(sum) : -INFINITY;
   }
 }
 
-// joins the parts of the keys: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, parts in order.  One thread per row and four
-// channels.
+// joins the parts of the keys: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, parts in order.  A block takes 1024 / d rows
+// (d / 4 threads each), the parts' (m, l, sum) pass through LDS once.
 template <int DT>
 __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a) {
-  const int d4 = a.d >> 2;
-  const int64_t rows = (int64_t)a.Be * a.kvh * a.R, total = rows * d4;
-  const float* mls = a.ws + (int64_t)a.nsplit * rows * a.d;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / d4;
-    const int c = (int)(i - row * d4) * 4;
-    float m = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, mls[2 * ((int64_t)s * rows + row)]);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float* ml = mls + 2 * ((int64_t)s * rows + row);
-      const float w = fast_exp2(ml[0] - mu);
-      l = fmaf(w, ml[1], l);
-      o += *reinterpret_cast<const f32x4*>(a.ws + ((int64_t)s * rows + row) * a.d + c) * w;
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int64_t eg = row / a.R;
-    const int g = (int)(eg % a.kvh);
-    int img, qi, hh;
-    flat_row(a, (int)(row - eg * a.R), img, qi, hh);
-    const int64_t b = eg / a.kvh * a.G + img;
-    const int head = g * a.hg + hh;
-    *reinterpret_cast<uint2*>(a.out + b * a.sob + (int64_t)qi * a.sor + (int64_t)head * a.d + c) =
-        make_uint2(pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv));
-    if (a.lse && c == 0) a.lse[(b * a.kvh * a.hg + head) * a.Nq + qi] = l > 0.f ? (mu + log2f(l)) * LN2 : -INFINITY;
+  __shared__ f32x4 part[32 * 64];  // [rows of the block][parts]
+  const int d4 = a.d >> 2, per = 256 / d4 < 32 ? 256 / d4 : 32, n = a.nsplit;
+  const int64_t rows = (int64_t)a.Be * a.kvh * a.R, row0 = (int64_t)blockIdx.x * per;
+  const f32x4* mls = reinterpret_cast<const f32x4*>(a.ws + (int64_t)n * rows * a.d);
+  for (int i = threadIdx.x; i < per * n; i += 256) {
+    const int s = i / per, r = i - s * per;
+    if (row0 + r < rows) part[r * n + s] = mls[(int64_t)s * rows + row0 + r];
   }
+  const int r = threadIdx.x / d4, c = (threadIdx.x - r * d4) * 4;
+  const int64_t row = row0 + r;
+  const bool mine = r < per && row < rows;
+  f32x4 x[8];
+  const float* src = a.ws + row * a.d + c;
+  if (mine) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s < n) x[s] = *reinterpret_cast<const f32x4*>(src + (int64_t)s * rows * a.d);
+  }
+  __syncthreads();
+  if (!mine) return;
+  float m = -INFINITY;
+  for (int s = 0; s < n; ++s) m = fmaxf(m, part[r * n + s][0]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f, sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < n; s0 += 8) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s0 + s < n) {
+        const f32x4 q = part[r * n + s0 + s];
+        const float w = fast_exp2(q[0] - mu);
+        l = fmaf(w, q[1], l);
+        sum = fmaf(w, q[2], sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(w, x[s][i], o[i]);
+      }
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s0 + 8 + s < n) x[s] = *reinterpret_cast<const f32x4*>(src + (int64_t)(s0 + 8 + s) * rows * a.d);
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int64_t eg = row / a.R;
+  const int g = (int)(eg % a.kvh);
+  int img, qi, hh;
+  flat_row(a, (int)(row - eg * a.R), img, qi, hh);
+  const int64_t b = eg / a.kvh * a.G + img;
+  const int head = g * a.hg + hh;
+  *reinterpret_cast<uint2*>(a.out + b * a.sob + (int64_t)qi * a.sor + (int64_t)head * a.d + c) =
+      make_uint2(pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv));
+  if (a.lse && c == 0) a.lse[(b * a.kvh * a.hg + head) * a.Nq + qi] = sum > 0.f ? (mu + log2f(sum)) * LN2 : -INFINITY;
 }
 
 struct Plan {
   bool resident;
-  int nw, nb, nsplit, lds;
+  int nw, chk, nb, nsplit, lds;
 };
-// Resident keys while two blocks of them fit a CU.  Blocks: enough for three rounds of every CU at the LDS each takes, never
-// more than one per NW query tiles.  Streamed with one wave per block when one tile holds all queries (the other waves would
-// only wait), else four; the keys are cut while the blocks do not fill the chip and a part keeps at least 256 keys.
+// Resident keys while two blocks of them fit a CU (4 waves), or one block of 8 waves when there are query tiles for them; the
+// blocks are as many as are resident at once.  Streamed with one wave per block when one tile holds all queries (other waves
+// would only wait), else four.  The keys are cut into parts while not even half the chip has a block, a part keeping at least
+// 256 keys.
 Plan plan(const Args& a) {
   Plan p{};
-  const int ks = k_steps(a.d), cus = cu_count();
-  const int T = (a.R + 31) / 32;
-  p.resident = lds_of(ks, true, a.Nk) <= RES_LDS;
-  p.nw = (!p.resident && T == 1) ? 1 : 4;
-  p.lds = lds_of(ks, p.resident, a.Nk);
-  const int most = (T + p.nw - 1) / p.nw, eg = a.Be * a.kvh;
-  if (p.resident) {
-    const int want = 4 * cus;
-    p.nb = (want + eg - 1) / eg;
+  const int ks = k_steps(a.d), cus = cu_count(), eg = a.Be * a.kvh;
+  const int T = (a.R + 31) / 32, all = kv_lds(ks, (a.Nk + 63) / 64 * 64);
+  p.nsplit = 1;
+  if (all <= 80000 || (all <= 160000 && T >= 16)) {
+    p.resident = true;
+    p.nw = all <= 80000 ? 4 : 8;
+    p.chk = 32;
+    p.lds = all;
+    const int most = (T + p.nw - 1) / p.nw, fit = 160000 / (all > 1000 ? all : 1000), per_cu = p.nw == 8 ? 1 : fit < 4 ? fit : 4;
+    p.nb = (per_cu * cus + eg - 1) / eg;
     if (p.nb > most) p.nb = most;
-    p.nsplit = 1;
-  } else {
-    p.nb = most;
-    const int64_t blocks = (int64_t)eg * most, fill = p.nw == 1 ? 8 * cus : 2 * cus;
-    int64_t n = (fill + blocks - 1) / blocks;
+    return p;
+  }
+  p.nw = T == 1 ? 1 : 4;
+  p.chk = stream_keys(ks, p.nw);
+  p.lds = 2 * kv_lds(ks, p.chk);
+  p.nb = (T + p.nw - 1) / p.nw;
+  const int64_t blocks = (int64_t)eg * p.nb, fill = p.nw == 1 ? 4 * cus : cus;
+  if (2 * blocks <= fill) {
+    int64_t n = fill / blocks;
     const int parts = (a.Nk + 255) / 256;
     if (n > parts) n = parts;
-    if (n > 64) n = 64;
-    p.nsplit = n < 1 ? 1 : (int)n;
+    p.nsplit = n > 64 ? 64 : n < 1 ? 1 : (int)n;
   }
   return p;
 }
 
 size_t ws_bytes(const Args& a, const Plan& p) {
-  return p.nsplit > 1 ? (size_t)p.nsplit * a.Be * a.kvh * a.R * (a.d + 2) * sizeof(float) : 0;
+  return p.nsplit > 1 ? (size_t)p.nsplit * a.Be * a.kvh * a.R * (a.d + 4) * sizeof(float) : 0;
 }
 
 template <int DT, int KS>
 int launch(const Args& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)(a.Be * a.kvh) * (unsigned)p.nb, (unsigned)p.nsplit);
-  if (p.resident) hipLaunchKernelGGL((xattn_kernel<DT, KS, true, 4>), grid, dim3(256), p.lds, st, a);
-  else if (p.nw == 1) hipLaunchKernelGGL((xattn_kernel<DT, KS, false, 1>), grid, dim3(64), p.lds, st, a);
-  else hipLaunchKernelGGL((xattn_kernel<DT, KS, false, 4>), grid, dim3(256), p.lds, st, a);
+  constexpr int CH1 = stream_keys(KS, 1), CH4 = stream_keys(KS, 4);
+  if (p.resident && p.nw == 4) hipLaunchKernelGGL((xattn_kernel<DT, KS, true, 4, 32>), grid, dim3(256), p.lds, st, a);
+  else if (p.resident) hipLaunchKernelGGL((xattn_kernel<DT, KS, true, 8, 32>), grid, dim3(512), p.lds, st, a);
+  else if (p.nw == 1) hipLaunchKernelGGL((xattn_kernel<DT, KS, false, 1, CH1>), grid, dim3(64), p.lds, st, a);
+  else hipLaunchKernelGGL((xattn_kernel<DT, KS, false, 4, CH4>), grid, dim3(256), p.lds, st, a);
   MIMO_LAUNCH_CHECK();
   if (p.nsplit > 1) {
-    const int64_t total = (int64_t)a.Be * a.kvh * a.R * (a.d / 4), nwg = (total + 255) / 256;
-    hipLaunchKernelGGL((xattn_join_kernel<DT>), dim3((unsigned)(nwg > 4096 ? 4096 : nwg)), dim3(256), 0, st, a);
+    const int d4 = a.d / 4, per = 256 / d4 < 32 ? 256 / d4 : 32;
+    const int64_t rows = (int64_t)a.Be * a.kvh * a.R;
+    hipLaunchKernelGGL((xattn_join_kernel<DT>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a);
     MIMO_LAUNCH_CHECK();
   }
   return MIMO_OK;
@@ -324,7 +374,7 @@ extern "C" int mimo_cross_attention(int dtype, const void* q, const void* k, con
   if (!q || !out || (a.Nk > 0 && (!k || !v)) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return MIMO_EINVAL;
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v; a.out = (uint16_t*)out; a.lse = lse;
   const Plan pl = plan(a);
-  a.nb = pl.nb; a.nsplit = pl.nsplit;
+  a.nb = pl.nb; a.nsplit = pl.nsplit; a.lag = fminf(LAG / a.c, 1e30f);
   if (ws_bytes(a, pl) > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < ws_bytes(a, pl))) return MIMO_EINVAL;
   a.ws = (float*)workspace;
   if (dtype == MIMO_F16) return dispatch<MIMO_F16>(a, pl, (hipStream_t)stream);

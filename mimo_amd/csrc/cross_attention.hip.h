@@ -41,7 +41,7 @@ struct Args {
   int Be, G, Nq, Nk, kvh, hg, d, R;
   FastDiv by_hg, by_nq;
   float c;                       // scale * log2(e): scores leave the matrix unit unscaled
-  float scale;
+  float scale, lag;
   int nb;                        // blocks per (e, g)
   int nsplit;                    // parts the keys (forward, dq) or the flat rows (dk / dv) are cut into
 };
@@ -113,26 +113,83 @@ __device__ __forceinline__ void load_row(uint4 (&f)[KS], const uint16_t* p, int 
   }
 }
 
-// Key and value rows [key0, key0 + n) of (e, g) into row-major LDS tiles of pitch 16 KS + 8 halfs (an odd number of 16-byte
-// units: a 16-lane group of b128 row reads covers all banks).  Rows the mask drops and channels >= d are ZERO whatever memory
-// holds there (NaN included); bias[i] = 0 or -inf is added to their scores.
-template <int KS, int THREADS>
-__device__ __forceinline__ void stage_kv(const Args& a, int e, int g, int len, int key0, int n, uint16_t* ks, uint16_t* vs,
-                                         float* bias, int tid) {
-  constexpr int P = 16 * KS + 8, CH = 2 * KS;
-  const uint16_t* kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
-  const uint16_t* vb = a.v + (int64_t)e * a.svb + (int64_t)g * a.d;
-  for (int i = tid; i < n * CH; i += THREADS) {
-    const int row = i / CH, cc = (i - row * CH) * 8, key = key0 + row;
-    uint4 kv = make_uint4(0, 0, 0, 0), vv = make_uint4(0, 0, 0, 0);
-    if (cc < a.d && key_valid(a, e, len, key)) {
-      kv = *reinterpret_cast<const uint4*>(kb + (int64_t)key * a.skr + cc);
-      vv = *reinterpret_cast<const uint4*>(vb + (int64_t)key * a.svr + cc);
-    }
-    *reinterpret_cast<uint4*>(ks + row * P + cc) = kv;
-    *reinterpret_cast<uint4*>(vs + row * P + cc) = vv;
+// lanes per row of 16-byte chunks: a power of two, so that a thread keeps its column and walks rows at a fixed distance
+constexpr int lanes_of(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 8 : ks <= 8 ? 16 : 32; }
+
+// Key and value rows [key0, key0 + N) of (e, g) on their way into row-major LDS tiles of pitch 16 KS + 8 halfs (an odd number of
+// 16-byte units: a 16-lane group of b128 row reads covers all banks).  issue() requests the rows, commit() writes them: between
+// the two a block computes on other rows.  Only keys below len are read; what the mask drops, what lies behind len and channels
+// >= d are ZERO in LDS whatever memory holds there (NaN included), and bias[i] = 0 or -inf is added to their scores.
+// ones: V's channel d, which pads the last 32-channel tile, is 1 — the product with P then also leaves the sum of P in that row.
+template <int KS, int THREADS, int N>
+struct Stager {
+  static constexpr int P = 16 * KS + 8, LPR = lanes_of(KS), RP = THREADS / LPR, NC = (N + RP - 1) / RP;
+  uint4 kr[NC], vr[NC];
+  uint8_t keep;  // the mask's byte of key key0 + lane
+  int left;      // keys of this piece
+  const uint16_t *kb, *vb;
+  __device__ __forceinline__ void open(const Args& a, int e, int g) {
+    kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
+    vb = a.v + (int64_t)e * a.svb + (int64_t)g * a.d;
   }
-  for (int i = tid; i < n; i += THREADS) bias[i] = key_valid(a, e, len, key0 + i) ? 0.f : -INFINITY;
+  __device__ __forceinline__ void issue(const Args& a, int e, int len, int key0, int tid) {
+    asm volatile("" : "+v"(tid));  // addresses are made anew for every piece: kept over the products they would cost registers
+    const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
+    const uint16_t* kp = kb + (int64_t)(key0 + row0) * a.skr + cc;
+    const uint16_t* vp = vb + (int64_t)(key0 + row0) * a.svr + cc;
+    left = len - key0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+      if (cc < a.d && row0 + i * RP < left) {
+        kr[i] = *reinterpret_cast<const uint4*>(kp + (int64_t)(i * RP) * a.skr);
+        vr[i] = *reinterpret_cast<const uint4*>(vp + (int64_t)(i * RP) * a.svr);
+      }
+    }
+    static_assert(N <= 64, "a lane per key of the mask");
+    keep = 1;
+    if (a.mask && (tid & 63) < left) keep = a.mask[(int64_t)e * a.smb + key0 + (tid & 63)];
+  }
+  template <int DT>
+  __device__ __forceinline__ void commit(const Args& a, uint16_t* ks, uint16_t* vs, float* bias, bool ones, int tid) {
+    asm volatile("" : "+v"(tid));
+    const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
+    const unsigned long long live = __builtin_amdgcn_ballot_w64(keep != 0);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int row = row0 + i * RP;
+      if (cc < 16 * KS && (N % RP == 0 || row < N)) {
+        uint4 x = kr[i], y = vr[i];
+        if (a.mask && !((live >> row) & 1)) x = y = make_uint4(0, 0, 0, 0);
+        if (ones && cc == a.d) y.x = HT<DT>::from_f(1.f);
+        *reinterpret_cast<uint4*>(ks + row * P + cc) = x;
+        *reinterpret_cast<uint4*>(vs + row * P + cc) = y;
+      }
+    }
+    if (tid < N) {
+      bias[tid] = tid < left && keep ? 0.f : -INFINITY;
+      if (ones && a.d == 16 * KS) vs[tid * P + a.d] = HT<DT>::from_f(1.f);
+    }
+  }
+};
+
+// all keys of (e, g), 96 at a time on their way
+template <int DT, int KS, int THREADS>
+__device__ __forceinline__ void stage_all(const Args& a, int e, int g, int len, uint16_t* ks, uint16_t* vs, float* bias, bool ones, int tid) {
+  constexpr int P = 16 * KS + 8;
+  for (int k0 = 0; k0 < len; k0 += 96) {
+    Stager<KS, THREADS, 32> s[3];
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (k0 + 32 * u < len) {
+        s[u].open(a, e, g);
+        s[u].issue(a, e, len, k0 + 32 * u, tid);
+      }
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (k0 + 32 * u < len)
+        s[u].template commit<DT>(a, ks + (k0 + 32 * u) * P, vs + (k0 + 32 * u) * P, bias + k0 + 32 * u, ones, tid);
+  }
 }
 
 // bytes of LDS that n staged keys take (+ the transposed reads of the last row's last tile, which run up to 16 halfs past it)

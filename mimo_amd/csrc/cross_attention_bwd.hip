@@ -17,69 +17,95 @@
 namespace mimo_xattn {
 namespace {
 
-constexpr int CH = 64;
-constexpr int RES_LDS = 80000;
+constexpr int stream_keys(int ks) { return ks >= 6 ? 32 : 64; }  // keys per streamed buffer of dq
 
-template <int DT, int KS, bool RESIDENT>
-__global__ __launch_bounds__(256, KS <= 3 ? 3 : KS <= 6 ? 2 : 1) void xattn_dq_kernel(const Args a) {
-  constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 256;
+// RESIDENT: NW = 4 or 8 waves per block as in the forward; streamed: 4
+template <int DT, int KS, bool RESIDENT, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 1) void xattn_dq_kernel(const Args a) {
+  constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW, CH = stream_keys(KS);
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h2 = lane >> 5, li = lane & 31;
   const unsigned L = xcd_remap(blockIdx.x, gridDim.x);
   const int g = (int)(L % (unsigned)a.kvh);
-  const int j = (int)(L / (unsigned)a.kvh) % a.nb, e = (int)(L / (unsigned)a.kvh) / a.nb;
+  const int e = (int)(L / (unsigned)a.kvh) % a.Be, j = (int)(L / (unsigned)a.kvh) / a.Be;
   const int len = valid_len(a, e);
   const int T = (a.R + 31) >> 5;
-  const int npad = RESIDENT ? (a.Nk + 31) / 32 * 32 : CH;
-  uint16_t* const ks = reinterpret_cast<uint16_t*>(smem);
-  uint16_t* const vs = ks + npad * P;
-  float* const bias = reinterpret_cast<float*>(smem + 2 * npad * P * 2 + 64);
+  const int npad = RESIDENT ? (a.Nk + 31) / 32 * 32 : CH, stride = kv_lds(KS, npad);
+  auto ks_of = [&](int b) { return reinterpret_cast<uint16_t*>(smem + b * stride); };
+  auto vs_of = [&](int b) { return reinterpret_cast<uint16_t*>(smem + b * stride) + npad * P; };
+  auto bias_of = [&](int b) { return reinterpret_cast<float*>(smem + b * stride + 2 * npad * P * 2 + 64); };
+  Stager<KS, THREADS, CH> stager;
+  stager.open(a, e, g);
   if constexpr (RESIDENT) {
-    stage_kv<KS, THREADS>(a, e, g, len, 0, (len + 31) / 32 * 32, ks, vs, bias, tid);
+    stage_all<DT, KS, THREADS>(a, e, g, len, ks_of(0), vs_of(0), bias_of(0), false, tid);
     __syncthreads();
   }
-  const int step = a.nb * 4;
-  int t = j * 4 + wave;
-  const int rounds = (T - j * 4 + step - 1) / step;
+  const int step = a.nb * NW;
+  int t = j * NW + wave;
+  const int rounds = (T - j * NW + step - 1) / step;
+
+  struct Row {
+    uint4 q[KS], d[KS], o[KS];
+    float lse;
+  };
+  auto place = [&](int tt, int64_t& b, int& qi, int& head) {
+    int img, hh;
+    flat_row(a, min(32 * tt + li, a.R - 1), img, qi, hh);
+    head = g * a.hg + hh;
+    b = (int64_t)e * a.G + img;
+  };
+  auto request = [&](int tt, Row& r) {
+    int64_t b;
+    int qi, head;
+    place(tt, b, qi, head);
+    const int64_t col = (int64_t)head * a.d;
+    load_row<KS>(r.d, a.dout + b * a.sdb + (int64_t)qi * a.sdr + col, a.d, h2);
+    load_row<KS>(r.o, a.o + b * a.sob + (int64_t)qi * a.sor + col, a.d, h2);
+    load_row<KS>(r.q, a.q + b * a.sqb + (int64_t)qi * a.sqr + col, a.d, h2);
+    r.lse = a.lse_in[(b * a.kvh * a.hg + head) * a.Nq + qi];
+  };
+  // narrow heads: the next tile's rows are requested before this one's products (wider ones have no registers for that)
+  constexpr bool AHEAD = RESIDENT && KS <= 5;
+  Row nx;
+  if (AHEAD && t < T) request(t, nx);
 
   for (int round = 0; RESIDENT ? t < T : round < rounds; t += step, ++round) {
     const int f = 32 * t + li;
     const bool live = f < a.R;
-    int img, qi, hh;
-    flat_row(a, min(f, a.R - 1), img, qi, hh);
-    const int head = g * a.hg + hh;
-    const int64_t b = (int64_t)e * a.G + img, col = (int64_t)head * a.d;
-    const int64_t stat = (b * a.kvh * a.hg + head) * a.Nq + qi;
     uint4 qf[KS], df[KS];
-    load_row<KS>(qf, a.q + b * a.sqb + (int64_t)qi * a.sqr + col, a.d, h2);
-    load_row<KS>(df, a.dout + b * a.sdb + (int64_t)qi * a.sdr + col, a.d, h2);
-    float delta = 0.f;
+    float delta = 0.f, l2;
     {
-      const uint16_t* po = a.o + b * a.sob + (int64_t)qi * a.sor + col;
+      if constexpr (!AHEAD) request(min(t, T - 1), nx);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int kk = 16 * s + 8 * h2;
         float x[8], y[8];
-        unpack8<DT>(*reinterpret_cast<const uint4*>(po + (kk < a.d ? kk : 0)), x);
-        unpack8<DT>(df[s], y);
+        unpack8<DT>(nx.o[s], x);
+        unpack8<DT>(nx.d[s], y);
         float p = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) p = fmaf(x[i], y[i], p);
         delta += kk < a.d ? p : 0.f;
+        qf[s] = nx.q[s];
+        df[s] = nx.d[s];
       }
+      l2 = nx.lse * LOG2E;
+      if (AHEAD && t + step < T) request(t + step, nx);
       delta += __shfl_xor(delta, 32, 64);
     }
-    float l2 = a.lse_in[stat] * LOG2E;
     if (l2 == -INFINITY) l2 = INFINITY;  // a row without a key: P = exp2(0 - inf) = 0
-    if (t < T && live && h2 == 0) a.delta[stat] = delta;
+    int64_t b;
+    int qi, head;
+    place(min(t, T - 1), b, qi, head);
+    if (t < T && live && h2 == 0) a.delta[(b * a.kvh * a.hg + head) * a.Nq + qi] = delta;
     f32x16 acc[OT];
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
 
-    auto tile = [&](int kr, bool masked) {
+    auto tile = [&](const uint16_t* ks, const uint16_t* vs, const float* bias, int kr, bool masked) {
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
@@ -106,32 +132,42 @@ __global__ __launch_bounds__(256, KS <= 3 ? 3 : KS <= 6 ? 2 : 1) void xattn_dq_k
       }
     };
     if constexpr (RESIDENT) {
-      for (int kr = 0; kr < len; kr += 32) tile(kr, a.mask || kr + 32 > len);
+      for (int kr = 0; kr < len; kr += 32) tile(ks_of(0), vs_of(0), bias_of(0), kr, a.mask || kr + 32 > len);
     } else {
-      for (int k0 = 0; k0 < len; k0 += CH) {
+      const int chunks = (len + CH - 1) / CH;
+      if (chunks > 0) {
+        stager.issue(a, e, len, 0, tid);
+        if (round > 0) __syncthreads();
+        stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), false, tid);
+        if (chunks > 1) stager.issue(a, e, len, CH, tid);
+      }
+      for (int i = 0; i < chunks; ++i) {
         __syncthreads();
-        stage_kv<KS, THREADS>(a, e, g, len, k0, CH, ks, vs, bias, tid);
-        __syncthreads();
+        const int bf = i & 1;
         if (t < T) {
-          tile(0, a.mask || k0 + 32 > len);
-          if (k0 + 32 < len) tile(32, a.mask || k0 + 64 > len);
+          tile(ks_of(bf), vs_of(bf), bias_of(bf), 0, a.mask || i * CH + 32 > len);
+          if (CH > 32 && i * CH + 32 < len) tile(ks_of(bf), vs_of(bf), bias_of(bf), 32, a.mask || i * CH + 64 > len);
+        }
+        if (i + 1 < chunks) {
+          stager.template commit<DT>(a, ks_of(bf ^ 1), vs_of(bf ^ 1), bias_of(bf ^ 1), false, tid);
+          if (i + 2 < chunks) stager.issue(a, e, len, (i + 2) * CH, tid);
         }
       }
     }
     if (t >= T) continue;
-    uint16_t* p = a.out + b * a.sob + (int64_t)qi * a.sor + col;
+    uint16_t* p = a.out + b * a.sob + (int64_t)qi * a.sor + (int64_t)head * a.d;
 #pragma unroll
     for (int i = 0; i < OT; ++i) store_tile<DT>(acc[i], a.scale, p, live, i, a.d, h2);
   }
 }
 
-// QT query rows per LDS buffer
-constexpr int qt_rows(int ks) { return ks <= 5 ? 64 : 32; }
-constexpr int dkv_lds(int ks) { return 2 * (2 * qt_rows(ks) * (16 * ks + 8) * 2 + 2 * qt_rows(ks) * 4 + 64); }
+// query rows per LDS buffer: what a thread can hold on its way
+constexpr int qt_rows(int ks, int nw) { return ks <= 4 && nw > 1 ? 64 : 32; }
+constexpr int dkv_lds(int ks, int nw) { return 2 * (2 * qt_rows(ks, nw) * (16 * ks + 8) * 2 + 2 * qt_rows(ks, nw) * 4 + 64); }
 
 template <int DT, int KS, int NW>
-__global__ __launch_bounds__(64 * NW, KS <= 5 ? 2 : 1) void xattn_dkv_kernel(const Args a) {
-  constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW, QT = qt_rows(KS), CHN = 2 * KS;
+__global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) void xattn_dkv_kernel(const Args a) {
+  constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW, QT = qt_rows(KS, NW);
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int BUF = 2 * QT * P * 2 + 2 * QT * 4 + 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -139,7 +175,7 @@ __global__ __launch_bounds__(64 * NW, KS <= 5 ? 2 : 1) void xattn_dkv_kernel(con
   // blocks of one XCD: the key heads of the same rows, then the key groups
   const unsigned L = xcd_remap(blockIdx.x, gridDim.x);
   const int g = (int)(L % (unsigned)a.kvh);
-  const int kt = (int)(L / (unsigned)a.kvh) % a.nb, e = (int)(L / (unsigned)a.kvh) / a.nb;
+  const int e = (int)(L / (unsigned)a.kvh) % a.Be, kt = (int)(L / (unsigned)a.kvh) / a.Be;
   const int len = valid_len(a, e);
   const int key = (kt * NW + wave) * 32 + li;
   const bool valid = key_valid(a, e, len, min(key, a.Nk - 1)) && key < a.Nk;
@@ -168,48 +204,70 @@ __global__ __launch_bounds__(64 * NW, KS <= 5 ? 2 : 1) void xattn_dkv_kernel(con
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
-  // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta into buffer b; rows that do not exist: zeros, P = 0
-  auto stage = [&](int t, int b) {
-    uint16_t* qs = reinterpret_cast<uint16_t*>(smem + b * BUF);
-    uint16_t* ds = qs + QT * P;
-    float* l2 = reinterpret_cast<float*>(smem + b * BUF + 2 * QT * P * 2 + 64);
-    for (int i = tid; i < QT * CHN; i += THREADS) {
-      const int row = i / CHN, cc = (i - row * CHN) * 8, f = t * QT + row;
-      uint4 x = make_uint4(0, 0, 0, 0), y = make_uint4(0, 0, 0, 0);
-      if (f < a.R && cc < a.d) {
+  // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to buffer b (commit); rows that
+  // do not exist: zeros, P = 0
+  constexpr int LPR = lanes_of(KS), RP = THREADS / LPR, NC = (QT + RP - 1) / RP;
+  uint4 xr[NC], yr[NC];
+  float lr, dr;
+  auto issue = [&](int t) {
+    int id = tid;
+    asm volatile("" : "+v"(id));  // addresses are made anew for every tile
+    const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int row = row0 + i * RP, f = t * QT + row;
+      xr[i] = yr[i] = make_uint4(0, 0, 0, 0);
+      if (cc < a.d && f < a.R && (QT % RP == 0 || row < QT)) {
         int img, qi, hh;
         flat_row(a, f, img, qi, hh);
         const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
-        x = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
-        y = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
+        xr[i] = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
+        yr[i] = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
       }
-      *reinterpret_cast<uint4*>(qs + row * P + cc) = x;
-      *reinterpret_cast<uint4*>(ds + row * P + cc) = y;
     }
-    for (int i = tid; i < QT; i += THREADS) {
-      const int f = t * QT + i;
-      float l = INFINITY, dl = 0.f;
-      if (f < a.R) {
-        int img, qi, hh;
-        flat_row(a, f, img, qi, hh);
-        const int64_t stat = (((int64_t)e * a.G + img) * a.kvh * a.hg + g * a.hg + hh) * a.Nq + qi;
-        l = a.lse_in[stat] * LOG2E;
-        l = l == -INFINITY ? INFINITY : l;
-        dl = a.delta[stat];
-      }
-      l2[i] = l;
-      l2[QT + i] = dl;
+    static_assert(QT <= THREADS, "a thread per row");
+    lr = -INFINITY;
+    dr = 0.f;
+    const int f = t * QT + id;
+    if (id < QT && f < a.R) {
+      int img, qi, hh;
+      flat_row(a, f, img, qi, hh);
+      const int64_t stat = (((int64_t)e * a.G + img) * a.kvh * a.hg + g * a.hg + hh) * a.Nq + qi;
+      lr = a.lse_in[stat];
+      dr = a.delta[stat];
     }
   };
-  if (t_lo < t_hi) stage(t_lo, 0);
+  auto commit = [&](int b) {
+    int id = tid;
+    asm volatile("" : "+v"(id));
+    const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
+    uint16_t* qs = reinterpret_cast<uint16_t*>(smem + b * BUF);
+    float* l2 = reinterpret_cast<float*>(smem + b * BUF + 2 * QT * P * 2 + 64);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int row = row0 + i * RP;
+      if (cc < 16 * KS && (QT % RP == 0 || row < QT)) {
+        *reinterpret_cast<uint4*>(qs + row * P + cc) = xr[i];
+        *reinterpret_cast<uint4*>(qs + QT * P + row * P + cc) = yr[i];
+      }
+    }
+    if (id < QT) {
+      l2[id] = lr == -INFINITY ? INFINITY : lr * LOG2E;
+      l2[QT + id] = dr;
+    }
+  };
+  if (t_lo < t_hi) {
+    issue(t_lo);
+    commit(0);
+    if (t_lo + 1 < t_hi) issue(t_lo + 1);
+  }
   for (int t = t_lo; t < t_hi; ++t) {
     const int b = (t - t_lo) & 1;
     __syncthreads();
-    if (t + 1 < t_hi) stage(t + 1, b ^ 1);
-    if (!any) continue;
     const uint16_t* qs = reinterpret_cast<const uint16_t*>(smem + b * BUF);
     const uint16_t* ds = qs + QT * P;
     const float* l2 = reinterpret_cast<const float*>(smem + b * BUF + 2 * QT * P * 2 + 64);
+    if (any) {
 #pragma unroll
     for (int q0 = 0; q0 < QT; q0 += 32) {
       f32x16 s, dp;
@@ -240,6 +298,11 @@ __global__ __launch_bounds__(64 * NW, KS <= 5 ? 2 : 1) void xattn_dkv_kernel(con
           dk[i] = HT<DT>::mfma32(read_tr(qs, P, q0 + 16 * u, 32 * i, lane), sf, dk[i]);
         }
       }
+    }
+    }
+    if (t + 1 < t_hi) {
+      commit(b ^ 1);  // (read last in the previous round, which every wave has left)
+      if (t + 2 < t_hi) issue(t + 2);
     }
   }
   if (key >= a.Nk) return;
@@ -282,26 +345,31 @@ __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(const float* ws, ui
 
 struct Plan {
   bool resident;
-  int lds, nb;             // dq
+  int dq_nw, lds, nb;      // dq
   int nw, groups, nsplit;  // dk / dv
 };
-// dq: as the forward.  dk / dv: as many waves per block as there are key tiles (1, 2 or 4), the rows cut into parts until two
-// blocks per CU have work and a part keeps at least four tiles.
+// (the widest heads leave one or two waves no registers for the rows on their way)
+constexpr int min_waves(int ks) { return ks >= 8 ? 3 : 1; }
+// dq: as the forward.  dk / dv: the number of waves per block (up to four) that leaves the fewest without a key tile; the rows are
+// cut into parts until the chip has as many waves as fit, a part keeping at least four row tiles.
 Plan plan(const Args& a) {
   Plan p{};
   const int ks = k_steps(a.d), cus = cu_count(), eg = a.Be * a.kvh;
-  const int npad = (a.Nk + 31) / 32 * 32;
-  p.resident = kv_lds(ks, npad) <= RES_LDS;
-  p.lds = p.resident ? kv_lds(ks, npad) : kv_lds(ks, CH);
-  const int most = ((a.R + 31) / 32 + 3) / 4, want = p.resident ? 4 * cus : most * eg;
-  p.nb = (want + eg - 1) / eg;
+  const int all = kv_lds(ks, (a.Nk + 63) / 64 * 64), tq = (a.R + 31) / 32;
+  p.resident = all <= 80000 || (all <= 160000 && tq >= 16);
+  p.dq_nw = p.resident && all > 80000 ? 8 : 4;
+  p.lds = p.resident ? all : 2 * kv_lds(ks, stream_keys(ks));
+  const int most = (tq + p.dq_nw - 1) / p.dq_nw, fit = 160000 / (all > 1000 ? all : 1000), per_cu = p.dq_nw == 8 ? 1 : fit < 4 ? fit : 4;
+  p.nb = p.resident ? (per_cu * cus + eg - 1) / eg : most;
   if (p.nb > most) p.nb = most;
   const int tiles = a.Nk > 0 ? (a.Nk + 31) / 32 : 1;  // (without keys there is no dk / dv launch)
-  p.nw = tiles <= 1 ? 1 : tiles == 2 ? 2 : 4;
+  p.nw = 4;
+  for (int w = 3; w >= min_waves(ks); --w)
+    if ((tiles + w - 1) / w * w < (tiles + p.nw - 1) / p.nw * p.nw) p.nw = w;
   p.groups = (tiles + p.nw - 1) / p.nw;
-  const int T = (a.R + qt_rows(ks) - 1) / qt_rows(ks);
-  const int64_t blocks = (int64_t)eg * p.groups;
-  int64_t n = ((int64_t)(p.nw == 4 ? 2 : p.nw == 2 ? 4 : 8) * cus + blocks - 1) / blocks;
+  const int T = (a.R + qt_rows(ks, p.nw) - 1) / qt_rows(ks, p.nw);
+  const int64_t blocks = (int64_t)eg * p.groups, waves = (int64_t)(ks <= 5 ? 8 : 4) * cus;
+  int64_t n = (waves / p.nw + blocks - 1) / blocks;
   if (n > T / 4) n = T / 4;
   if (n > 256) n = 256;
   p.nsplit = n < 1 ? 1 : (int)n;
@@ -319,16 +387,19 @@ template <int DT, int KS>
 int launch(Args& a, const Plan& p, hipStream_t st) {
   const unsigned eg = (unsigned)(a.Be * a.kvh);
   a.nb = p.nb; a.nsplit = 1;
-  if (p.resident) hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, true>), dim3(eg * (unsigned)p.nb), dim3(256), p.lds, st, a);
-  else hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, false>), dim3(eg * (unsigned)p.nb), dim3(256), p.lds, st, a);
+  if (p.resident && p.dq_nw == 8) hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, true, 8>), dim3(eg * (unsigned)p.nb), dim3(512), p.lds, st, a);
+  else if (p.resident) hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, true, 4>), dim3(eg * (unsigned)p.nb), dim3(256), p.lds, st, a);
+  else hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, false, 4>), dim3(eg * (unsigned)p.nb), dim3(256), p.lds, st, a);
   MIMO_LAUNCH_CHECK();
   if (a.Nk == 0) return MIMO_OK;
   a.nb = p.groups; a.nsplit = p.nsplit;
   const dim3 grid(eg * (unsigned)p.groups, (unsigned)p.nsplit);
-  constexpr int lds = dkv_lds(KS);
-  if (p.nw == 1) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 1>), grid, dim3(64), lds, st, a);
-  else if (p.nw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(128), lds, st, a);
-  else hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 4>), grid, dim3(256), lds, st, a);
+  if constexpr (min_waves(KS) == 1) {
+    if (p.nw == 1) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 1>), grid, dim3(64), dkv_lds(KS, 1), st, a);
+    if (p.nw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(128), dkv_lds(KS, 2), st, a);
+  }
+  if (p.nw == 3) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 3>), grid, dim3(192), dkv_lds(KS, 3), st, a);
+  if (p.nw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 4>), grid, dim3(256), dkv_lds(KS, 4), st, a);
   MIMO_LAUNCH_CHECK();
   if (p.nsplit > 1) {
     const int64_t plane = (int64_t)a.Be * a.Nk * a.kvh * a.d, nwg = (plane / 2 + 255) / 256;

@@ -327,11 +327,6 @@ def gemm(a, w, *, bias=None, img_bias=None, rows_per_img=0, residual=None, out_f
     return out, ln_out
 
 
-def _require(ok, what):
-    if not ok:
-        raise L.MimoHipError(what)
-
-
 class _on_device:
     """The launch happens on the tensors' own device, whatever the current one is."""
 
@@ -348,11 +343,8 @@ class _on_device:
         return False
 
 
-def _stride(t, i):
-    """Element stride of axis i, 0 where the axis has one entry (its stride is then arbitrary)."""
-    return t.stride(i) if t.shape[i] > 1 else 0
-
-
+# Argument checks of the operators below: every refusal is a MimoHipError raised before any launch.  (They run on every call,
+# also on the ones that take ten microseconds: a message is formatted only when it is raised.)
 def _ld(t):
     """Row pitch of a matrix in elements (0: every row is the same one)."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -360,37 +352,55 @@ def _ld(t):
 
 def _rows_ok(t, name):
     """Rows of whole 16-byte chunks: what the kernels' wide loads need."""
-    _require(t.stride(-1) == 1 or t.shape[-1] <= 1 or t.numel() == 0, f"{name}: the last axis is contiguous")
-    _require(t.data_ptr() % 16 == 0 and all(_stride(t, i) % 8 == 0 for i in range(t.dim() - 1)),
-             f"{name}: 16-byte aligned rows (strides {t.stride()})")
+    if t.numel() == 0:
+        return
+    st, sh = t.stride(), t.shape
+    if st[-1] != 1 and sh[-1] > 1:
+        raise L.MimoHipError(f"{name}: the last axis is contiguous (strides {st})")
+    bad = t.data_ptr() & 15
+    for n, x in zip(sh[:-1], st):
+        if n > 1:
+            bad |= x & 7
+    if bad:
+        raise L.MimoHipError(f"{name}: 16-byte aligned rows (strides {st})")
 
 
-def _adapter_params(a, w, down, up, index, rows_per_index, scale, w_shape):
-    """Checks the operands of an adapter product and lays the adapters down for the C-ABI; returns (params, tensors they point at)."""
+def _same(ref, **tensors):
+    """Operands of one call: one type, one device."""
+    dt, dev = ref.dtype, ref.device
+    for name, t in tensors.items():
+        if t.dtype != dt or t.device != dev:
+            raise L.MimoHipError(f"{name}: {t.dtype} on {t.device}, the others are {dt} on {dev}")
+
+
+def _adapter_params(a, w, down, up, index, rows_per_index, scale, transposed=False):
+    """Checks the operands of an adapter product and lays the adapters down for the C-ABI."""
     dt_code(a.dtype)
-    _require(a.dim() == 2 and w.dim() == 2 and down.dim() == 3 and up.dim() == 3, "a [M, K], w [N, K], down [S, r, K], up [S, N, r]")
+    if a.dim() != 2 or w.dim() != 2 or down.dim() != 3 or up.dim() != 3:
+        raise L.MimoHipError("a [M, K], w [N, K], down [S, r, K], up [S, N, r]")
     M, K = a.shape
     S, r, _ = down.shape
     N = up.shape[1]
-    _require(down.shape == (S, r, K) and up.shape == (S, N, r) and w.shape == w_shape(N, K),
-             f"a {tuple(a.shape)}, w {tuple(w.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)} do not fit together")
-    _require(S > 0 and 0 < r <= 128 and r % 8 == 0, f"{S} adapters of rank {r}: ranks are multiples of 8 up to 128 (packing.pack_adapters pads)")
-    _require(N % 8 == 0 and K % 8 == 0 and N > 0 and K > 0 and N * K < 1 << 30, f"widths {N}, {K}: multiples of 8")
-    for t, name in ((a, "a"), (w, "w"), (down, "down"), (up, "up")):
-        _require(t.device == a.device and t.dtype == a.dtype, f"{name}: {t.dtype} on {t.device}, a is {a.dtype} on {a.device}")
+    if down.shape[2] != K or up.shape[0] != S or up.shape[2] != r or w.shape != ((K, N) if transposed else (N, K)):
+        raise L.MimoHipError(f"a {tuple(a.shape)}, w {tuple(w.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)} do not fit together")
+    if S <= 0 or not 0 < r <= 128 or r & 7:
+        raise L.MimoHipError(f"{S} adapters of rank {r}: ranks are multiples of 8 up to 128 (packing.pack_adapters pads)")
+    if N <= 0 or K <= 0 or (N | K) & 7 or N * K >= 1 << 30 or S > 65535 or M >= (1 << 31) - 1:
+        raise L.MimoHipError(f"{M} rows, widths {N} and {K} (multiples of 8), {S} adapters: beyond what the kernels address")
+    _same(a, w=w, down=down, up=up)
     for t, name in ((w, "w"), (down, "down"), (up, "up")):
-        _require(t.is_contiguous() and t.data_ptr() % 16 == 0, f"{name}: contiguous, 16-byte aligned")
+        if not t.is_contiguous() or t.data_ptr() & 15:
+            raise L.MimoHipError(f"{name}: contiguous, 16-byte aligned")
     _rows_ok(a, "a")
-    rows_per_index = int(rows_per_index)
-    _require(rows_per_index > 0, f"rows_per_index {rows_per_index}")
-    _require(index.dim() == 1 and index.dtype == torch.int32 and index.device == a.device and index.is_contiguous() and
-             index.numel() >= (M + rows_per_index - 1) // rows_per_index,
-             f"index: contiguous int32 on {a.device}, an entry per {rows_per_index} of {M} rows")
-    if scale is not None:
-        _require(scale.shape == (S,) and scale.dtype == torch.float32 and scale.device == a.device and scale.is_contiguous(),
-                 f"scale: contiguous fp32 [{S}] on {a.device}")
+    if rows_per_index < 1:
+        raise L.MimoHipError(f"rows_per_index {rows_per_index}")
+    if index.dim() != 1 or index.dtype != torch.int32 or index.device != a.device or not index.is_contiguous() or \
+            index.shape[0] * rows_per_index < M:
+        raise L.MimoHipError(f"index: contiguous int32 on {a.device}, an entry per {rows_per_index} of {M} rows")
+    if scale is not None and (scale.shape != (S,) or scale.dtype != torch.float32 or scale.device != a.device or not scale.is_contiguous()):
+        raise L.MimoHipError(f"scale: contiguous fp32 [{S}] on {a.device}")
     _chk(a, "a")
-    return L.AdapterParams(down.data_ptr(), up.data_ptr(), _ptr(scale), index.data_ptr(), rows_per_index, S, r)
+    return L.AdapterParams(down.data_ptr(), up.data_ptr(), _ptr(scale), index.data_ptr(), int(rows_per_index), S, r)
 
 
 # the low-rank values of adapter_gemm with nothing lost: value + remainder planes of the operand type (fp16 22, bf16 24 mantissa bits)
@@ -406,15 +416,15 @@ def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=No
     consecutive rows, in any order; an entry outside [0, S) (use -1) means no adapter.  scale: fp32 [S] (None: 1); bias: fp32 [N];
     residual: fp32 or half [M, N].  Returns half, or fp32 with out_f32.
     want_low: returns (out, low), low half [M, LOW_PLANES r] = the rows' scaled low-rank values, value and remainders, for the backward."""
-    p = _adapter_params(a, w, down, up, index, rows_per_index, scale, lambda N, K: (N, K))
+    p = _adapter_params(a, w, down, up, index, rows_per_index, scale)
     M, K = a.shape
     N, r = w.shape[0], p.rank
-    if bias is not None:
-        _require(bias.shape == (N,) and bias.dtype == torch.float32 and bias.device == a.device and bias.is_contiguous(), f"bias: fp32 [{N}]")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != torch.float32 or bias.device != a.device or not bias.is_contiguous()):
+        raise L.MimoHipError(f"bias: contiguous fp32 [{N}] on {a.device}")
     if residual is not None:
-        _require(residual.shape == (M, N) and residual.device == a.device and residual.dtype in (torch.float32, a.dtype) and
-                 (residual.stride(1) == 1 or N == 1) and _stride(residual, 0) % 4 == 0 and residual.data_ptr() % 16 == 0,
-                 f"residual: fp32 or {a.dtype} [{M}, {N}], 16-byte aligned rows")
+        if residual.shape != (M, N) or residual.device != a.device or residual.dtype not in (torch.float32, a.dtype):
+            raise L.MimoHipError(f"residual: fp32 or {a.dtype} [{M}, {N}] on {a.device}")
+        _rows_ok(residual, "residual")
     split = bool(want_low or out_f32)
     with _on_device(a.device):
         out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_f32 else a.dtype)
@@ -423,7 +433,8 @@ def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=No
             fl = 2 * M * N * K + 2 * M * r * (N + K)
             _count(fl)
             flags = (L.EPI_OUT_F32 if out_f32 else 0) | (L.EPI_RES_F32 if residual is not None and residual.dtype == torch.float32 else 0)
-            with _Bracket("gemm_kernel", fl, _nbytes(a, w, out, residual, down, up), f"adapter_gemm M{M} N{N} K{K} r{r}"):
+            with _Bracket("gemm_kernel", fl, _nbytes(a, w, out, residual, down, up) if EVENTS is not None else 0,
+                          f"adapter_gemm M{M} N{N} K{K} r{r}"):
                 L.call("mimo_adapter_gemm", dt_code(a.dtype), a.data_ptr(), _ld(a), w.data_ptr(), out.data_ptr(), N, M, N, K,
                        _ptr(bias), _ptr(residual), 0 if residual is None else _ld(residual), flags, ctypes.byref(p), low.data_ptr(),
                        int(split), _stream())
@@ -435,13 +446,16 @@ def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=
     operands, w_t = the transposed weight [K, N] (contiguous, laid out once) and its low (want_low=True).  da: half [M, K] (None
     with want_da=False); ddown fp32 [S, r, K] and dup fp32 [S, N, r] are summed over the rows of each adapter in a fixed order:
     the same bits on every run, zeros for an adapter without rows.  (The residual's gradient is dout, the bias's its column sum.)"""
-    p = _adapter_params(a, w_t, down, up, index, rows_per_index, scale, lambda N, K: (K, N))
+    p = _adapter_params(a, w_t, down, up, index, rows_per_index, scale, transposed=True)
     M, K = a.shape
     N, r, S = up.shape[1], p.rank, p.count
-    _require(dout.shape == (M, N) and dout.dtype == a.dtype and dout.device == a.device, f"dout: {a.dtype} [{M}, {N}]")
+    if dout.shape != (M, N) or low.shape != (M, LOW_PLANES[a.dtype] * r):
+        raise L.MimoHipError(f"dout {tuple(dout.shape)}, low {tuple(low.shape)}: [{M}, {N}] and the forward's [{M}, {LOW_PLANES[a.dtype] * r}] "
+                             "(want_low=True)")
+    _same(a, dout=dout, low=low)
     _rows_ok(dout, "dout")
-    _require(low.shape == (M, LOW_PLANES[a.dtype] * r) and low.dtype == a.dtype and low.device == a.device and low.is_contiguous() and
-             low.data_ptr() % 16 == 0, f"low: the forward's [{M}, {LOW_PLANES[a.dtype] * r}] (want_low=True)")
+    if not low.is_contiguous() or low.data_ptr() & 15:
+        raise L.MimoHipError("low: contiguous, 16-byte aligned")
     with _on_device(a.device):
         da = torch.empty((M, K), device=a.device, dtype=a.dtype) if want_da else None
         if not M:
@@ -452,7 +466,8 @@ def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=
         _count(fl)
         nb = L.load().mimo_adapter_gemm_backward_workspace(dt_code(a.dtype), ctypes.byref(p), M, N, K)
         ws = torch.empty(((nb + 3) // 4,), device=a.device, dtype=torch.float32)
-        with _Bracket("gemm_kernel", fl, _nbytes(dout, a, w_t, da, ddown, dup), f"adapter_gemm_backward M{M} N{N} K{K} r{r}"):
+        with _Bracket("gemm_kernel", fl, _nbytes(dout, a, w_t, da, ddown, dup) if EVENTS is not None else 0,
+                      f"adapter_gemm_backward M{M} N{N} K{K} r{r}"):
             L.call("mimo_adapter_gemm_backward", dt_code(a.dtype), dout.data_ptr(), _ld(dout), a.data_ptr(), _ld(a),
                    w_t.data_ptr(), _ptr(da), K, M, N, K, ctypes.byref(p), low.data_ptr(), ddown.data_ptr(), dup.data_ptr(), ws.data_ptr(),
                    nb, _stream())
@@ -952,30 +967,42 @@ def attention(q, k, v, heads, *, k2=None, v2=None, seg2_first_batch=0, scale=Non
 def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
     """Checks the operands of a cross attention and lays their geometry down for the C-ABI."""
     dt_code(q.dtype)
-    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v: [batch, tokens, channels]")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise L.MimoHipError("q, k, v: [batch, tokens, channels]")
     B, Nq, C = q.shape
     Be, Nk, Ck = k.shape
-    kv_heads = heads if kv_heads is None else kv_heads
-    _require(heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and C % heads == 0, f"{C} channels in {heads} heads over {kv_heads} key heads")
+    if kv_heads is None:
+        kv_heads = heads
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads or C % heads:
+        raise L.MimoHipError(f"{C} channels in {heads} heads over {kv_heads} key heads")
     d = C // heads
-    _require(d % 8 == 0 and 8 <= d <= 160, f"head width {d}: a multiple of 8 up to 160")
-    _require(Ck == kv_heads * d and v.shape == k.shape, f"k {tuple(k.shape)}, v {tuple(v.shape)}: [encoder rows, keys, {kv_heads * d}]")
-    _require(Be > 0 and B % Be == 0, f"{B} images over {Be} encoder rows")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _require(t.device == q.device and t.dtype == q.dtype, f"{name}: {t.dtype} on {t.device}, q is {q.dtype} on {q.device}")
-        _rows_ok(t, name)
+    if d & 7 or not 8 <= d <= 160:
+        raise L.MimoHipError(f"head width {d}: a multiple of 8 up to 160")
+    if Ck != kv_heads * d or v.shape != k.shape:
+        raise L.MimoHipError(f"k {tuple(k.shape)}, v {tuple(v.shape)}: [encoder rows, keys, {kv_heads * d}]")
+    if Be <= 0 or B % Be:
+        raise L.MimoHipError(f"{B} images over {Be} encoder rows")
+    if B // Be * Nq * (heads // kv_heads) >= 1 << 30 or Be * kv_heads >= 1 << 16 or Nk >= 1 << 30:
+        raise L.MimoHipError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: beyond what the kernels address")
+    _same(q, k=k, v=v)
+    _rows_ok(q, "q")
+    _rows_ok(k, "k")
+    _rows_ok(v, "v")
     scale = d ** -0.5 if scale is None else float(scale)
-    _require(0.0 < scale < float("inf"), f"scale {scale}")
-    p = L.CrossAttentionParams(B, Be, Nq, Nk, heads, kv_heads, d, scale, _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
-                               _stride(v, 0), _stride(v, 1))
+    if not 0.0 < scale < float("inf"):
+        raise L.MimoHipError(f"scale {scale}")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    p = L.CrossAttentionParams(B, Be, Nq, Nk, heads, kv_heads, d, scale, sq[0] if B > 1 else 0, sq[1] if Nq > 1 else 0,
+                               sk[0] if Be > 1 else 0, sk[1] if Nk > 1 else 0, sv[0] if Be > 1 else 0, sv[1] if Nk > 1 else 0)
     if kv_len is not None:
-        _require(kv_len.device == q.device and kv_len.dtype == torch.int32 and kv_len.shape == (Be,) and kv_len.is_contiguous(),
-                 f"kv_len: contiguous int32 [{Be}] on {q.device}")
+        if kv_len.device != q.device or kv_len.dtype != torch.int32 or kv_len.shape != (Be,) or not kv_len.is_contiguous():
+            raise L.MimoHipError(f"kv_len: contiguous int32 [{Be}] on {q.device}")
         p.kv_len = kv_len.data_ptr()
     if mask is not None:
-        _require(mask.device == q.device and mask.dtype in (torch.bool, torch.uint8) and mask.shape == (Be, Nk) and
-                 (Nk <= 1 or mask.stride(1) == 1), f"mask: bool or uint8 [{Be}, {Nk}] on {q.device}, True where the key counts")
-        p.mask, p.mask_row = mask.data_ptr(), _stride(mask, 0)
+        if mask.device != q.device or mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (Be, Nk) or \
+                (Nk > 1 and mask.stride(1) != 1):
+            raise L.MimoHipError(f"mask: bool or uint8 [{Be}, {Nk}] on {q.device}, True where the key counts")
+        p.mask, p.mask_row = mask.data_ptr(), mask.stride(0) if Be > 1 else 0
     _chk(q, "q")
     return p
 
@@ -998,7 +1025,7 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, kv_len=None, mask=None, sc
             _count(fl)
             nb = L.load().mimo_cross_attention_workspace(ctypes.byref(p))
             ws = torch.empty((nb // 4,), device=q.device, dtype=torch.float32) if nb else None
-            with _Bracket("attn_kernel", fl, _nbytes(q, k, v, out)):
+            with _Bracket("attn_kernel", fl, _nbytes(q, k, v, out) if EVENTS is not None else 0):
                 L.call("mimo_cross_attention", dt_code(q.dtype), q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(), _ptr(lse),
                        ctypes.byref(p), _ptr(ws), nb, _stream())
     return (out, lse) if want_lse else out
@@ -1009,13 +1036,15 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, *, kv_heads=None, k
     gradient dout [B, Nq, heads d] (any strides of whole 16-byte chunks).  dk and dv are summed over the images and query heads that
     share a key, in a fixed order: the same bits on every run.  Keys that do not count get zeros."""
     p = _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale)
-    _require(dout.shape == q.shape and dout.dtype == q.dtype and dout.device == q.device, f"dout {tuple(dout.shape)}: as q")
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise L.MimoHipError(f"dout {tuple(dout.shape)}, out {tuple(out.shape)}: as q {tuple(q.shape)}")
+    _same(q, dout=dout, out=out)
     _rows_ok(dout, "dout")
-    _require(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.is_contiguous() and
-             out.data_ptr() % 16 == 0, "out: the forward's output")
-    _require(lse.shape == (p.B, heads, p.Nq) and lse.dtype == torch.float32 and lse.device == q.device and lse.is_contiguous(),
-             "lse: the forward's fp32 [B, heads, Nq]")
-    p.dout_batch, p.dout_row = _stride(dout, 0), _stride(dout, 1)
+    if not out.is_contiguous() or out.data_ptr() & 15:
+        raise L.MimoHipError("out: contiguous, 16-byte aligned")
+    if lse.shape != (p.B, heads, p.Nq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise L.MimoHipError("lse: the forward's contiguous fp32 [B, heads, Nq]")
+    p.dout_batch, p.dout_row = dout.stride(0) if p.B > 1 else 0, dout.stride(1) if p.Nq > 1 else 0
     with _on_device(q.device):
         dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         if not dq.numel():
@@ -1026,7 +1055,7 @@ def cross_attention_backward(dout, q, k, v, out, lse, heads, *, kv_heads=None, k
         _count(fl)
         nb = L.load().mimo_cross_attention_backward_workspace(ctypes.byref(p))
         ws = torch.empty((nb // 4,), device=q.device, dtype=torch.float32)
-        with _Bracket("attn_kernel", fl, _nbytes(dout, q, k, v, out, dq, dk, dv)):
+        with _Bracket("attn_kernel", fl, _nbytes(dout, q, k, v, out, dq, dk, dv) if EVENTS is not None else 0):
             L.call("mimo_cross_attention_backward", dt_code(q.dtype), dout.data_ptr(), q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(),
                    lse.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dv), ctypes.byref(p), ws.data_ptr(), nb, _stream())
     return dq, dk, dv
