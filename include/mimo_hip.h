@@ -421,7 +421,8 @@ int mimo_attention_fp8qk(int dtype, const void* q, int64_t ldq, const void* k, i
  *   backward: dout with strides dout_batch, dout_row; out, lse from the forward; dq [B, Nq, heads d], dk, dv [Be, Nk, kv_heads d]
  *   half16 contiguous: dk / dv are summed over the images and query heads that share a key, in a fixed order (no atomics).
  *   workspace: 16-byte aligned scratch of at least the size that the *_workspace call returns for the same params (0: none
- *   needed); it holds nothing between calls.  Nq >= 1, Nk >= 0, B / Be * Nq * (heads / kv_heads) < 2^30, Be * kv_heads < 2^16.
+ *   needed); it holds nothing between calls.  Nq >= 1, Nk >= 0, B / Be * Nq * (heads / kv_heads) < 2^30, Be * kv_heads < 2^16,
+ *   heads * Nq < 2^27.
  * --------------------------------------------------------------------------------- */
 typedef struct mimo_cross_attention_params {
   int B, Be, Nq, Nk, heads, kv_heads, d;

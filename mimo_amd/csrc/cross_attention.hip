@@ -22,7 +22,9 @@ int fill(Args& a, const mimo_cross_attention_params* p) {
   if ((p->q_batch & 7) || (p->q_row & 7) || (p->k_batch & 7) || (p->k_row & 7) || (p->v_batch & 7) || (p->v_row & 7)) return MIMO_EINVAL;
   a.Be = p->Be; a.G = p->B / p->Be; a.Nq = p->Nq; a.Nk = p->Nk; a.kvh = p->kv_heads; a.hg = p->heads / p->kv_heads; a.d = p->d;
   const int64_t R = (int64_t)a.G * a.Nq * a.hg;
-  if (R >= 0x40000000LL || (int64_t)p->Be * p->kv_heads >= 0x10000 || p->Nk >= 0x40000000) return MIMO_EINVAL;
+  if (R >= 0x40000000LL || (int64_t)p->Be * p->kv_heads >= 0x10000 || p->Nk >= 0x40000000 || (int64_t)p->heads * p->Nq >= 0x8000000 ||
+      p->heads >= 0x10000)
+    return MIMO_EINVAL;
   a.R = (int)R;
   a.by_hg = fast_div((uint32_t)a.hg); a.by_nq = fast_div((uint32_t)a.Nq);
   a.scale = p->scale; a.c = p->scale * LOG2E;
@@ -200,34 +202,34 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
       const int r = (a.d & 31) >> 3;  // row d of O^T: register 4 r of the last tile, lanes 0..31
       l = __shfl(r == 1 ? ot[OT - 1][4] : r == 2 ? ot[OT - 1][8] : ot[OT - 1][12], li, 64);
     }
-    const int f = 32 * t + li;
-    const bool live = f < a.R;
-    int img, qi, hh;
-    flat_row(a, min(f, a.R - 1), img, qi, hh);
-    const int head = g * a.hg + hh;
-    const int64_t b = (int64_t)e * a.G + img;
-    if (a.nsplit > 1) {  // partial: unnormalised rows, then (reference maximum in log2 units, divisor, sum)
-      const int64_t row = (((int64_t)blockIdx.y * a.Be + e) * a.kvh + g) * a.R + f;
-      float* po = a.ws + row * a.d;
-      if (live) {
+    if constexpr (!RESIDENT) {
+      if (a.nsplit > 1) {  // partial: unnormalised rows, then (reference maximum in log2 units, divisor, sum)
+        const int f = 32 * t + li;
+        const int64_t row = (((int64_t)blockIdx.y * a.Be + e) * a.kvh + g) * a.R + f;
+        float* po = a.ws + row * a.d;
+        if (f < a.R) {
 #pragma unroll
-        for (int i = 0; i < OT; ++i)
+          for (int i = 0; i < OT; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int d0 = 32 * i + 8 * c + 4 * h2;
-            if (d0 < a.d) *reinterpret_cast<f32x4*>(po + d0) = (f32x4){ot[i][4 * c], ot[i][4 * c + 1], ot[i][4 * c + 2], ot[i][4 * c + 3]};
-          }
-        if (h2 == 0)
-          *reinterpret_cast<f32x4*>(a.ws + (int64_t)a.nsplit * a.Be * a.kvh * a.R * a.d + 4 * row) = (f32x4){m_ref * a.c, l, sum, 0.f};
+            for (int c = 0; c < 4; ++c) {
+              const int d0 = 32 * i + 8 * c + 4 * h2;
+              if (d0 < a.d)
+                *reinterpret_cast<f32x4*>(po + d0) = (f32x4){ot[i][4 * c], ot[i][4 * c + 1], ot[i][4 * c + 2], ot[i][4 * c + 3]};
+            }
+          if (h2 == 0)
+            *reinterpret_cast<f32x4*>(a.ws + (int64_t)a.nsplit * a.Be * a.kvh * a.R * a.d + 4 * row) = (f32x4){m_ref * a.c, l, sum, 0.f};
+        }
+        continue;
       }
-      continue;
     }
+    const RowPlace place = row_place(a, e, g, t, li, a.out, a.lse);
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint16_t* p = a.out + b * a.sob + (int64_t)qi * a.sor + (int64_t)head * a.d;
 #pragma unroll
-    for (int i = 0; i < OT; ++i) store_tile<DT>(ot[i], inv, p, live, i, a.d, h2);
-    if (a.lse && live && h2 == 0)
-      a.lse[(b * a.kvh * a.hg + head) * a.Nq + qi] = sum > 0.f ? m_ref * a.scale + logf(sum) : -INFINITY;
+    for (int i = 0; i < OT; ++i) store_tile<DT>(ot[i], inv, place, i, a.d, h2);
+    if (a.lse) {
+      const float v = sum > 0.f ? m_ref * a.scale + logf(sum) : -INFINITY;
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), place.table, h2 == 0 ? place.stat : 0xF0000000u, 0, 0);
+    }
   }
 }
 

@@ -87,10 +87,32 @@ __device__ __forceinline__ uint4 pack_k(const f32x16& s, int u) {
                     pack2<DT>(s[8 * u + 4], s[8 * u + 5]), pack2<DT>(s[8 * u + 6], s[8 * u + 7]));
 }
 
+// Where the 32 flat rows of tile t go in a contiguous [B, Nq, heads d] tensor and in a [B, heads, Nq] table: uniform bases plus
+// 32-bit lane offsets for buffer stores, out of range for rows that do not exist.  No store is behind a branch: the loop knows how
+// many follow the next tile's loads and waits for those loads alone, not for the stores' acknowledgement.
+struct RowPlace {
+  __amdgpu_buffer_rsrc_t out, table;
+  unsigned row, stat;
+};
+__device__ __forceinline__ RowPlace row_place(const Args& a, int e, int g, int t, int li, uint16_t* out, float* table) {
+  RowPlace p;
+  const int f = 32 * t + li;
+  int img, qi, hh;
+  flat_row(a, f < a.R ? f : a.R - 1, img, qi, hh);
+  const uint32_t tq0 = div_fast((uint32_t)(32 * t), a.by_hg), img0 = div_fast(tq0, a.by_nq);
+  const int heads = a.kvh * a.hg, head = g * a.hg + hh, C = heads * a.d;
+  p.out = __builtin_amdgcn_make_buffer_rsrc(out + ((int64_t)e * a.G * a.Nq + tq0) * C, 0, 0x7fffffff, 0x00020000);
+  p.table = __builtin_amdgcn_make_buffer_rsrc(table + ((int64_t)e * a.G + img0) * heads * a.Nq, 0, table ? 0x7fffffff : 0, 0x00020000);
+  p.row = f < a.R ? (unsigned)((img * a.Nq + qi - (int)tq0) * C + head * a.d) * 2u : 0xF0000000u;
+  p.stat = f < a.R ? (unsigned)(((img - (int)img0) * heads + head) * a.Nq + qi) * 4u : 0xF0000000u;
+  return p;
+}
+
 // stores 32 channels (tile dt) of the flat rows a 32x32 accumulator tile holds as columns: the two lane halves exchange
-// quadruples so that a lane writes 16 bytes.  p = the row's first channel; live = the row exists.
+// quadruples so that a lane writes 16 bytes.
 template <int DT>
-__device__ __forceinline__ void store_tile(const f32x16& o, float f, uint16_t* p, bool live, int dt, int d, int h2) {
+__device__ __forceinline__ void store_tile(const f32x16& o, float f, const RowPlace& p, int dt, int d, int h2) {
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int c = 0; c < 4; c += 2) {
     const auto x = __builtin_amdgcn_permlane32_swap(pack2<DT>(o[4 * c] * f, o[4 * c + 1] * f),
@@ -98,7 +120,8 @@ __device__ __forceinline__ void store_tile(const f32x16& o, float f, uint16_t* p
     const auto y = __builtin_amdgcn_permlane32_swap(pack2<DT>(o[4 * c + 2] * f, o[4 * c + 3] * f),
                                                     pack2<DT>(o[4 * c + 6] * f, o[4 * c + 7] * f), false, false);
     const int d0 = 32 * dt + 8 * c + 8 * h2;
-    if (live && d0 < d) *reinterpret_cast<uint4*>(p + d0) = make_uint4(x[0], y[0], x[1], y[1]);
+    const u32x4 v = {x[0], y[0], x[1], y[1]};
+    __builtin_amdgcn_raw_buffer_store_b128(v, p.out, d0 < d ? p.row + 2u * (unsigned)d0 : 0xF0000000u, 0, 0);
   }
 }
 

@@ -71,8 +71,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 
   if (AHEAD && t < T) request(t, nx);
 
   for (int round = 0; RESIDENT ? t < T : round < rounds; t += step, ++round) {
-    const int f = 32 * t + li;
-    const bool live = f < a.R;
     uint4 qf[KS], df[KS];
     float delta = 0.f, l2;
     {
@@ -95,10 +93,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 
       delta += __shfl_xor(delta, 32, 64);
     }
     if (l2 == -INFINITY) l2 = INFINITY;  // a row without a key: P = exp2(0 - inf) = 0
-    int64_t b;
-    int qi, head;
-    place(min(t, T - 1), b, qi, head);
-    if (t < T && live && h2 == 0) a.delta[(b * a.kvh * a.hg + head) * a.Nq + qi] = delta;
+    const RowPlace out = row_place(a, e, g, min(t, T - 1), li, a.out, a.delta);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, delta), out.table, t < T && h2 == 0 ? out.stat : 0xF0000000u, 0, 0);
     f32x16 acc[OT];
 #pragma unroll
     for (int i = 0; i < OT; ++i)
@@ -155,9 +151,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 
       }
     }
     if (t >= T) continue;
-    uint16_t* p = a.out + b * a.sob + (int64_t)qi * a.sor + (int64_t)head * a.d;
 #pragma unroll
-    for (int i = 0; i < OT; ++i) store_tile<DT>(acc[i], a.scale, p, live, i, a.d, h2);
+    for (int i = 0; i < OT; ++i) store_tile<DT>(acc[i], a.scale, out, i, a.d, h2);
   }
 }
 

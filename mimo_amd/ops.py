@@ -982,7 +982,7 @@ def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
         raise L.MimoHipError(f"k {tuple(k.shape)}, v {tuple(v.shape)}: [encoder rows, keys, {kv_heads * d}]")
     if Be <= 0 or B % Be:
         raise L.MimoHipError(f"{B} images over {Be} encoder rows")
-    if B // Be * Nq * (heads // kv_heads) >= 1 << 30 or Be * kv_heads >= 1 << 16 or Nk >= 1 << 30:
+    if B // Be * Nq * (heads // kv_heads) >= 1 << 30 or Be * kv_heads >= 1 << 16 or Nk >= 1 << 30 or heads * Nq >= 1 << 27 or heads >= 1 << 16:
         raise L.MimoHipError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: beyond what the kernels address")
     _same(q, k=k, v=v)
     _rows_ok(q, "q")
