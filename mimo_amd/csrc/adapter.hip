@@ -84,24 +84,43 @@ __device__ __forceinline__ void store_planes(const LowArgs& a, uint16_t* p, f32x
 
 __device__ __forceinline__ float scale_of(const LowArgs& a, int ad) { return ad < 0 ? 0.f : a.scale ? a.scale[ad] : 1.f; }
 
-// u for rows by the 32 (MFMA 16x16x32, down as the row operand: a lane ends with four consecutive ranks of one row).
-// KSPLIT: the block's four waves share 32 rows and take every fourth k-step, joined in LDS in wave order — few rows; else
-// each wave has 32 rows of its own.  Bound by the stream of X; the adapter's k-steps come from L1 / L2.
+// u for rows by the 32 (MFMA 16x16x32, down as the row operand: a lane ends with four consecutive ranks of one row).  A wave takes
+// pieces of 64 channels: eight neighbouring lanes read 128 bytes of a row of X (of down), the piece passes through the wave's own
+// LDS patch into fragments, the next piece is on its way meanwhile — fragments straight from memory (a row per lane) cost the
+// address path a look-up per lane.  KSPLIT: the block's waves share 32 rows and take pieces in turn, joined in LDS in wave order —
+// few rows; else each of four waves has 32 rows of its own.  Bound by the stream of X; down comes from L2.
+constexpr int low_waves(int rt, bool ksplit) { return ksplit && rt < 8 ? 8 : 4; }
 template <int DT, int RT, bool KSPLIT>
-__global__ __launch_bounds__(256) void adapter_low_kernel(const LowArgs a) {
-  __shared__ f32x4 part[KSPLIT ? 4 * RT * 2 * 64 : 1];
+__global__ __launch_bounds__(64 * low_waves(RT, KSPLIT)) void adapter_low_kernel(const LowArgs a) {
+  constexpr int NW = low_waves(RT, KSPLIT), P = 72, PATCH = (32 + 16 * RT) * P;  // pitch: an odd number of 16-byte units
+  constexpr int BYTES = NW * PATCH * 2, PART = KSPLIT ? NW * RT * 2 * 64 * 16 : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[BYTES > PART ? BYTES : PART];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lg = lane >> 4, li = lane & 15;
+  const int lg = lane >> 4, li = lane & 15, row0 = lane >> 3, c8 = (lane & 7) * 8;
+  uint16_t* const xs = reinterpret_cast<uint16_t*>(smem) + wave * PATCH;
+  uint16_t* const dsm = xs + 32 * P;
   const int64_t m0 = KSPLIT ? (int64_t)blockIdx.x * 32 : ((int64_t)blockIdx.x * 4 + wave) * 32;
   if (m0 >= a.rows.M) return;
   int ad[2], todo[2];
-  const uint16_t* x[2];
 #pragma unroll
-  for (int mi = 0; mi < 2; ++mi) {
-    const int64_t m = m0 + 16 * mi + li;
-    ad[mi] = todo[mi] = adapter_of(a.rows, m);
-    x[mi] = a.X + (m < a.rows.M ? m : m0) * a.ldx;
-  }
+  for (int mi = 0; mi < 2; ++mi) ad[mi] = todo[mi] = adapter_of(a.rows, m0 + 16 * mi + li);
+  const int pieces = (a.K + 63) / 64, first = KSPLIT ? wave : 0, way = KSPLIT ? NW : 1;
+  uint4 xr[4], dr[2 * RT];
+  auto request = [&](int p, int cur) {
+    const int k = 64 * p + c8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = m0 + row0 + 8 * i;
+      xr[i] = make_uint4(0, 0, 0, 0);
+      if (k < a.K && m < a.rows.M) xr[i] = *reinterpret_cast<const uint4*>(a.X + m * a.ldx + k);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) {
+      const int j = row0 + 8 * i;
+      dr[i] = make_uint4(0, 0, 0, 0);
+      if (k < a.K && j < a.r) dr[i] = *reinterpret_cast<const uint4*>(a.down + ((int64_t)cur * a.r + j) * a.K + k);
+    }
+  };
   f32x4 res[RT][2];
 #pragma unroll
   for (int t = 0; t < RT; ++t) res[t][0] = res[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -109,22 +128,30 @@ __global__ __launch_bounds__(256) void adapter_low_kernel(const LowArgs a) {
     f32x4 acc[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; ++t) acc[t][0] = acc[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const uint16_t* dn = a.down + (int64_t)cur * a.r * a.K;
-    const int steps = (a.K + 31) / 32;
-#pragma unroll 4
-    for (int s = KSPLIT ? wave : 0; s < steps; s += KSPLIT ? 4 : 1) {
-      const int kk = 32 * s + 8 * lg;
-      uint4 fx[2], fa[RT];
+    if (first < pieces) request(first, cur);
+    for (int p = first; p < pieces; p += way) {
+      // LDS operations of a wave are carried out in order; the fences keep the compiler from reordering what other lanes wrote
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-      for (int mi = 0; mi < 2; ++mi) fx[mi] = kk < a.K ? *reinterpret_cast<const uint4*>(x[mi] + kk) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(xs + (row0 + 8 * i) * P + c8) = xr[i];
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-        fa[t] = (kk < a.K && 16 * t + li < a.r) ? *reinterpret_cast<const uint4*>(dn + (int64_t)(16 * t + li) * a.K + kk)
-                                               : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 2 * RT; ++i) *reinterpret_cast<uint4*>(dsm + (row0 + 8 * i) * P + c8) = dr[i];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (p + way < pieces) request(p + way, cur);
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
+      for (int h = 0; h < 2; ++h) {
+        uint4 fx[2];
 #pragma unroll
-        for (int mi = 0; mi < 2; ++mi) acc[t][mi] = HT<DT>::mfma16(fa[t], fx[mi], acc[t][mi]);
+        for (int mi = 0; mi < 2; ++mi) fx[mi] = *reinterpret_cast<const uint4*>(xs + (16 * mi + li) * P + 32 * h + 8 * lg);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const uint4 fa = *reinterpret_cast<const uint4*>(dsm + (16 * t + li) * P + 32 * h + 8 * lg);
+#pragma unroll
+          for (int mi = 0; mi < 2; ++mi) acc[t][mi] = HT<DT>::mfma16(fa, fx[mi], acc[t][mi]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
     for (int mi = 0; mi < 2; ++mi) {
@@ -137,18 +164,21 @@ __global__ __launch_bounds__(256) void adapter_low_kernel(const LowArgs a) {
     }
   }
   if constexpr (KSPLIT) {
+    f32x4* const part = reinterpret_cast<f32x4*>(smem);
+    lds_barrier();  // the patches are read
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int mi = 0; mi < 2; ++mi) part[((wave * RT + t) * 2 + mi) * 64 + lane] = res[t][mi];
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int mi = 0; mi < 2; ++mi) {
+        if ((2 * t + mi) % NW != wave) continue;  // (each wave finishes its share of the tiles)
         f32x4 v = part[(t * 2 + mi) * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += part[((w * RT + t) * 2 + mi) * 64 + lane];
+        for (int w = 1; w < NW; ++w) v += part[((w * RT + t) * 2 + mi) * 64 + lane];
         res[t][mi] = v;
       }
   }
@@ -159,7 +189,7 @@ __global__ __launch_bounds__(256) void adapter_low_kernel(const LowArgs a) {
     if (m >= a.rows.M) continue;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      if (KSPLIT && (2 * t + mi) % 4 != wave) continue;
+      if (KSPLIT && (2 * t + mi) % NW != wave) continue;
       const int j = 16 * t + 4 * lg;
       if (j >= a.r) continue;
       f32x4 v = res[t][mi] * sc;
@@ -215,10 +245,10 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(const TransposeA
     const int r0 = t / tc * 32, c0 = t % tc * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
     for (int i = y; i < 32; i += 8)
       if (r0 + i < R && c0 + x < C) tile[i][x] = in[(int64_t)(r0 + i) * C + c0 + x];
-    __syncthreads();
+    lds_barrier();
     for (int i = y; i < 32; i += 8)
       if (c0 + i < C && r0 + x < R) out[(int64_t)(c0 + i) * R + r0 + x] = tile[x][i];
-    __syncthreads();
+    lds_barrier();
   }
 }
 
@@ -234,6 +264,7 @@ struct OuterArgs {
   float lo_scale[2];  // what the remainder plane has to be multiplied with
   Rows rows;
   int r, ct0;      // ct0: column tiles of the first pair
+  FastDiv by_rpi, by_lc;
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -264,20 +295,27 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     range[0] = 0x7fffffff;
     range[1] = -1;
   }
-  __syncthreads();
+  lds_barrier();
   const int64_t G = (a.rows.M + a.rows.rpi - 1) / a.rows.rpi;
   int lo = 0x7fffffff, hi = -1;
-  for (int64_t i = tid; i < G; i += 256)
-    if (a.rows.index[i] == who) {
-      lo = lo < (int)i ? lo : (int)i;
-      hi = (int)i;
-    }
+  for (int64_t i0 = tid; i0 < G; i0 += 256 * 8) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i0 + 256 * u < G ? a.rows.index[i0 + 256 * u] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (v[u] == who) {
+        const int i = (int)i0 + 256 * u;
+        lo = lo < i ? lo : i;
+        hi = i;
+      }
+  }
   if (hi >= 0) {
     atomicMin(&range[0], lo);
     atomicMax(&range[1], hi);
   }
   for (int i = tid; i < MR * LP / 2; i += 256) reinterpret_cast<uint32_t*>(ls)[i] = 0u;  // columns behind the planes are never staged
-  __syncthreads();
+  lds_barrier();
   f32x4 acc[NA][RT][2];
 #pragma unroll
   for (int p = 0; p < NA; ++p)
@@ -290,39 +328,49 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     const int64_t tiles = (m_hi - m_lo + MR - 1) / MR, per = (tiles + gridDim.z - 1) / gridDim.z;
     const int64_t t_lo = blockIdx.z * per, t_hi = t_lo + per < tiles ? t_lo + per : tiles;
     const int lc = NP * a.r / 8;  // 16-byte chunks of a row of low
-    uint4 xr[NX], lr[NL];
-    auto fetch = [&](int64_t t) {
-      const int64_t m0 = m_lo + t * MR;
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const int id = tid + 256 * i, c = c0 + (id & 15) * 8;
-        const int64_t m = m0 + (id >> 4);
-        xr[i] = make_uint4(0, 0, 0, 0);
-        if (c < C && adapter_of(a.rows, m) == who) xr[i] = *reinterpret_cast<const uint4*>(a.x[z] + m * a.ldx[z] + c);
-      }
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int id = tid + 256 * i, row = id / lc;
-        const int64_t m = m0 + row;
-        lr[i] = make_uint4(0, 0, 0, 0);
-        if (row < MR && adapter_of(a.rows, m) == who) lr[i] = *reinterpret_cast<const uint4*>(a.low[z] + m * NP * a.r + (id - row * lc) * 8);
-      }
+    // a tile on its way.  No branch and no dependent load between the requests: rows behind the last one repeat it, columns behind
+    // the last one the first; `raw` = the index entry of row lane, it selects when the rows are written
+    struct Piece {
+      uint4 x[NX], l[NL];
+      int raw;
+      int64_t m0;
     };
-    if (t_lo < t_hi) fetch(t_lo);
-    for (int64_t t = t_lo; t < t_hi; ++t) {
-      __syncthreads();
+    auto fetch = [&](Piece& q, int64_t t) {
+      int id0 = tid;
+      asm volatile("" : "+v"(id0));
+      const int64_t m0 = q.m0 = m_lo + t * MR;
+      const int left = (int)(m_hi - m0 < MR ? m_hi - m0 : MR) - 1;
+      const int c = c0 + (id0 & 15) * 8;
+      const uint16_t* x = a.x[z] + m0 * a.ldx[z] + (c < C ? c : 0);
+      const uint16_t* l = a.low[z] + m0 * NP * a.r;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) q.x[i] = *reinterpret_cast<const uint4*>(x + min((id0 >> 4) + 16 * i, left) * a.ldx[z]);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int id = id0 + 256 * i, row = (int)div_fast(id, a.by_lc);
+        q.l[i] = *reinterpret_cast<const uint4*>(l + min(row, left) * NP * a.r + (id - row * lc) * 8);
+      }
+      const unsigned m = (unsigned)m0 + min(lane, left);
+      q.raw = a.rows.index[div_fast(m, a.by_rpi)];
+    };
+    auto use = [&](const Piece& q) {
+      int id0 = tid;
+      asm volatile("" : "+v"(id0));
+      const unsigned long long live = __builtin_amdgcn_ballot_w64(q.raw == who && q.m0 + lane < m_hi);
+      lds_barrier();
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
-        const int id = tid + 256 * i;
-        *reinterpret_cast<uint4*>(xs + (id >> 4) * XP + (id & 15) * 8) = xr[i];
+        const int row = (id0 >> 4) + 16 * i;
+        *reinterpret_cast<uint4*>(xs + row * XP + (id0 & 15) * 8) = (live >> row) & 1 ? q.x[i] : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int id = tid + 256 * i, row = id / lc;
-        if (row < MR) *reinterpret_cast<uint4*>(ls + row * LP + (id - row * lc) * 8) = lr[i];
+        const int id = id0 + 256 * i, row = (int)div_fast(id, a.by_lc);
+        if (row < MR) *reinterpret_cast<uint4*>(ls + row * LP + (id - row * lc) * 8) = (live >> row) & 1 ? q.l[i] : make_uint4(0, 0, 0, 0);
       }
-      __syncthreads();
-      if (t + 1 < t_hi) fetch(t + 1);
+      lds_barrier();
+    };
+    auto products = [&]() {
 #pragma unroll
       for (int k0 = 0; k0 < MR; k0 += 32) {
         uint4 fx[2];
@@ -337,6 +385,28 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
             for (int c = 0; c < 2; ++c) acc[p % NA][q][c] = HT<DT>::mfma16(fl, fx[c], acc[p % NA][q][c]);
           }
         }
+      }
+    };
+    if constexpr (RT <= 4) {  // two tiles ahead of the products (the largest ranks have registers for one)
+      Piece q0, q1;
+      if (t_lo < t_hi) fetch(q0, t_lo);
+      if (t_lo + 1 < t_hi) fetch(q1, t_lo + 1);
+      for (int64_t t = t_lo; t < t_hi; t += 2) {
+        use(q0);
+        if (t + 2 < t_hi) fetch(q0, t + 2);
+        products();
+        if (t + 1 >= t_hi) break;
+        use(q1);
+        if (t + 3 < t_hi) fetch(q1, t + 3);
+        products();
+      }
+    } else {
+      Piece q0;
+      if (t_lo < t_hi) fetch(q0, t_lo);
+      for (int64_t t = t_lo; t < t_hi; ++t) {
+        use(q0);
+        if (t + 1 < t_hi) fetch(q0, t + 1);
+        products();
       }
     }
   }
@@ -356,22 +426,190 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
   }
 }
 
-// the sum of the parts in order: ddown [n, r, K] as it lies, dup [n, N, r] transposed
+// the sum of the parts in order: ddown [n, r, K] as it lies, dup [n, N, r] transposed.  A thread takes four columns; eight parts are
+// on their way at a time.
 __global__ __launch_bounds__(256) void adapter_join_kernel(const float* p0, const float* p1, float* ddown, float* dup, int n, int r, int K,
                                                            int N, int parts) {
-  const int64_t s0 = (int64_t)n * r * K, s1 = (int64_t)n * r * N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < s0 + s1; i += (int64_t)gridDim.x * 256) {
-    const bool first = i < s0;
-    const int64_t at = first ? i : i - s0, plane = first ? s0 : s1;
-    const float* p = (first ? p0 : p1) + at;
-    float s = p[0];
-    for (int q = 1; q < parts; ++q) s += p[(int64_t)q * plane];
-    if (first) {
-      ddown[at] = s;
-    } else {
-      const int64_t row = at / N;  // (adapter, rank)
-      dup[(row / r * N + (at - row * N)) * r + row % r] = s;
+  const int64_t s0 = (int64_t)n * r * K, s1 = (int64_t)n * r * N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= s0 + s1) return;
+  const bool first = i < s0;
+  const int64_t at = first ? i : i - s0, plane = first ? s0 : s1;
+  const float* p = (first ? p0 : p1) + at;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int q0 = 0; q0 < parts; q0 += 8) {
+    f32x4 x[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q0 + q < parts) x[q] = *reinterpret_cast<const f32x4*>(p + (int64_t)(q0 + q) * plane);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q0 + q < parts) s += x[q];
+  }
+  if (first) {
+    *reinterpret_cast<f32x4*>(ddown + at) = s;
+  } else {
+    const int64_t row = at / N, c = at - row * N;  // row: (adapter, rank)
+    float* o = dup + (row / r * N + c) * r + row % r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[(int64_t)k * r] = s[k];
+  }
+}
+
+// A few rows (M <= 16 MG) against the whole weight: a block of eight waves takes 16 columns, the waves share K (every eighth
+// k-step) and meet in LDS in wave order.  Bound by latency: one trip to W, one to the adapters.  RT > 0 (MG = 1): u is computed
+// here too, by every block for itself — the rows' down weights come from L2 and a launch is saved; RT = 0: u is given.
+struct SkinnyArgs {
+  const uint16_t *X, *W, *down, *up;
+  const float *scale, *bias;
+  const void* res;
+  void* out;
+  uint16_t* low;
+  int64_t ldx, ldo, ldr;
+  Rows rows;
+  int N, K, r, planes, cols;  // cols: columns of low that take part (planes r for a fp32 result, else r)
+  unsigned flags;
+};
+template <int DT, int MG, int RT>
+__global__ __launch_bounds__(512) void adapter_skinny_kernel(const SkinnyArgs a) {
+  constexpr int ULP = 3 * 16 * (RT > 0 ? RT : 1) + 8;
+  __shared__ f32x4 part[8][MG + RT][64];
+  __shared__ __attribute__((aligned(16))) uint16_t us[RT > 0 ? 16 * ULP : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lg = lane >> 4, li = lane & 15, n0 = blockIdx.x * 16;
+  int ad[MG];
+  const uint16_t* x[MG];
+#pragma unroll
+  for (int g = 0; g < MG; ++g) {
+    const int64_t m = 16 * g + li;
+    x[g] = a.X + (m < a.rows.M ? m : 0) * a.ldx;
+    ad[g] = adapter_of(a.rows, m);
+  }
+  const uint16_t* w = a.W + (int64_t)(n0 + li < a.N ? n0 + li : 0) * a.K;
+  const int steps = (a.K + 31) / 32;
+  f32x4 acc[MG];
+#pragma unroll
+  for (int g = 0; g < MG; ++g) acc[g] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  constexpr int UB = MG == 1 ? 5 : 3;
+  for (int s0 = wave; s0 < steps; s0 += 8 * UB) {
+    uint4 fw[UB], fx[UB][MG];
+#pragma unroll
+    for (int b = 0; b < UB; ++b) {
+      const int kk = 32 * (s0 + 8 * b) + 8 * lg;
+      fw[b] = make_uint4(0, 0, 0, 0);
+      if (kk < a.K) fw[b] = *reinterpret_cast<const uint4*>(w + kk);
+#pragma unroll
+      for (int g = 0; g < MG; ++g) {
+        fx[b][g] = make_uint4(0, 0, 0, 0);
+        if (kk < a.K) fx[b][g] = *reinterpret_cast<const uint4*>(x[g] + kk);
+      }
     }
+#pragma unroll
+    for (int b = 0; b < UB; ++b)
+#pragma unroll
+      for (int g = 0; g < MG; ++g) acc[g] = HT<DT>::mfma16(fw[b], fx[b][g], acc[g]);
+  }
+  if constexpr (RT > 0) {
+    f32x4 u[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) u[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    int todo[1] = {ad[0]};
+    for (int cur = next_adapter<1>(todo); cur >= 0; cur = next_adapter<1>(todo)) {
+      const uint16_t* dn = a.down + (int64_t)cur * a.r * a.K;
+      f32x4 v[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) v[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int s0 = wave; s0 < steps; s0 += 8 * UB) {
+        uint4 fd[UB][RT], fx[UB];
+#pragma unroll
+        for (int b = 0; b < UB; ++b) {
+          const int kk = 32 * (s0 + 8 * b) + 8 * lg;
+          fx[b] = make_uint4(0, 0, 0, 0);
+          if (kk < a.K) fx[b] = *reinterpret_cast<const uint4*>(x[0] + kk);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            fd[b][t] = make_uint4(0, 0, 0, 0);
+            if (kk < a.K && 16 * t + li < a.r) fd[b][t] = *reinterpret_cast<const uint4*>(dn + (int64_t)(16 * t + li) * a.K + kk);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < UB; ++b)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) v[t] = HT<DT>::mfma16(fd[b][t], fx[b], v[t]);
+      }
+      const bool mine = todo[0] == cur;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[t][i] = mine ? v[t][i] : u[t][i];
+      todo[0] = mine ? -1 : todo[0];
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) part[wave][MG + t][lane] = u[t];
+  }
+#pragma unroll
+  for (int g = 0; g < MG; ++g) part[wave][g][lane] = acc[g];
+  lds_barrier();
+  // wave t < RT finishes rank tile t, then wave g of the first MG finishes row group g
+  if constexpr (RT > 0) {
+    if (wave < RT) {
+      f32x4 v = part[0][MG + wave][lane];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) v += part[q][MG + wave][lane];
+      const int j = 16 * wave + 4 * lg;
+      if (j < a.r) {
+        const LowArgs la{nullptr, nullptr, a.scale, nullptr, 0, a.rows, 0, a.r, a.planes, 1.f};
+        v *= scale_of(la, ad[0]);
+        if (ad[0] < 0) v = (f32x4){0.f, 0.f, 0.f, 0.f};
+        store_planes<DT>(la, us + li * ULP + j, v);
+        if (blockIdx.x == 0 && a.low && li < a.rows.M) store_planes<DT>(la, a.low + (int64_t)li * a.planes * a.r + j, v);
+      }
+    }
+    lds_barrier();
+  }
+  if (wave >= MG) return;
+  // (a wave's row group by its number: unrolled so that ad[] stays in registers)
+#pragma unroll
+  for (int g = 0; g < MG; ++g) {
+    if (wave != g) continue;
+    f32x4 v = part[0][g][lane];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) v += part[q][g][lane];
+    const int64_t m = 16 * g + li;
+    int todo[1] = {ad[g]};
+    for (int cur = next_adapter<1>(todo); cur >= 0; cur = next_adapter<1>(todo)) {
+      const bool mine = todo[0] == cur;
+      const uint16_t* up = a.up + ((int64_t)cur * a.N + (n0 + li < a.N ? n0 + li : 0)) * a.r;
+      f32x4 y = v;
+      for (int k0 = 0; k0 < a.cols; k0 += 32) {
+        const int kk = k0 + 8 * lg;
+        int ku = kk;
+        while (ku >= a.r) ku -= a.r;
+        uint4 fb = make_uint4(0, 0, 0, 0), fu = make_uint4(0, 0, 0, 0);
+        if (kk < a.cols) {
+          fb = *reinterpret_cast<const uint4*>(up + ku);
+          if (mine) fu = RT > 0 ? *reinterpret_cast<const uint4*>(us + li * ULP + kk)
+                                : *reinterpret_cast<const uint4*>(a.low + m * a.planes * a.r + kk);
+        }
+        y = HT<DT>::mfma16(fb, fu, y);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = mine ? y[i] : v[i];
+      todo[0] = mine ? -1 : todo[0];
+    }
+    const int n = n0 + 4 * lg;
+    if (m >= a.rows.M || n >= a.N) continue;  // (N % 8 == 0: whole quadruples)
+    if (a.bias) v += *reinterpret_cast<const f32x4*>(a.bias + n);
+    if (a.res) {
+      if (a.flags & MIMO_EPI_RES_F32) {
+        v += *reinterpret_cast<const f32x4*>((const float*)a.res + m * a.ldr + n);
+      } else {
+        const uint2 h = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + m * a.ldr + n);
+        v += (f32x4){HT<DT>::to_f((uint16_t)(h.x & 0xffffu)), HT<DT>::to_f((uint16_t)(h.x >> 16)), HT<DT>::to_f((uint16_t)(h.y & 0xffffu)),
+                     HT<DT>::to_f((uint16_t)(h.y >> 16))};
+      }
+    }
+    if (a.flags & MIMO_EPI_OUT_F32) *reinterpret_cast<f32x4*>((float*)a.out + m * a.ldo + n) = v;
+    else *reinterpret_cast<uint2*>((uint16_t*)a.out + m * a.ldo + n) = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
   }
 }
 
@@ -391,7 +629,7 @@ int launch_low(const LowArgs& a, hipStream_t st) {
   if (nwg > 0x7fffffff) return MIMO_EINVAL;
 #define LOW(RT)                                                                                                                  \
   do {                                                                                                                           \
-    if (ksplit) hipLaunchKernelGGL((adapter_low_kernel<DT, RT, true>), dim3((unsigned)nwg), dim3(256), 0, st, a);                \
+    if (ksplit) hipLaunchKernelGGL((adapter_low_kernel<DT, RT, true>), dim3((unsigned)nwg), dim3(64 * low_waves(RT, true)), 0, st, a); \
     else hipLaunchKernelGGL((adapter_low_kernel<DT, RT, false>), dim3((unsigned)nwg), dim3(256), 0, st, a);                      \
   } while (0)
   if (rt == 1) LOW(1);
@@ -429,8 +667,10 @@ int launch_tiles(GemmArgs& g, hipStream_t st) {
     const int64_t nwg = ((g.M + 127) / 128) * tn_s;
     if (nwg > 0x3fffffff) return MIMO_EINVAL;
     if (nwg <= cus) {
-      const int64_t nwg64 = ((g.M + 63) / 64) * tn_s;
-      hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 2, 2, 2, 3>), dim3((unsigned)nwg64), dim3(256), 0, st, g);
+      // (128-column tiles: three ring slots of 64 x 128 leave room for a second block per CU)
+      g.tiles_n = (g.N + 127) / 128;
+      const int64_t nwg64 = ((g.M + 63) / 64) * g.tiles_n;
+      hipLaunchKernelGGL((gemm_kernel<DT, 4, 0, 2, 2, 3, 2, 3>), dim3((unsigned)nwg64), dim3(256), 0, st, g);
     } else {
       hipLaunchKernelGGL((gemm_kernel<DT, NR, 0, 2, 2, 2, 4, 3>), dim3((unsigned)nwg), dim3(256), 0, st, g);
     }
@@ -498,8 +738,32 @@ GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t
   return g;
 }
 
+// Up to 64 rows: the skinny kernel; u inside it for one or two rows (it takes their adapters one after another).
 template <int DT>
-int forward(GemmArgs g, const LowArgs& la, hipStream_t st) {
+int launch_skinny(const GemmArgs& g, const LowArgs& la, bool give_low, hipStream_t st) {
+  SkinnyArgs a{g.A, g.W, la.down, g.ad_up, la.scale, g.bias, g.res, g.out, give_low ? la.low : nullptr, g.lda, g.ldo, g.ldr, la.rows,
+               g.N, g.K, la.r, la.planes, g.ad_cols, g.flags};
+  const dim3 grid((unsigned)((g.N + 15) / 16));
+  const int rt = (la.r + 15) / 16, mg = (int)((g.M + 15) / 16);
+  if (g.M <= 2 && rt <= 4) {
+    if (rt == 1) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 1>), grid, dim3(512), 0, st, a);
+    else if (rt == 2) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 2>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 4>), grid, dim3(512), 0, st, a);
+    MIMO_LAUNCH_CHECK();
+    return MIMO_OK;
+  }
+  if (const int rc = launch_low<DT>(la, st)) return rc;
+  a.low = la.low;
+  if (mg == 1) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 0>), grid, dim3(512), 0, st, a);
+  else if (mg == 2) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 2, 0>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((adapter_skinny_kernel<DT, 4, 0>), grid, dim3(512), 0, st, a);
+  MIMO_LAUNCH_CHECK();
+  return MIMO_OK;
+}
+
+template <int DT>
+int forward(const GemmArgs& g, const LowArgs& la, hipStream_t st) {
+  if (g.M <= 64) return launch_skinny<DT>(g, la, la.planes > 1, st);
   if (const int rc = launch_low<DT>(la, st)) return rc;
   return launch_gemm<DT>(g, st);
 }
@@ -513,7 +777,7 @@ BackwardPlan backward_plan(int dtype, const mimo_adapter_params* p, int64_t M, i
   BackwardPlan b{};
   const int64_t n = p->count, r = p->rank;
   const int64_t blocks = n * ((N + 127) / 128 + (K + 127) / 128), tiles = (M + 63) / 64;
-  int64_t parts = (2 * (int64_t)cu_count() + blocks - 1) / blocks;  // two blocks per CU; a part keeps at least four row tiles
+  int64_t parts = (3 * (int64_t)cu_count() + blocks - 1) / blocks;  // three blocks per CU; a part keeps at least four row tiles
   if (parts > tiles / 4) parts = tiles / 4;
   if (parts > 256) parts = 256;
   b.parts = parts < 1 ? 1 : (int)parts;
@@ -551,7 +815,7 @@ int backward(const void* dY, int64_t ldy, const void* A, int64_t lda, const void
     if (const int rc = launch_gemm<DT>(g, st)) return rc;
   }
   OuterArgs oa{{(const uint16_t*)A, (const uint16_t*)dY}, {t, (const uint16_t*)low}, {p0, p1}, {lda, ldy}, {K, N}, {1.f / up2, 1.f}, rows, r,
-               (K + 127) / 128};
+               (K + 127) / 128, fast_div(rows.rpi), fast_div((uint32_t)(NP * r / 8))};
   const dim3 grid((unsigned)((K + 127) / 128 + (N + 127) / 128), (unsigned)n, (unsigned)b.parts);
   const int rt = (r + 15) / 16;
   if (rt == 1) hipLaunchKernelGGL((adapter_outer_kernel<DT, 1>), grid, dim3(256), 0, st, oa);
@@ -559,8 +823,9 @@ int backward(const void* dY, int64_t ldy, const void* A, int64_t lda, const void
   else if (rt <= 4) hipLaunchKernelGGL((adapter_outer_kernel<DT, 4>), grid, dim3(256), 0, st, oa);
   else hipLaunchKernelGGL((adapter_outer_kernel<DT, 8>), grid, dim3(256), 0, st, oa);
   MIMO_LAUNCH_CHECK();
-  const int64_t total = (int64_t)n * r * (N + K), nwg = (total + 255) / 256;
-  hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)(nwg > 2048 ? 2048 : nwg)), dim3(256), 0, st, p0, p1, ddown, dup, n, r, K, N,
+  const int64_t total = (int64_t)n * r * (N + K), nwg = (total / 4 + 255) / 256;
+  if (nwg > 0x7fffffff) return MIMO_EINVAL;
+  hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)nwg), dim3(256), 0, st, p0, p1, ddown, dup, n, r, K, N,
                      b.parts);
   MIMO_LAUNCH_CHECK();
   return MIMO_OK;

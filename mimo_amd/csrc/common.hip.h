@@ -134,6 +134,25 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Rendezvous of a block over LDS: __syncthreads() also waits (vmcnt) for every global load and store under way
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// n / d for n < 2^31: (n * mul) >> (31 + shift), mul = floor(2^(31 + shift) / d) + 1, shift = ceil(log2 d); exact, because
+// mul d exceeds 2^(31 + shift) by at most d <= 2^shift and n < 2^31.
+struct FastDiv {
+  uint32_t d, mul;
+  int shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  while ((1ull << f.shift) < d) ++f.shift;
+  f.mul = (uint32_t)((1ull << (31 + f.shift)) / d + 1);
+  return f;
+}
+__device__ __forceinline__ uint32_t div_fast(uint32_t n, const FastDiv& f) {
+  return f.d == 1u ? n : (uint32_t)(((uint64_t)n * f.mul) >> (31 + f.shift));
+}
+
 // XCD-aware bijective remap of a 1-D block id: blocks b, b+8, b+16 ... (which the dispatcher
 // places on the same XCD) get consecutive logical ids, so tiles that share an operand panel
 // share one L2 (cdna_hip_programming.md T1, bijective form).

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
   stager.open(a, e, g);
   if constexpr (RESIDENT) {
     stage_all<DT, KS, THREADS>(a, e, g, len, ks_of(0), vs_of(0), bias_of(0), ones, tid);
-    __syncthreads();
+    lds_barrier();
   }
   const int step = a.nb * NW;
   int t = j * NW + wave;
@@ -181,12 +181,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
       const int chunks = (k_hi - k_lo + CHK - 1) / CHK;
       if (chunks > 0) {
         stager.issue(a, e, k_hi, k_lo, tid);
-        if (round > 0) __syncthreads();  // the previous round's last chunk is read
+        if (round > 0) lds_barrier();  // the previous round's last chunk is read
         stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), ones, tid);
         if (chunks > 1) stager.issue(a, e, k_hi, k_lo + CHK, tid);
       }
       for (int i = 0; i < chunks; ++i) {
-        __syncthreads();
+        lds_barrier();
         const int b = i & 1;
         if (t < T) tiles(ks_of(b), vs_of(b), bias_of(b), 0, IC<CHK / 32>{}, a.mask || k_lo + (i + 1) * CHK > k_hi);
         if (i + 1 < chunks) {
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const Args a) {
     for (int s = 0; s < 8; ++s)
       if (s < n) x[s] = *reinterpret_cast<const f32x4*>(src + (int64_t)s * rows * a.d);
   }
-  __syncthreads();
+  lds_barrier();
   if (!mine) return;
   float m = -INFINITY;
   for (int s = 0; s < n; ++s) m = fmaxf(m, part[r * n + s][0]);

@@ -12,22 +12,6 @@ namespace mimo_xattn {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// n / d for n < 2^31: (n * mul) >> (31 + shift), mul = floor(2^(31 + shift) / d) + 1, shift = ceil(log2 d); exact, because
-// mul d exceeds 2^(31 + shift) by at most d <= 2^shift and n < 2^31.
-struct FastDiv {
-  uint32_t d, mul;
-  int shift;
-};
-inline FastDiv fast_div(uint32_t d) {
-  FastDiv f{d, 0, 0};
-  while ((1ull << f.shift) < d) ++f.shift;
-  f.mul = (uint32_t)((1ull << (31 + f.shift)) / d + 1);
-  return f;
-}
-__device__ __forceinline__ uint32_t div_fast(uint32_t n, const FastDiv& f) {
-  return f.d == 1u ? n : (uint32_t)(((uint64_t)n * f.mul) >> (31 + f.shift));
-}
-
 struct Args {
   const uint16_t *q, *k, *v;
   const uint16_t *o, *dout;      // backward: the forward's output and its gradient
@@ -141,7 +125,7 @@ constexpr int lanes_of(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 8 : ks <= 8 ? 16
 
 // Key and value rows [key0, key0 + N) of (e, g) on their way into row-major LDS tiles of pitch 16 KS + 8 halfs (an odd number of
 // 16-byte units: a 16-lane group of b128 row reads covers all banks).  issue() requests the rows, commit() writes them: between
-// the two a block computes on other rows.  Only keys below len are read; what the mask drops, what lies behind len and channels
+// the two a block computes on other rows.  Only keys below len are read; what the mask drops, rows behind len and channels
 // >= d are ZERO in LDS whatever memory holds there (NaN included), and bias[i] = 0 or -inf is added to their scores.
 // ones: V's channel d, which pads the last 32-channel tile, is 1 — the product with P then also leaves the sum of P in that row.
 template <int KS, int THREADS, int N>
@@ -155,42 +139,40 @@ struct Stager {
     kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
     vb = a.v + (int64_t)e * a.svb + (int64_t)g * a.d;
   }
+  // (no branch, no select between the requests: keys behind the last one repeat it, channels behind the last one the first)
   __device__ __forceinline__ void issue(const Args& a, int e, int len, int key0, int tid) {
     asm volatile("" : "+v"(tid));  // addresses are made anew for every piece: kept over the products they would cost registers
-    const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
-    const uint16_t* kp = kb + (int64_t)(key0 + row0) * a.skr + cc;
-    const uint16_t* vp = vb + (int64_t)(key0 + row0) * a.svr + cc;
-    left = len - key0;
+    const int row0 = tid / LPR, c = (tid & (LPR - 1)) * 8, cc = c < a.d ? c : 0;
+    left = len - key0;  // > 0
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (cc < a.d && row0 + i * RP < left) {
-        kr[i] = *reinterpret_cast<const uint4*>(kp + (int64_t)(i * RP) * a.skr);
-        vr[i] = *reinterpret_cast<const uint4*>(vp + (int64_t)(i * RP) * a.svr);
-      }
+      const int key = key0 + min(row0 + i * RP, left - 1);
+      kr[i] = *reinterpret_cast<const uint4*>(kb + (int64_t)key * a.skr + cc);
+      vr[i] = *reinterpret_cast<const uint4*>(vb + (int64_t)key * a.svr + cc);
     }
     static_assert(N <= 64, "a lane per key of the mask");
     keep = 1;
-    if (a.mask && (tid & 63) < left) keep = a.mask[(int64_t)e * a.smb + key0 + (tid & 63)];
+    if (a.mask) keep = a.mask[(int64_t)e * a.smb + key0 + min(tid & 63, left - 1)];
   }
   template <int DT>
   __device__ __forceinline__ void commit(const Args& a, uint16_t* ks, uint16_t* vs, float* bias, bool ones, int tid) {
     asm volatile("" : "+v"(tid));
     const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
-    const unsigned long long live = __builtin_amdgcn_ballot_w64(keep != 0);
+    const bool mine = (tid & 63) < left && keep != 0;
+    const unsigned long long live = __builtin_amdgcn_ballot_w64(mine);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int row = row0 + i * RP;
       if (cc < 16 * KS && (N % RP == 0 || row < N)) {
-        uint4 x = kr[i], y = vr[i];
-        if (a.mask && !((live >> row) & 1)) x = y = make_uint4(0, 0, 0, 0);
+        const bool ok = ((live >> (row & 63)) & 1) && cc < a.d;
+        uint4 x = ok ? kr[i] : make_uint4(0, 0, 0, 0), y = ok ? vr[i] : make_uint4(0, 0, 0, 0);
         if (ones && cc == a.d) y.x = HT<DT>::from_f(1.f);
         *reinterpret_cast<uint4*>(ks + row * P + cc) = x;
         *reinterpret_cast<uint4*>(vs + row * P + cc) = y;
       }
     }
     if (tid < N) {
-      bias[tid] = tid < left && keep ? 0.f : -INFINITY;
+      bias[tid] = mine ? 0.f : -INFINITY;
       if (ones && a.d == 16 * KS) vs[tid * P + a.d] = HT<DT>::from_f(1.f);
     }
   }

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 
   stager.open(a, e, g);
   if constexpr (RESIDENT) {
     stage_all<DT, KS, THREADS>(a, e, g, len, ks_of(0), vs_of(0), bias_of(0), false, tid);
-    __syncthreads();
+    lds_barrier();
   }
   const int step = a.nb * NW;
   int t = j * NW + wave;
@@ -133,12 +133,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 
       const int chunks = (len + CH - 1) / CH;
       if (chunks > 0) {
         stager.issue(a, e, len, 0, tid);
-        if (round > 0) __syncthreads();
+        if (round > 0) lds_barrier();
         stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), false, tid);
         if (chunks > 1) stager.issue(a, e, len, CH, tid);
       }
       for (int i = 0; i < chunks; ++i) {
-        __syncthreads();
+        lds_barrier();
         const int bf = i & 1;
         if (t < T) {
           tile(ks_of(bf), vs_of(bf), bias_of(bf), 0, a.mask || i * CH + 32 > len);
@@ -199,38 +199,33 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
-  // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to buffer b (commit); rows that
-  // do not exist: zeros, P = 0
+  // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to buffer b (commit).  Rows
+  // behind the last one repeat it with lse = inf: P = 0.  Channels behind the last one repeat the first: K and V are zero there.
   constexpr int LPR = lanes_of(KS), RP = THREADS / LPR, NC = (QT + RP - 1) / RP;
   uint4 xr[NC], yr[NC];
   float lr, dr;
+  int on_way = 0;
   auto issue = [&](int t) {
     int id = tid;
     asm volatile("" : "+v"(id));  // addresses are made anew for every tile
-    const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
+    const int row0 = id / LPR, c = (id & (LPR - 1)) * 8, cc = c < a.d ? c : 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int row = row0 + i * RP, f = t * QT + row;
-      xr[i] = yr[i] = make_uint4(0, 0, 0, 0);
-      if (cc < a.d && f < a.R && (QT % RP == 0 || row < QT)) {
-        int img, qi, hh;
-        flat_row(a, f, img, qi, hh);
-        const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
-        xr[i] = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
-        yr[i] = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
-      }
-    }
-    static_assert(QT <= THREADS, "a thread per row");
-    lr = -INFINITY;
-    dr = 0.f;
-    const int f = t * QT + id;
-    if (id < QT && f < a.R) {
+      const int f = min(t * QT + row0 + i * RP, a.R - 1);
       int img, qi, hh;
       flat_row(a, f, img, qi, hh);
-      const int64_t stat = (((int64_t)e * a.G + img) * a.kvh * a.hg + g * a.hg + hh) * a.Nq + qi;
-      lr = a.lse_in[stat];
-      dr = a.delta[stat];
+      const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
+      xr[i] = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
+      yr[i] = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
     }
+    static_assert(QT <= THREADS, "a thread per row");
+    const int f = min(t * QT + (id & (QT - 1)), a.R - 1);
+    int img, qi, hh;
+    flat_row(a, f, img, qi, hh);
+    const int64_t stat = (((int64_t)e * a.G + img) * a.kvh * a.hg + g * a.hg + hh) * a.Nq + qi;
+    lr = a.lse_in[stat];
+    dr = a.delta[stat];
+    on_way = t;
   };
   auto commit = [&](int b) {
     int id = tid;
@@ -247,7 +242,7 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
       }
     }
     if (id < QT) {
-      l2[id] = lr == -INFINITY ? INFINITY : lr * LOG2E;
+      l2[id] = lr == -INFINITY || on_way * QT + id >= a.R ? INFINITY : lr * LOG2E;
       l2[QT + id] = dr;
     }
   };
@@ -258,7 +253,7 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
   }
   for (int t = t_lo; t < t_hi; ++t) {
     const int b = (t - t_lo) & 1;
-    __syncthreads();
+    lds_barrier();
     const uint16_t* qs = reinterpret_cast<const uint16_t*>(smem + b * BUF);
     const uint16_t* ds = qs + QT * P;
     const float* l2 = reinterpret_cast<const float*>(smem + b * BUF + 2 * QT * P * 2 + 64);

@@ -1213,6 +1213,13 @@ __global__ __launch_bounds__(64 * WM * WN, (EPI == 3 && WM * WN == 4) ? 2 : (WM 
 
   MIMO_TRACE_REAL(g, tr, 0xfe);
   MIMO_TRACE(g, tr, 1);
+  [[maybe_unused]] auto vote = [&]() {
+    tile_ad = adapter_vote<(BM + 63) / 64>(ad_rows);
+    if (tile_ad >= 0) kt_hi += (g.ad_cols + BK - 1) / BK;
+  };
+  if constexpr (EPI == 3) {
+    if (g.nkt < NSTAGE - 1) vote();  // a low-rank K-tile is among the first requests already
+  }
 #pragma unroll
   for (int i = 0; i < NSTAGE - 1; ++i) load_tile(kt_lo + i, i);
   if constexpr (EPI == 2) {   // (the K loop's barriers order these LDS writes before the epilogue's reads)
@@ -1221,9 +1228,8 @@ __global__ __launch_bounds__(64 * WM * WN, (EPI == 3 && WM * WN == 4) ? 2 : (WM 
       row_stats_finish(g, BM, BN, tid, rsq, csq, mr, mr + 2 * BM);
     }
   }
-  if constexpr (EPI == 3) {  // (requested before K-tile 0, whose arrival the first step waits for anyway)
-    tile_ad = adapter_vote<(BM + 63) / 64>(ad_rows);
-    if (tile_ad >= 0) kt_hi += (g.ad_cols + BK - 1) / BK;
+  if constexpr (EPI == 3) {
+    if (g.nkt >= NSTAGE - 1) vote();  // (requested before K-tile 0, whose arrival the first step waits for anyway)
   }
   for (int kt = kt_lo; kt < kt_hi; kt += NSTAGE) {
     step(IC<0>{}, kt);
