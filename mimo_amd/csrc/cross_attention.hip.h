@@ -139,16 +139,18 @@ struct Stager {
     kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
     vb = a.v + (int64_t)e * a.svb + (int64_t)g * a.d;
   }
-  // (no branch, no select between the requests: keys behind the last one repeat it, channels behind the last one the first)
+  // (one branch around all requests, no select between them: keys behind the last one repeat it)
   __device__ __forceinline__ void issue(const Args& a, int e, int len, int key0, int tid) {
     asm volatile("" : "+v"(tid));  // addresses are made anew for every piece: kept over the products they would cost registers
-    const int row0 = tid / LPR, c = (tid & (LPR - 1)) * 8, cc = c < a.d ? c : 0;
+    const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
     left = len - key0;  // > 0
+    if (cc < a.d) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int key = key0 + min(row0 + i * RP, left - 1);
-      kr[i] = *reinterpret_cast<const uint4*>(kb + (int64_t)key * a.skr + cc);
-      vr[i] = *reinterpret_cast<const uint4*>(vb + (int64_t)key * a.svr + cc);
+      for (int i = 0; i < NC; ++i) {
+        const int key = key0 + min(row0 + i * RP, left - 1);
+        kr[i] = *reinterpret_cast<const uint4*>(kb + (int64_t)key * a.skr + cc);
+        vr[i] = *reinterpret_cast<const uint4*>(vb + (int64_t)key * a.svr + cc);
+      }
     }
     static_assert(N <= 64, "a lane per key of the mask");
     keep = 1;

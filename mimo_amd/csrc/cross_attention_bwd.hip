@@ -200,7 +200,7 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
   // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to buffer b (commit).  Rows
-  // behind the last one repeat it with lse = inf: P = 0.  Channels behind the last one repeat the first: K and V are zero there.
+  // behind the last one repeat it with lse = inf: P = 0.  Channels behind the last one are zeros.
   constexpr int LPR = lanes_of(KS), RP = THREADS / LPR, NC = (QT + RP - 1) / RP;
   uint4 xr[NC], yr[NC];
   float lr, dr;
@@ -208,15 +208,17 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
   auto issue = [&](int t) {
     int id = tid;
     asm volatile("" : "+v"(id));  // addresses are made anew for every tile
-    const int row0 = id / LPR, c = (id & (LPR - 1)) * 8, cc = c < a.d ? c : 0;
+    const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
+    if (cc < a.d) {  // (one branch around all requests)
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int f = min(t * QT + row0 + i * RP, a.R - 1);
-      int img, qi, hh;
-      flat_row(a, f, img, qi, hh);
-      const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
-      xr[i] = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
-      yr[i] = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
+      for (int i = 0; i < NC; ++i) {
+        const int f = min(t * QT + min(row0 + i * RP, QT - 1), a.R - 1);
+        int img, qi, hh;
+        flat_row(a, f, img, qi, hh);
+        const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
+        xr[i] = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
+        yr[i] = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
+      }
     }
     static_assert(QT <= THREADS, "a thread per row");
     const int f = min(t * QT + (id & (QT - 1)), a.R - 1);
@@ -237,8 +239,8 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
     for (int i = 0; i < NC; ++i) {
       const int row = row0 + i * RP;
       if (cc < 16 * KS && (QT % RP == 0 || row < QT)) {
-        *reinterpret_cast<uint4*>(qs + row * P + cc) = xr[i];
-        *reinterpret_cast<uint4*>(qs + QT * P + row * P + cc) = yr[i];
+        *reinterpret_cast<uint4*>(qs + row * P + cc) = cc < a.d ? xr[i] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(qs + QT * P + row * P + cc) = cc < a.d ? yr[i] : make_uint4(0, 0, 0, 0);
       }
     }
     if (id < QT) {
