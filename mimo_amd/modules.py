@@ -40,6 +40,8 @@ class Ctx:
         self.t_emb = None       # half [b, C0]: precomputed sinusoidal timestep embedding (UNetBase.timestep_table) or None
         self.temb = None        # fp32 [b, sum(Cout)]: every ResBlock's time_emb_proj(silu(emb)) at once
         self.attn2 = None       # fp32 [b, sum(C)]: every block's collapsed cross-attention output
+        self.tokens = None      # half [b, L, cross_dim]: encoder states of several tokens (then attn2 is None), and
+        self.tokens_mask = None  # uint8 [b, L] or None: which of them count
         self.band_rows = None   # VAE tiled decode: images taller than this run GroupNorm-apply + conv per row band (exact halos)
         self.stop_after = None  # write mode: block after whose bank write the rest of the graph is dead
         self.bank_rows = None   # write mode: batch rows to bank (None = all)
@@ -136,6 +138,7 @@ class HipModule(nn.Module):
             m.__dict__.pop("_pk", None)
             m.__dict__.pop("_pk_split", None)
             m.__dict__.pop("_pk_split_parts", None)
+            m.__dict__.pop("_pk_tokens", None)
 
     def _apply(self, fn, *a, **k):
         self.invalidate()
@@ -437,6 +440,36 @@ class SpatialTransformerBlock(HipModule):
         wo, wv = a2.to_out[0].weight.detach().double().cpu(), a2.to_v.weight.detach().double().cpu()
         return (wo @ wv).float().to(a2.to_out[0].weight.device), _f32(a2.to_out[0].bias)
 
+    def packed_tokens(self, dtype):
+        """attn2's projections for encoder states of several tokens, packed on first use (a model that only ever sees one token
+        never holds them)."""
+        cache = self.__dict__.setdefault("_pk_tokens", {})
+        key = (dtype, self._dev())
+        if key not in cache:
+            if cache:
+                _PACK_EPOCH[0] += 1
+            cache.clear()
+            a2, h = self.attn2, lambda w: w.detach().to(dtype).contiguous()
+            with torch.no_grad():
+                cache[key] = dict(q=h(a2.to_q.weight), kv=h(torch.cat([a2.to_k.weight, a2.to_v.weight], 0)),
+                                  o_w=h(a2.to_out[0].weight), o_b=_f32(a2.to_out[0].bias),
+                                  n2w=_f32(self.norm2.weight), n2b=_f32(self.norm2.bias))
+        return cache[key]
+
+    def _attn2_tokens(self, ctx, o, t, n_img, N):
+        """to_out(attn1) + t, then norm2 and the cross attention to ctx.tokens with its output projection: the fp32 stream and
+        norm3 of it.  The b encoder rows are read in place by the F images of each (src/models/transformer_3d.py:107-110 repeats
+        them F times)."""
+        p, p2, C = self.packed(ctx.dtype), self.packed_tokens(ctx.dtype), self.dim
+        b, n_tok, width = ctx.tokens.shape
+        y, n2 = ops.gemm(o, p["o_w"], bias=p["o_b"], residual=t, out_f32=True,
+                         ln=dict(gamma=p2["n2w"], beta=p2["n2b"], eps=self.norm2.eps, fold=False))
+        q = ops.gemm(n2, p2["q"]).view(n_img, N, C)
+        kv = ops.gemm(ctx.tokens.view(b * n_tok, width), p2["kv"]).view(b, n_tok, 2 * C)
+        o2 = ops.cross_attention(q, kv[..., :C], kv[..., C:], self.heads, mask=ctx.tokens_mask)
+        return ops.gemm(o2.view(-1, C), p2["o_w"], bias=p2["o_b"], residual=y, out_f32=True,
+                        ln=dict(gamma=p["n3w"], beta=p["n3b"], eps=self.norm3.eps, fold=True))
+
     def ln1(self, dtype):
         """norm1 as the `ln=` argument of the GEMM that produces this block's input (fused into its epilogue at C = 320,
         folded into the QKV projection at C >= 640 — except in write mode, which banks the normalised tensor itself)."""
@@ -475,6 +508,9 @@ class SpatialTransformerBlock(HipModule):
                               seg2_first_batch=first, q_prescaled=True)
         else:
             o = ops.attention(q, k, v, self.heads, q_prescaled=True)
+        if ctx.tokens is not None:
+            y, n3 = self._attn2_tokens(ctx, o.view(-1, C), t, n_img, N)
+            return _ff_proj_run(ctx, p, y, n3, proj, x, N) if proj is not None else _ff_run(ctx, p, y, n3, out_f32)
         s, e = self.attn2_slice
         if proj is not None:
             out = _block_tail_run(ctx, p, o.view(-1, C), t, proj, x, ("o_b", "n3w", "n3b"), self.norm3.eps,

@@ -223,6 +223,8 @@ class UNetBase(HipModule):
         len(timesteps) * b rows instead of three M = 2 launches per forward) and the 16 collapsed cross-attentions (one
         GEMM per clip: they do not depend on the step).  Returns (temb fp32 [S, b, sum(Cout)], attn2 fp32 [b, sum(C)]);
         run_tokens(temb=..., attn2=...) then starts at conv_in.  The arithmetic per row is that of _time_and_cross."""
+        if _several_tokens(ehs):
+            raise ValueError("clip_tables: one token per row (cross attention to several depends on the image, not on the clip alone)")
         if self.precision == "split" or (ops.EDGE_SPLIT & 2):
             from . import precise
             return precise.clip_tables(self, timesteps, ehs, b)
@@ -255,13 +257,31 @@ class UNetBase(HipModule):
         e1 = ops.gemm(t_emb, p["t1_w"], bias=p["t1_b"], silu=True)
         emb = ops.gemm(e1, p["t2_w"], bias=p["t2_b"], silu=True)  # silu(emb): every consumer applies the nonlinearity first
         ctx.temb = ops.gemm(emb, p["temb_w"], bias=p["temb_b"], out_f32=True)
+        if ctx.tokens is not None:
+            return
         e = ehs.reshape(ctx.b, -1).to(device=dev, dtype=ctx.dtype).contiguous()
         ctx.attn2 = ops.gemm(e, p["a2_w"], bias=p["a2_b"], out_f32=True)
 
-    def run_tokens(self, x_tok, timestep, ehs, b, F, pose_tok=None, ctx=None, t_emb=None, temb=None, attn2=None):
-        """x_tok: half [b*F, h, w, Cin_pad8]; ehs: [b, 1, 768]; pose_tok: [b*F, h, w, C0] (fp32|half) or None.
+    def _tokens(self, ctx, ehs, mask):
+        """Encoder states of several tokens, or of any number with a mask: every block's cross attention runs on them
+        (one unmasked token collapses to a vector per image instead, SpatialTransformerBlock.attn2_matrix)."""
+        if mask is None and not _several_tokens(ehs):
+            return
+        if ehs.dim() != 3 or ehs.shape[0] != ctx.b or ehs.shape[1] < 1 or ehs.shape[2] != self.cross_dim:
+            raise ValueError(f"encoder_hidden_states {tuple(ehs.shape)}: [{ctx.b}, tokens, {self.cross_dim}]")
+        if mask is not None:
+            if mask.shape != ehs.shape[:2] or mask.dtype not in (torch.bool, torch.uint8, torch.int32, torch.int64):
+                raise ValueError(f"encoder_attention_mask {tuple(mask.shape)} {mask.dtype}: bool or 0 / 1 {tuple(ehs.shape[:2])}, nonzero = attend")
+            ctx.tokens_mask = (mask != 0).to(device=self.device, dtype=torch.uint8).contiguous()
+        ctx.tokens = ehs.to(device=self.device, dtype=ctx.dtype).contiguous()
+
+    def run_tokens(self, x_tok, timestep, ehs, b, F, pose_tok=None, ctx=None, t_emb=None, temb=None, attn2=None, ehs_mask=None):
+        """x_tok: half [b*F, h, w, Cin_pad8]; ehs: [b, L, 768] (ehs_mask: [b, L] or None; with L = 1 and no mask the cross
+        attentions collapse); pose_tok: [b*F, h, w, C0] (fp32|half) or None.
         Returns fp32 tokens [b*F, h, w, Cout_pad4] (or the last hidden state when there is no output head).
         precision "split": x_tok may be fp32 (then nothing of the input is rounded); see mimo_amd.precise."""
+        if (attn2 is not None or self.precision == "split") and (ehs_mask is not None or _several_tokens(ehs)):
+            raise ValueError("several or masked encoder tokens: precision \"half\", without the tables of clip_tables()")
         if self.precision == "split":
             from . import precise
             return precise.run_tokens(self, x_tok, timestep, ehs, b, F, pose_tok, ctx, temb, attn2)
@@ -272,6 +292,7 @@ class UNetBase(HipModule):
         if temb is not None and attn2 is not None:
             assert temb.shape[0] == b and attn2.shape[0] == b and temb.stride(1) == 1 and attn2.stride(1) == 1
             ctx.temb, ctx.attn2 = temb, attn2
+        self._tokens(ctx, ehs, ehs_mask)
         self._time_and_cross(ctx, p, timestep, ehs)
         n, H, W, _ = x_tok.shape
         up = 2 ** self.num_upsamplers
@@ -332,8 +353,10 @@ class UNet3DConditionModel(UNetBase):
 
     def forward(self, sample, timestep, encoder_hidden_states, class_labels=None, pose_cond_fea=None,
                 attention_mask=None, down_block_additional_residuals=None, mid_block_additional_residual=None,
-                return_dict=True):
-        """sample [b,8,f,h,w], pose_cond_fea [b,320,f,h,w] -> (sample [b,4,f,h,w],) like the reference."""
+                return_dict=True, encoder_attention_mask=None):
+        """sample [b,8,f,h,w], pose_cond_fea [b,320,f,h,w] -> (sample [b,4,f,h,w],) like the reference.
+        encoder_hidden_states [b, L, cross_attention_dim], any L; encoder_attention_mask: bool or 0 / 1 [b, L], nonzero = attend
+        (a row that attends to nothing adds only the output projection's bias)."""
         b, c, f, h, w = sample.shape
         dt = self.compute_dtype
         if self.precision == "split" or (ops.EDGE_SPLIT & 4):   # fp32 tokens: a layout copy, nothing is rounded
@@ -343,7 +366,7 @@ class UNet3DConditionModel(UNetBase):
         else:
             x = ops.ncfhw_to_tokens(sample.contiguous(), dt, cpad=8)
             pose = None if pose_cond_fea is None else ops.ncfhw_to_tokens(pose_cond_fea.contiguous(), dt)
-        y = self.run_tokens(x, timestep, encoder_hidden_states, b, f, pose)
+        y = self.run_tokens(x, timestep, encoder_hidden_states, b, f, pose, ehs_mask=encoder_attention_mask)
         out = ops.tokens_to_ncfhw(y, b, self.out_channels, f, h, w).to(sample.dtype)
         return _Out(sample=out) if return_dict else (out,)
 
@@ -392,8 +415,10 @@ class UNet2DConditionModel(UNetBase):
         self.config = _Config(sample_size=sample_size, in_channels=in_channels, block_out_channels=list(block_out_channels),
                               cross_attention_dim=cross_attention_dim)
 
-    def forward(self, sample, timestep, encoder_hidden_states, return_dict=True, stop_after=None, bank_rows=None, **unused):
-        """sample [b,4,h,w] -> hidden state [b,320,h,w] (the reference discards it; the banks are the product)."""
+    def forward(self, sample, timestep, encoder_hidden_states, return_dict=True, stop_after=None, bank_rows=None,
+                encoder_attention_mask=None, **unused):
+        """sample [b,4,h,w] -> hidden state [b,320,h,w] (the reference discards it; the banks are the product).
+        encoder_hidden_states, encoder_attention_mask: as UNet3DConditionModel.forward."""
         b, c, h, w = sample.shape
         dt = self.compute_dtype
         if self.precision == "split":
@@ -404,7 +429,7 @@ class UNet2DConditionModel(UNetBase):
         ctx = Ctx(dt, b, 1)
         ctx.stop_after, ctx.bank_rows = stop_after, bank_rows
         try:
-            y = self.run_tokens(x, timestep, encoder_hidden_states, b, 1, None, ctx)
+            y = self.run_tokens(x, timestep, encoder_hidden_states, b, 1, None, ctx, ehs_mask=encoder_attention_mask)
         except EarlyExit:
             return None
         out = y.permute(0, 3, 1, 2).contiguous().to(sample.dtype)
@@ -422,6 +447,10 @@ class UNet2DConditionModel(UNetBase):
         sd = {k: v for k, v in _load_weights(path).items() if not k.startswith(("conv_out.", "conv_norm_out."))}
         model.load_state_dict(sd, strict=False)
         return model
+
+
+def _several_tokens(ehs):
+    return ehs is not None and ehs.dim() == 3 and ehs.shape[1] > 1
 
 
 class _Out:
