@@ -142,9 +142,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[u][r]);
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
       const bool move = mt > m_ref + a.lag;  // (m_ref = -inf: any finite maximum)
-      if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
-        const float alpha = move ? fast_exp2((m_ref - mt) * a.c) : 1.f;  // m_ref = -inf: 0
-        m_ref = move ? mt : m_ref;
+      const float old = m_ref;
+      m_ref = move ? mt : old;
+      if (__builtin_amdgcn_ballot_w64(move && old != -INFINITY) != 0ull) {  // (nothing is summed yet against -inf)
+        const float alpha = move && old != -INFINITY ? fast_exp2((old - mt) * a.c) : 1.f;
         sum *= alpha;
 #pragma unroll
         for (int i = 0; i < OT; ++i)

@@ -120,8 +120,10 @@ __device__ __forceinline__ void load_row(uint4 (&f)[KS], const uint16_t* p, int 
   }
 }
 
-// lanes per row of 16-byte chunks: a power of two, so that a thread keeps its column and walks rows at a fixed distance
-constexpr int lanes_of(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 8 : ks <= 8 ? 16 : 32; }
+// lanes per row of 16-byte chunks: a power of two, so that a thread keeps its columns and walks rows at a fixed distance; at most
+// eight (a line of 128 bytes), which take wider rows in several chunks each: a row's address is made once for all of them
+constexpr int lanes_of(int ks) { return ks <= 2 ? 4 : 8; }
+constexpr int chunks_of(int ks) { return (2 * ks + lanes_of(ks) - 1) / lanes_of(ks); }
 
 // Key and value rows [key0, key0 + N) of (e, g) on their way into row-major LDS tiles of pitch 16 KS + 8 halfs (an odd number of
 // 16-byte units: a 16-lane group of b128 row reads covers all banks).  issue() requests the rows, commit() writes them: between
@@ -130,8 +132,8 @@ constexpr int lanes_of(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 8 : ks <= 8 ? 16
 // ones: V's channel d, which pads the last 32-channel tile, is 1 — the product with P then also leaves the sum of P in that row.
 template <int KS, int THREADS, int N>
 struct Stager {
-  static constexpr int P = 16 * KS + 8, LPR = lanes_of(KS), RP = THREADS / LPR, NC = (N + RP - 1) / RP;
-  uint4 kr[NC], vr[NC];
+  static constexpr int P = 16 * KS + 8, LPR = lanes_of(KS), CH = chunks_of(KS), RP = THREADS / LPR, NC = (N + RP - 1) / RP;
+  uint4 kr[NC][CH], vr[NC][CH];
   uint8_t keep;  // the mask's byte of key key0 + lane
   int left;      // keys of this piece
   const uint16_t *kb, *vb;
@@ -139,18 +141,21 @@ struct Stager {
     kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
     vb = a.v + (int64_t)e * a.svb + (int64_t)g * a.d;
   }
-  // (one branch around all requests, no select between them: keys behind the last one repeat it)
+  // (no select between the requests: keys behind the last one repeat it)
   __device__ __forceinline__ void issue(const Args& a, int e, int len, int key0, int tid) {
     asm volatile("" : "+v"(tid));  // addresses are made anew for every piece: kept over the products they would cost registers
     const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
     left = len - key0;  // > 0
-    if (cc < a.d) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int key = key0 + min(row0 + i * RP, left - 1);
-        kr[i] = *reinterpret_cast<const uint4*>(kb + (int64_t)key * a.skr + cc);
-        vr[i] = *reinterpret_cast<const uint4*>(vb + (int64_t)key * a.svr + cc);
-      }
+    for (int i = 0; i < NC; ++i) {
+      const int key = key0 + min(row0 + i * RP, left - 1);
+      const uint16_t *kp = kb + (int64_t)key * a.skr + cc, *vp = vb + (int64_t)key * a.svr + cc;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (cc + 8 * LPR * c < a.d) {
+          kr[i][c] = *reinterpret_cast<const uint4*>(kp + 8 * LPR * c);
+          vr[i][c] = *reinterpret_cast<const uint4*>(vp + 8 * LPR * c);
+        }
     }
     static_assert(N <= 64, "a lane per key of the mask");
     keep = 1;
@@ -165,12 +170,17 @@ struct Stager {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int row = row0 + i * RP;
-      if (cc < 16 * KS && (N % RP == 0 || row < N)) {
-        const bool ok = ((live >> (row & 63)) & 1) && cc < a.d;
-        uint4 x = ok ? kr[i] : make_uint4(0, 0, 0, 0), y = ok ? vr[i] : make_uint4(0, 0, 0, 0);
-        if (ones && cc == a.d) y.x = HT<DT>::from_f(1.f);
-        *reinterpret_cast<uint4*>(ks + row * P + cc) = x;
-        *reinterpret_cast<uint4*>(vs + row * P + cc) = y;
+      const bool alive = (live >> (row & 63)) & 1;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = cc + 8 * LPR * c;
+        if (col < 16 * KS && (N % RP == 0 || row < N)) {
+          const bool ok = alive && col < a.d;
+          uint4 x = ok ? kr[i][c] : make_uint4(0, 0, 0, 0), y = ok ? vr[i][c] : make_uint4(0, 0, 0, 0);
+          if (ones && col == a.d) y.x = HT<DT>::from_f(1.f);
+          *reinterpret_cast<uint4*>(ks + row * P + col) = x;
+          *reinterpret_cast<uint4*>(vs + row * P + col) = y;
+        }
       }
     }
     if (tid < N) {

@@ -21,7 +21,7 @@ constexpr int stream_keys(int ks) { return ks >= 6 ? 32 : 64; }  // keys per str
 
 // RESIDENT: NW = 4 or 8 waves per block as in the forward; streamed: 4
 template <int DT, int KS, bool RESIDENT, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 1) void xattn_dq_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_kernel(const Args a) {
   constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW, CH = stream_keys(KS);
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -157,24 +157,31 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : KS <= 3 ? 3 : KS <= 6 ? 2 : 
 }
 
 // query rows per LDS buffer: what a thread can hold on its way
-constexpr int qt_rows(int ks, int nw) { return ks <= 4 && nw > 1 ? 64 : 32; }
+constexpr int qt_rows(int ks, int nw) { return ks <= 4 && nw > 2 ? 64 : 32; }
 constexpr int dkv_lds(int ks, int nw) { return 2 * (2 * qt_rows(ks, nw) * (16 * ks + 8) * 2 + 2 * qt_rows(ks, nw) * 4 + 64); }
+// waves that share a key tile: dK and dV of a wide head do not fit one wave's registers beside its K and V, so two waves form the
+// same P and dS and each takes half of the channels
+constexpr int dkv_share(int ks) { return ks >= 8 ? 2 : 1; }
+constexpr int dkv_occ(int ks) { return ks <= 3 ? 3 : 2; }  // waves per SIMD
 
+// NW: key tiles of a block
 template <int DT, int KS, int NW>
-__global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) void xattn_dkv_kernel(const Args a) {
-  constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW, QT = qt_rows(KS, NW);
+__global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dkv_kernel(const Args a) {
+  constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, SHARE = dkv_share(KS), OW = (OT + SHARE - 1) / SHARE, THREADS = 64 * NW * SHARE,
+                QT = qt_rows(KS, NW);
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int BUF = 2 * QT * P * 2 + 2 * QT * 4 + 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h2 = lane >> 5, li = lane & 31;
+  const int part = SHARE == 1 ? 0 : wave & 1, o0 = part * OW;  // this wave's channel tiles: o0 .. o0 + OW (less one if OT is odd)
   // blocks of one XCD: the key heads of the same rows, then the key groups
   const unsigned L = xcd_remap(blockIdx.x, gridDim.x);
   const int g = (int)(L % (unsigned)a.kvh);
   const int e = (int)(L / (unsigned)a.kvh) % a.Be, kt = (int)(L / (unsigned)a.kvh) / a.Be;
   const int len = valid_len(a, e);
-  const int key = (kt * NW + wave) * 32 + li;
+  const int key0 = (kt * NW + wave / SHARE) * 32, key = key0 + li;
   const bool valid = key_valid(a, e, len, min(key, a.Nk - 1)) && key < a.Nk;
-  const bool any = (kt * NW + wave) * 32 < len;  // (wave-uniform)
+  const bool any = key0 < len;  // (wave-uniform)
   // flat rows of this part, in whole QT tiles
   const int T = (a.R + QT - 1) / QT, per = (T + a.nsplit - 1) / a.nsplit;
   const int t_lo = min(T, (int)blockIdx.y * per), t_hi = kt * NW * 32 < len ? min(T, t_lo + per) : t_lo;
@@ -193,32 +200,35 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
       }
     }
   }
-  f32x16 dk[OT], dv[OT];
+  f32x16 dk[OW], dv[OW];
 #pragma unroll
-  for (int i = 0; i < OT; ++i)
+  for (int i = 0; i < OW; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
   // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to buffer b (commit).  Rows
   // behind the last one repeat it with lse = inf: P = 0.  Channels behind the last one are zeros.
-  constexpr int LPR = lanes_of(KS), RP = THREADS / LPR, NC = (QT + RP - 1) / RP;
-  uint4 xr[NC], yr[NC];
+  constexpr int LPR = lanes_of(KS), CH = chunks_of(KS), RP = THREADS / LPR, NC = (QT + RP - 1) / RP;
+  uint4 xr[NC][CH], yr[NC][CH];
   float lr, dr;
   int on_way = 0;
   auto issue = [&](int t) {
     int id = tid;
     asm volatile("" : "+v"(id));  // addresses are made anew for every tile
     const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
-    if (cc < a.d) {  // (one branch around all requests)
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int f = min(t * QT + min(row0 + i * RP, QT - 1), a.R - 1);
-        int img, qi, hh;
-        flat_row(a, f, img, qi, hh);
-        const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
-        xr[i] = *reinterpret_cast<const uint4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
-        yr[i] = *reinterpret_cast<const uint4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
-      }
+    for (int i = 0; i < NC; ++i) {
+      const int f = min(t * QT + min(row0 + i * RP, QT - 1), a.R - 1);
+      int img, qi, hh;
+      flat_row(a, f, img, qi, hh);
+      const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
+      const uint16_t *qp = a.q + bb * a.sqb + (int64_t)qi * a.sqr + col, *dp = a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (cc + 8 * LPR * c < a.d) {
+          xr[i][c] = *reinterpret_cast<const uint4*>(qp + 8 * LPR * c);
+          yr[i][c] = *reinterpret_cast<const uint4*>(dp + 8 * LPR * c);
+        }
     }
     static_assert(QT <= THREADS, "a thread per row");
     const int f = min(t * QT + (id & (QT - 1)), a.R - 1);
@@ -238,9 +248,13 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int row = row0 + i * RP;
-      if (cc < 16 * KS && (QT % RP == 0 || row < QT)) {
-        *reinterpret_cast<uint4*>(qs + row * P + cc) = cc < a.d ? xr[i] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(qs + QT * P + row * P + cc) = cc < a.d ? yr[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = cc + 8 * LPR * c;
+        if (col < 16 * KS && (QT % RP == 0 || row < QT)) {
+          *reinterpret_cast<uint4*>(qs + row * P + col) = col < a.d ? xr[i][c] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(qs + QT * P + row * P + col) = col < a.d ? yr[i][c] : make_uint4(0, 0, 0, 0);
+        }
       }
     }
     if (id < QT) {
@@ -285,9 +299,10 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
       for (int u = 0; u < 2; ++u) {
         const uint4 pf = pack_k<DT>(s, u), sf = pack_k<DT>(dp, u);
 #pragma unroll
-        for (int i = 0; i < OT; ++i) {
-          dv[i] = HT<DT>::mfma32(read_tr(ds, P, q0 + 16 * u, 32 * i, lane), pf, dv[i]);
-          dk[i] = HT<DT>::mfma32(read_tr(qs, P, q0 + 16 * u, 32 * i, lane), sf, dk[i]);
+        for (int i = 0; i < OW; ++i) {
+          if (OT % SHARE && i == OW - 1 && part) continue;
+          dv[i] = HT<DT>::mfma32(read_tr(ds, P, q0 + 16 * u, 32 * (o0 + i), lane), pf, dv[i]);
+          dk[i] = HT<DT>::mfma32(read_tr(qs, P, q0 + 16 * u, 32 * (o0 + i), lane), sf, dk[i]);
         }
       }
     }
@@ -300,10 +315,10 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
   if (key >= a.Nk) return;
   const int64_t C = (int64_t)a.kvh * a.d, at = ((int64_t)e * a.Nk + key) * C + (int64_t)g * a.d, plane = (int64_t)a.Be * a.Nk * C;
 #pragma unroll
-  for (int i = 0; i < OT; ++i)
+  for (int i = 0; i < OW; ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int d0 = 32 * i + 8 * c + 4 * h2;
+      const int d0 = 32 * (o0 + i) + 8 * c + 4 * h2;
       if (d0 >= a.d) continue;
       f32x4 x, y;  // a key that the mask drops has no gradient (its columns hold what zeros gave)
 #pragma unroll
@@ -322,17 +337,24 @@ __global__ __launch_bounds__(64 * NW, KS <= 4 || (KS == 5 && NW > 2) ? 2 : 1) vo
     }
 }
 
-// dk / dv = the sum of the parts, in order
+// dk / dv = the sum of the parts: eight runs of them side by side (a block takes 32 pieces of four numbers), then the runs in order
 template <int DT>
 __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(const float* ws, uint16_t* dk, uint16_t* dv, int64_t plane, int parts) {
-  const int64_t n4 = plane >> 2;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n4; i += (int64_t)gridDim.x * 256) {
-    const int64_t at = i < n4 ? i : i - n4;
-    const float* w = ws + (i < n4 ? 0 : plane) + 4 * at;
-    f32x4 s = *reinterpret_cast<const f32x4*>(w);
-    for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(w + (int64_t)p * 2 * plane);
-    *reinterpret_cast<uint2*>((i < n4 ? dk : dv) + 4 * at) = make_uint2(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]));
+  __shared__ f32x4 sums[8][32];
+  const int64_t n4 = plane >> 2, i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+  const int run = threadIdx.x >> 5, per = (parts + 7) / 8, p0 = run * per, p1 = min(parts, p0 + per);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (i < 2 * n4) {
+    const float* w = ws + 4 * i;
+#pragma unroll 4
+    for (int p = p0; p < p1; ++p) s += *reinterpret_cast<const f32x4*>(w + (int64_t)p * 2 * plane);
   }
+  sums[run][threadIdx.x & 31] = s;
+  lds_barrier();
+  if (run || i >= 2 * n4) return;
+#pragma unroll
+  for (int r = 1; r < 8; ++r) s += sums[r][threadIdx.x];
+  *reinterpret_cast<uint2*>(i < n4 ? dk + 4 * i : dv + 4 * (i - n4)) = make_uint2(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]));
 }
 
 struct Plan {
@@ -340,10 +362,11 @@ struct Plan {
   int dq_nw, lds, nb;      // dq
   int nw, groups, nsplit;  // dk / dv
 };
-// (the widest heads leave one or two waves no registers for the rows on their way)
-constexpr int min_waves(int ks) { return ks >= 8 ? 3 : 1; }
-// dq: as the forward.  dk / dv: the number of waves per block (up to four) that leaves the fewest without a key tile; the rows are
-// cut into parts until the chip has as many waves as fit, a part keeping at least four row tiles.
+// key tiles per block: heads whose tiles take two waves have 2; from 80 channels on one wave alone could not hold the rows on their way
+constexpr int least_tiles(int ks) { return ks >= 5 ? 2 : 1; }
+constexpr int most_tiles(int ks) { return dkv_share(ks) == 2 ? 2 : 4; }
+// dq: as the forward.  dk / dv: the number of key tiles per block (up to four) that leaves the fewest waves without one; the rows are
+// cut into as many parts as fill the chip once with resident blocks, a part keeping at least four row tiles.
 Plan plan(const Args& a) {
   Plan p{};
   const int ks = k_steps(a.d), cus = cu_count(), eg = a.Be * a.kvh;
@@ -355,13 +378,13 @@ Plan plan(const Args& a) {
   p.nb = p.resident ? (per_cu * cus + eg - 1) / eg : most;
   if (p.nb > most) p.nb = most;
   const int tiles = a.Nk > 0 ? (a.Nk + 31) / 32 : 1;  // (without keys there is no dk / dv launch)
-  p.nw = 4;
-  for (int w = 3; w >= min_waves(ks); --w)
+  p.nw = most_tiles(ks);
+  for (int w = p.nw - 1; w >= least_tiles(ks); --w)
     if ((tiles + w - 1) / w * w < (tiles + p.nw - 1) / p.nw * p.nw) p.nw = w;
   p.groups = (tiles + p.nw - 1) / p.nw;
   const int T = (a.R + qt_rows(ks, p.nw) - 1) / qt_rows(ks, p.nw);
-  const int64_t blocks = (int64_t)eg * p.groups, waves = (int64_t)(ks <= 5 ? 8 : 4) * cus;
-  int64_t n = (waves / p.nw + blocks - 1) / blocks;
+  const int by_waves = 4 * dkv_occ(ks) / (p.nw * dkv_share(ks)), by_lds = 160000 / dkv_lds(ks, p.nw);
+  int64_t n = (int64_t)(by_waves < by_lds ? by_waves : by_lds) * cus / ((int64_t)eg * p.groups);
   if (n > T / 4) n = T / 4;
   if (n > 256) n = 256;
   p.nsplit = n < 1 ? 1 : (int)n;
@@ -386,16 +409,20 @@ int launch(Args& a, const Plan& p, hipStream_t st) {
   if (a.Nk == 0) return MIMO_OK;
   a.nb = p.groups; a.nsplit = p.nsplit;
   const dim3 grid(eg * (unsigned)p.groups, (unsigned)p.nsplit);
-  if constexpr (min_waves(KS) == 1) {
-    if (p.nw == 1) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 1>), grid, dim3(64), dkv_lds(KS, 1), st, a);
-    if (p.nw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(128), dkv_lds(KS, 2), st, a);
+  const int shm = dkv_lds(KS, p.nw);
+  if constexpr (dkv_share(KS) == 2) {
+    hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(256), shm, st, a);
+  } else {
+    if constexpr (least_tiles(KS) == 1)
+      if (p.nw == 1) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 1>), grid, dim3(64), shm, st, a);
+    if (p.nw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(128), shm, st, a);
+    if (p.nw == 3) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 3>), grid, dim3(192), shm, st, a);
+    if (p.nw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 4>), grid, dim3(256), shm, st, a);
   }
-  if (p.nw == 3) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 3>), grid, dim3(192), dkv_lds(KS, 3), st, a);
-  if (p.nw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 4>), grid, dim3(256), dkv_lds(KS, 4), st, a);
   MIMO_LAUNCH_CHECK();
   if (p.nsplit > 1) {
-    const int64_t plane = (int64_t)a.Be * a.Nk * a.kvh * a.d, nwg = (plane / 2 + 255) / 256;
-    hipLaunchKernelGGL((xattn_dkv_join_kernel<DT>), dim3((unsigned)(nwg > 2048 ? 2048 : nwg)), dim3(256), 0, st, a.ws, a.dk, a.dv, plane,
+    const int64_t plane = (int64_t)a.Be * a.Nk * a.kvh * a.d;
+    hipLaunchKernelGGL((xattn_dkv_join_kernel<DT>), dim3((unsigned)((plane / 2 + 31) / 32)), dim3(256), 0, st, a.ws, a.dk, a.dv, plane,
                        p.nsplit);
     MIMO_LAUNCH_CHECK();
   }
