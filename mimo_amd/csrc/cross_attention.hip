@@ -26,7 +26,7 @@ int fill(Args& a, const mimo_cross_attention_params* p) {
       p->heads >= 0x10000)
     return MIMO_EINVAL;
   a.R = (int)R;
-  a.by_hg = fast_div((uint32_t)a.hg); a.by_nq = fast_div((uint32_t)a.Nq);
+  a.by_hg = fast_div((uint32_t)a.hg); a.by_nq = fast_div((uint32_t)a.Nq); a.by_dc = fast_div((uint32_t)a.d / 8);
   a.scale = p->scale; a.c = p->scale * LOG2E;
   a.sqb = p->q_batch; a.sqr = p->q_row; a.skb = p->k_batch; a.skr = p->k_row; a.svb = p->v_batch; a.svr = p->v_row;
   a.smb = p->mask_row;
@@ -184,6 +184,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
         stager.issue(a, e, k_hi, k_lo, tid);
         if (round > 0) lds_barrier();  // the previous round's last chunk is read
         stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), ones, tid);
+        settle<KS>(qf);
         if (chunks > 1) stager.issue(a, e, k_hi, k_lo + CHK, tid);
       }
       for (int i = 0; i < chunks; ++i) {

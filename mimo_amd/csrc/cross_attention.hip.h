@@ -23,7 +23,7 @@ struct Args {
   const uint8_t* mask;           // [Be, Nk] or null
   int64_t sqb, sqr, skb, skr, svb, svr, sob, sor, sdb, sdr, smb;  // element strides: batch, row (o / dout: sob.., sdb..)
   int Be, G, Nq, Nk, kvh, hg, d, R;
-  FastDiv by_hg, by_nq;
+  FastDiv by_hg, by_nq, by_dc;   // query heads per key head, tokens, 16-byte chunks of a head
   float c;                       // scale * log2(e): scores leave the matrix unit unscaled
   float scale, lag;
   int nb;                        // blocks per (e, g)
@@ -118,6 +118,14 @@ __device__ __forceinline__ void load_row(uint4 (&f)[KS], const uint16_t* p, int 
     const int kk = 16 * s + 8 * h2;
     f[s] = *reinterpret_cast<const uint4*>(p + (kk < d ? kk : 0));
   }
+}
+
+// waits for requested fragments HERE.  Used first inside a loop that keeps other requests on their way, they would be waited for
+// in every round of it, and the younger requests with them.
+template <int KS>
+__device__ __forceinline__ void settle(uint4 (&f)[KS]) {
+#pragma unroll
+  for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(f[s].x), "+v"(f[s].y), "+v"(f[s].z), "+v"(f[s].w));
 }
 
 // lanes per row of 16-byte chunks: a power of two, so that a thread keeps its columns and walks rows at a fixed distance; at most

@@ -17,6 +17,11 @@
 namespace mimo_xattn {
 namespace {
 
+template <int V>
+struct IC {
+  static constexpr int value = V;
+};
+
 constexpr int stream_keys(int ks) { return ks >= 6 ? 32 : 64; }  // keys per streamed buffer of dq
 
 // RESIDENT: NW = 4 or 8 waves per block as in the forward; streamed: 4
@@ -135,6 +140,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
         stager.issue(a, e, len, 0, tid);
         if (round > 0) lds_barrier();
         stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), false, tid);
+        settle<KS>(qf);
+        settle<KS>(df);
         if (chunks > 1) stager.issue(a, e, len, CH, tid);
       }
       for (int i = 0; i < chunks; ++i) {
@@ -158,11 +165,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
 
 // query rows per LDS buffer: what a thread can hold on its way
 constexpr int qt_rows(int ks, int nw) { return ks <= 4 && nw > 2 ? 64 : 32; }
-constexpr int dkv_lds(int ks, int nw) { return 2 * (2 * qt_rows(ks, nw) * (16 * ks + 8) * 2 + 2 * qt_rows(ks, nw) * 4 + 64); }
+constexpr int dkv_buffers(int ks, int nw) { return 2 * (2 * qt_rows(ks, nw) * (16 * ks + 8) * 2 + 2 * qt_rows(ks, nw) * 4 + 64); }
 // waves that share a key tile: dK and dV of a wide head do not fit one wave's registers beside its K and V, so two waves form the
 // same P and dS and each takes half of the channels
+// (and V's fragments are in LDS)
 constexpr int dkv_share(int ks) { return ks >= 8 ? 2 : 1; }
-constexpr int dkv_occ(int ks) { return ks <= 3 ? 3 : 2; }  // waves per SIMD
+constexpr int dkv_lds(int ks, int nw) { return dkv_buffers(ks, nw) + (dkv_share(ks) == 2 ? nw * ks * 1024 : 0); }
+constexpr int dkv_occ(int ks) { return ks <= 2 ? 3 : 2; }    // waves per SIMD
+constexpr int dkv_depth(int ks) { return ks <= 4 || ks >= 8 ? 2 : 1; }  // row tiles on their way in registers, where there are some to spare
 
 // NW: key tiles of a block
 template <int DT, int KS, int NW>
@@ -186,18 +196,22 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
   const int T = (a.R + QT - 1) / QT, per = (T + a.nsplit - 1) / a.nsplit;
   const int t_lo = min(T, (int)blockIdx.y * per), t_hi = kt * NW * 32 < len ? min(T, t_lo + per) : t_lo;
 
-  uint4 kf[KS], vf[KS];
+  uint4 kf[KS], vf[SHARE == 1 ? KS : 1];
+  uint4* vl = reinterpret_cast<uint4*>(smem + dkv_buffers(KS, NW) + wave / SHARE * KS * 1024) + lane;  // SHARE == 2: [KS][64]
   {
     const uint16_t* kp = a.k + (int64_t)e * a.skb + (int64_t)(valid ? key : 0) * a.skr + (int64_t)g * a.d;
     const uint16_t* vp = a.v + (int64_t)e * a.svb + (int64_t)(valid ? key : 0) * a.svr + (int64_t)g * a.d;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int kk = 16 * s + 8 * h2;
-      kf[s] = vf[s] = make_uint4(0, 0, 0, 0);
+      uint4 x = make_uint4(0, 0, 0, 0), y = x;
       if (valid && kk < a.d) {
-        kf[s] = *reinterpret_cast<const uint4*>(kp + kk);
-        vf[s] = *reinterpret_cast<const uint4*>(vp + kk);
+        x = *reinterpret_cast<const uint4*>(kp + kk);
+        y = *reinterpret_cast<const uint4*>(vp + kk);
       }
+      kf[s] = x;
+      if (SHARE == 1) vf[SHARE == 1 ? s : 0] = y;
+      else if (part == 0) vl[64 * s] = y;
     }
   }
   f32x16 dk[OW], dv[OW];
@@ -206,68 +220,76 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
-  // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to buffer b (commit).  Rows
-  // behind the last one repeat it with lse = inf: P = 0.  Channels behind the last one are zeros.
-  constexpr int LPR = lanes_of(KS), CH = chunks_of(KS), RP = THREADS / LPR, NC = (QT + RP - 1) / RP;
-  uint4 xr[NC][CH], yr[NC][CH];
-  float lr, dr;
-  int on_way = 0;
-  auto issue = [&](int t) {
-    int id = tid;
-    asm volatile("" : "+v"(id));  // addresses are made anew for every tile
-    const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
+  // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to a buffer (commit).  Rows
+  // behind the last one repeat it with lse = inf: P = 0.  The 16-byte chunks of a tile are dealt to the threads one after another and
+  // the last threads repeat the last chunk: no request is behind a branch, so a wait for the oldest tile leaves the younger ones on
+  // their way.  The channels behind the last one are zeroed once.
+  constexpr int NC = (QT * 2 * KS + THREADS - 1) / THREADS, DEPTH = dkv_depth(KS);
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 xr[DEPTH][NC], yr[DEPTH][NC];
+  float lr[DEPTH], dr[DEPTH];
+  int place[NC];  // row << 8 | channel of this thread's chunks
+  {
+    const int dc = a.d >> 3;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int f = min(t * QT + min(row0 + i * RP, QT - 1), a.R - 1);
-      int img, qi, hh;
-      flat_row(a, f, img, qi, hh);
-      const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + cc;
-      const uint16_t *qp = a.q + bb * a.sqb + (int64_t)qi * a.sqr + col, *dp = a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col;
+      const int c = min(tid + i * THREADS, QT * dc - 1), row = (int)div_fast((uint32_t)c, a.by_dc);
+      place[i] = row << 8 | (c - row * dc) * 8;
+    }
+    for (int c = tid; c < 2 * 2 * QT * (2 * KS - dc); c += THREADS) {  // (usually none)
+      const int row = c / (2 * KS - dc), col = dc + c - row * (2 * KS - dc);  // rows of q, dO of buffer 0, then of buffer 1
+      *reinterpret_cast<uint4*>(smem + (row >= 2 * QT ? BUF - 2 * QT * P * 2 : 0) + row * P * 2 + col * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  auto issue = [&](int t, auto w_c) __attribute__((always_inline)) {
+    constexpr int w = decltype(w_c)::value;
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        if (cc + 8 * LPR * c < a.d) {
-          xr[i][c] = *reinterpret_cast<const uint4*>(qp + 8 * LPR * c);
-          yr[i][c] = *reinterpret_cast<const uint4*>(dp + 8 * LPR * c);
-        }
+    for (int i = 0; i < NC; ++i) {
+      int at = place[i], img, qi, hh;
+      asm volatile("" : "+v"(at));  // addresses are made anew for every tile: kept over the products they would cost registers
+      flat_row(a, min(t * QT + (at >> 8), a.R - 1), img, qi, hh);
+      const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + (at & 255);
+      xr[w][i] = *reinterpret_cast<const u32x4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
+      yr[w][i] = *reinterpret_cast<const u32x4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
     }
     static_assert(QT <= THREADS, "a thread per row");
-    const int f = min(t * QT + (id & (QT - 1)), a.R - 1);
     int img, qi, hh;
-    flat_row(a, f, img, qi, hh);
+    flat_row(a, min(t * QT + (tid & (QT - 1)), a.R - 1), img, qi, hh);
     const int64_t stat = (((int64_t)e * a.G + img) * a.kvh * a.hg + g * a.hg + hh) * a.Nq + qi;
-    lr = a.lse_in[stat];
-    dr = a.delta[stat];
-    on_way = t;
+    lr[w] = a.lse_in[stat];
+    dr[w] = a.delta[stat];
   };
-  auto commit = [&](int b) {
-    int id = tid;
-    asm volatile("" : "+v"(id));
-    const int row0 = id / LPR, cc = (id & (LPR - 1)) * 8;
+  auto commit = [&](int t, int b, auto w_c) __attribute__((always_inline)) {
+    constexpr int w = decltype(w_c)::value;
     uint16_t* qs = reinterpret_cast<uint16_t*>(smem + b * BUF);
     float* l2 = reinterpret_cast<float*>(smem + b * BUF + 2 * QT * P * 2 + 64);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int row = row0 + i * RP;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int col = cc + 8 * LPR * c;
-        if (col < 16 * KS && (QT % RP == 0 || row < QT)) {
-          *reinterpret_cast<uint4*>(qs + row * P + col) = col < a.d ? xr[i][c] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(qs + QT * P + row * P + col) = col < a.d ? yr[i][c] : make_uint4(0, 0, 0, 0);
-        }
-      }
+      int at = place[i];
+      asm volatile("" : "+v"(at));
+      uint16_t* to = qs + (at >> 8) * P + (at & 255);
+      *reinterpret_cast<u32x4*>(to) = xr[w][i];
+      *reinterpret_cast<u32x4*>(to + QT * P) = yr[w][i];
     }
-    if (id < QT) {
-      l2[id] = lr == -INFINITY || on_way * QT + id >= a.R ? INFINITY : lr * LOG2E;
-      l2[QT + id] = dr;
+    float l = lr[w];
+    asm volatile("" : "+v"(l));  // (not earlier: what is made of it would wait for the requests)
+    if (tid < QT) {
+      l2[tid] = l == -INFINITY || t * QT + tid >= a.R ? INFINITY : l * LOG2E;
+      l2[QT + tid] = dr[w];
     }
   };
+  // row tile t is in buffer (t - t_lo) & 1; t + 1 .. t + DEPTH are on their way, t + 1 + k in registers (t + k - t_lo) % DEPTH
   if (t_lo < t_hi) {
-    issue(t_lo);
-    commit(0);
-    if (t_lo + 1 < t_hi) issue(t_lo + 1);
+    issue(t_lo, IC<0>{});
+    commit(t_lo, 0, IC<0>{});
+    settle<KS>(kf);
+    if constexpr (SHARE == 1) settle<KS>(vf);
+    issue(min(t_lo + 1, t_hi - 1), IC<0>{});
+    __builtin_amdgcn_sched_barrier(0);  // in the order in which the loop takes them
+    if (DEPTH == 2) issue(min(t_lo + 2, t_hi - 1), IC<DEPTH - 1>{});
+    __builtin_amdgcn_sched_barrier(0);
   }
-  for (int t = t_lo; t < t_hi; ++t) {
+  auto body = [&](int t, auto w_c) __attribute__((always_inline)) {
     const int b = (t - t_lo) & 1;
     lds_barrier();
     const uint16_t* qs = reinterpret_cast<const uint16_t*>(smem + b * BUF);
@@ -282,7 +304,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         s = HT<DT>::mfma32(*reinterpret_cast<const uint4*>(qs + (q0 + li) * P + 16 * i + 8 * h2), kf[i], s);
-        dp = HT<DT>::mfma32(*reinterpret_cast<const uint4*>(ds + (q0 + li) * P + 16 * i + 8 * h2), vf[i], dp);
+        dp = HT<DT>::mfma32(*reinterpret_cast<const uint4*>(ds + (q0 + li) * P + 16 * i + 8 * h2), SHARE == 1 ? vf[SHARE == 1 ? i : 0] : vl[64 * i], dp);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -307,10 +329,13 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       }
     }
     }
-    if (t + 1 < t_hi) {
-      commit(b ^ 1);  // (read last in the previous round, which every wave has left)
-      if (t + 2 < t_hi) issue(t + 2);
-    }
+    commit(t + 1, b ^ 1, w_c);  // (read last in the previous round, which every wave has left; behind the last tile: not read)
+    issue(min(t + 1 + DEPTH, t_hi - 1), w_c);
+  };
+  for (int t = t_lo; t < t_hi;) {  // (left from inside: no way around one of the bodies, or its rows would be waited for at once)
+    body(t, IC<0>{});
+    if (++t >= t_hi) break;
+    if (DEPTH == 2) body(t++, IC<DEPTH - 1>{});
   }
   if (key >= a.Nk) return;
   const int64_t C = (int64_t)a.kvh * a.d, at = ((int64_t)e * a.Nk + key) * C + (int64_t)g * a.d, plane = (int64_t)a.Be * a.Nk * C;
