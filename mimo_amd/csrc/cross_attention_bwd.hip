@@ -221,10 +221,11 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
   // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to a buffer (commit).  Rows
-  // behind the last one repeat it with lse = inf: P = 0.  The 16-byte chunks of a tile are dealt to the threads one after another and
-  // the last threads repeat the last chunk: no request is behind a branch, so a wait for the oldest tile leaves the younger ones on
-  // their way.  The channels behind the last one are zeroed once.
-  constexpr int NC = (QT * 2 * KS + THREADS - 1) / THREADS, DEPTH = dkv_depth(KS);
+  // behind the last one repeat it with lse = inf: P = 0.  Where there are eight threads to a row they take its 16-byte chunks, else
+  // the chunks of the tile are dealt to the threads one after another; threads without one repeat the last: no request is behind a
+  // branch, so a wait for the oldest tile leaves the younger ones on their way.  The channels behind the last one are zeroed once.
+  constexpr bool BY_ROW = THREADS >= 8 * QT && KS > 4;
+  constexpr int NC = BY_ROW ? (2 * KS + 7) / 8 : (QT * 2 * KS + THREADS - 1) / THREADS, DEPTH = dkv_depth(KS);
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
   u32x4 xr[DEPTH][NC], yr[DEPTH][NC];
   float lr[DEPTH], dr[DEPTH];
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     const int dc = a.d >> 3;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = min(tid + i * THREADS, QT * dc - 1), row = (int)div_fast((uint32_t)c, a.by_dc);
-      place[i] = row << 8 | (c - row * dc) * 8;
+      const int c = min(tid + i * THREADS, QT * dc - 1), row = BY_ROW ? min(tid >> 3, QT - 1) : (int)div_fast((uint32_t)c, a.by_dc);
+      place[i] = row << 8 | (BY_ROW ? min((tid & 7) + 8 * i, dc - 1) : c - row * dc) * 8;
     }
     for (int c = tid; c < 2 * 2 * QT * (2 * KS - dc); c += THREADS) {  // (usually none)
       const int row = c / (2 * KS - dc), col = dc + c - row * (2 * KS - dc);  // rows of q, dO of buffer 0, then of buffer 1
@@ -243,14 +244,20 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
   }
   auto issue = [&](int t, auto w_c) __attribute__((always_inline)) {
     constexpr int w = decltype(w_c)::value;
+    const uint16_t *qp = nullptr, *dp = nullptr;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      int at = place[i], img, qi, hh;
+      int at = place[i];
       asm volatile("" : "+v"(at));  // addresses are made anew for every tile: kept over the products they would cost registers
-      flat_row(a, min(t * QT + (at >> 8), a.R - 1), img, qi, hh);
-      const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d + (at & 255);
-      xr[w][i] = *reinterpret_cast<const u32x4*>(a.q + bb * a.sqb + (int64_t)qi * a.sqr + col);
-      yr[w][i] = *reinterpret_cast<const u32x4*>(a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col);
+      if (!BY_ROW || i == 0) {
+        int img, qi, hh;
+        flat_row(a, min(t * QT + (at >> 8), a.R - 1), img, qi, hh);
+        const int64_t bb = (int64_t)e * a.G + img, col = (int64_t)(g * a.hg + hh) * a.d;
+        qp = a.q + bb * a.sqb + (int64_t)qi * a.sqr + col;
+        dp = a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col;
+      }
+      xr[w][i] = *reinterpret_cast<const u32x4*>(qp + (at & 255));
+      yr[w][i] = *reinterpret_cast<const u32x4*>(dp + (at & 255));
     }
     static_assert(QT <= THREADS, "a thread per row");
     int img, qi, hh;
