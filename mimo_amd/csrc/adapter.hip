@@ -330,25 +330,27 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     const int lc = NP * a.r / 8;  // 16-byte chunks of a row of low
     // a tile on its way.  No branch and no dependent load between the requests: rows behind the last one repeat it, columns behind
     // the last one the first; `raw` = the index entry of row lane, it selects when the rows are written
+    typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
     struct Piece {
-      uint4 x[NX], l[NL];
+      u32x4 x[NX], l[NL];
       int raw;
-      int64_t m0;
+      int64_t end;  // rows of it that exist, or more
     };
     auto fetch = [&](Piece& q, int64_t t) {
       int id0 = tid;
       asm volatile("" : "+v"(id0));
-      const int64_t m0 = q.m0 = m_lo + t * MR;
+      const int64_t m0 = m_lo + (t < t_hi ? t : t_hi - 1) * MR;
+      q.end = t < t_hi ? m_hi - m0 : 0;
       const int left = (int)(m_hi - m0 < MR ? m_hi - m0 : MR) - 1;
       const int c = c0 + (id0 & 15) * 8;
       const uint16_t* x = a.x[z] + m0 * a.ldx[z] + (c < C ? c : 0);
       const uint16_t* l = a.low[z] + m0 * NP * a.r;
 #pragma unroll
-      for (int i = 0; i < NX; ++i) q.x[i] = *reinterpret_cast<const uint4*>(x + min((id0 >> 4) + 16 * i, left) * a.ldx[z]);
+      for (int i = 0; i < NX; ++i) q.x[i] = *reinterpret_cast<const u32x4*>(x + min((id0 >> 4) + 16 * i, left) * a.ldx[z]);
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int id = id0 + 256 * i, row = (int)div_fast(id, a.by_lc);
-        q.l[i] = *reinterpret_cast<const uint4*>(l + min(row, left) * NP * a.r + (id - row * lc) * 8);
+        q.l[i] = *reinterpret_cast<const u32x4*>(l + min(row, left) * NP * a.r + (id - row * lc) * 8);
       }
       const unsigned m = (unsigned)m0 + min(lane, left);
       q.raw = a.rows.index[div_fast(m, a.by_rpi)];
@@ -356,17 +358,17 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     auto use = [&](const Piece& q) {
       int id0 = tid;
       asm volatile("" : "+v"(id0));
-      const unsigned long long live = __builtin_amdgcn_ballot_w64(q.raw == who && q.m0 + lane < m_hi);
+      const unsigned long long live = __builtin_amdgcn_ballot_w64(q.raw == who && lane < q.end);
       lds_barrier();
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         const int row = (id0 >> 4) + 16 * i;
-        *reinterpret_cast<uint4*>(xs + row * XP + (id0 & 15) * 8) = (live >> row) & 1 ? q.x[i] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<u32x4*>(xs + row * XP + (id0 & 15) * 8) = (live >> row) & 1 ? q.x[i] : (u32x4){0u, 0u, 0u, 0u};
       }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int id = id0 + 256 * i, row = (int)div_fast(id, a.by_lc);
-        if (row < MR) *reinterpret_cast<uint4*>(ls + row * LP + (id - row * lc) * 8) = (live >> row) & 1 ? q.l[i] : make_uint4(0, 0, 0, 0);
+        if (row < MR) *reinterpret_cast<u32x4*>(ls + row * LP + (id - row * lc) * 8) = (live >> row) & 1 ? q.l[i] : (u32x4){0u, 0u, 0u, 0u};
       }
       lds_barrier();
     };
@@ -387,26 +389,22 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
         }
       }
     };
-    if constexpr (RT <= 4) {  // two tiles ahead of the products (the largest ranks have registers for one)
-      Piece q0, q1;
-      if (t_lo < t_hi) fetch(q0, t_lo);
-      if (t_lo + 1 < t_hi) fetch(q1, t_lo + 1);
-      for (int64_t t = t_lo; t < t_hi; t += 2) {
-        use(q0);
-        if (t + 2 < t_hi) fetch(q0, t + 2);
-        products();
-        if (t + 1 >= t_hi) break;
-        use(q1);
-        if (t + 3 < t_hi) fetch(q1, t + 3);
-        products();
-      }
-    } else {
-      Piece q0;
-      if (t_lo < t_hi) fetch(q0, t_lo);
-      for (int64_t t = t_lo; t < t_hi; ++t) {
-        use(q0);
-        if (t + 1 < t_hi) fetch(q0, t + 1);
-        products();
+    // two tiles ahead of the products (the largest ranks have registers for one).  A tile behind the last one repeats it and has no
+    // live rows: no way leads around a request or a step, so a tile is waited for while the younger one stays on its way
+    if (t_lo < t_hi) {
+      constexpr int AHEAD = RT <= 4 ? 2 : 1;
+      Piece q[AHEAD];
+      fetch(q[0], t_lo);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (AHEAD == 2) fetch(q[1], t_lo + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      for (int64_t t = t_lo; t < t_hi; t += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          use(q[i]);
+          fetch(q[i], t + i + AHEAD);
+          products();
+        }
       }
     }
   }

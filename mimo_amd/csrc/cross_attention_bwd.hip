@@ -281,7 +281,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     float l = lr[w];
     asm volatile("" : "+v"(l));  // (not earlier: what is made of it would wait for the requests)
     if (tid < QT) {
-      l2[tid] = l == -INFINITY || t * QT + tid >= a.R ? INFINITY : l * LOG2E;
+      l2[tid] = l == -INFINITY || t * QT + tid >= a.R || t >= t_hi ? INFINITY : l * LOG2E;
       l2[QT + tid] = dr[w];
     }
   };
@@ -336,13 +336,13 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       }
     }
     }
-    commit(t + 1, b ^ 1, w_c);  // (read last in the previous round, which every wave has left; behind the last tile: not read)
+    commit(t + 1, b ^ 1, w_c);  // (read last in the previous round, which every wave has left)
     issue(min(t + 1 + DEPTH, t_hi - 1), w_c);
   };
-  for (int t = t_lo; t < t_hi;) {  // (left from inside: no way around one of the bodies, or its rows would be waited for at once)
+  // (a tile behind the last one repeats it with P = 0: a way around a body would have its rows waited for at once)
+  for (int t = t_lo; t < t_hi; t += DEPTH) {
     body(t, IC<0>{});
-    if (++t >= t_hi) break;
-    if (DEPTH == 2) body(t++, IC<DEPTH - 1>{});
+    if (DEPTH == 2) body(t + 1, IC<DEPTH - 1>{});
   }
   if (key >= a.Nk) return;
   const int64_t C = (int64_t)a.kvh * a.d, at = ((int64_t)e * a.Nk + key) * C + (int64_t)g * a.d, plane = (int64_t)a.Be * a.Nk * C;
