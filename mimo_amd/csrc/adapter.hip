@@ -424,25 +424,26 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
   }
 }
 
-// the sum of the parts in order: ddown [n, r, K] as it lies, dup [n, N, r] transposed.  A thread takes four columns; eight parts are
-// on their way at a time.
+// the sum of the parts: eight runs of them side by side (a block takes 32 pieces of four columns), then the runs in order; ddown
+// [n, r, K] as it lies, dup [n, N, r] transposed
 __global__ __launch_bounds__(256) void adapter_join_kernel(const float* p0, const float* p1, float* ddown, float* dup, int n, int r, int K,
                                                            int N, int parts) {
-  const int64_t s0 = (int64_t)n * r * K, s1 = (int64_t)n * r * N, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= s0 + s1) return;
+  __shared__ f32x4 sums[8][32];
+  const int64_t s0 = (int64_t)n * r * K, s1 = (int64_t)n * r * N, i = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 4;
+  const int run = threadIdx.x >> 5, per = (parts + 7) / 8, q0 = run * per, q1 = min(parts, q0 + per);
   const bool first = i < s0;
   const int64_t at = first ? i : i - s0, plane = first ? s0 : s1;
-  const float* p = (first ? p0 : p1) + at;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int q0 = 0; q0 < parts; q0 += 8) {
-    f32x4 x[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q0 + q < parts) x[q] = *reinterpret_cast<const f32x4*>(p + (int64_t)(q0 + q) * plane);
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q0 + q < parts) s += x[q];
+  if (i < s0 + s1) {
+    const float* p = (first ? p0 : p1) + at;
+#pragma unroll 4
+    for (int q = q0; q < q1; ++q) s += *reinterpret_cast<const f32x4*>(p + (int64_t)q * plane);
   }
+  sums[run][threadIdx.x & 31] = s;
+  lds_barrier();
+  if (run || i >= s0 + s1) return;
+#pragma unroll
+  for (int u = 1; u < 8; ++u) s += sums[u][threadIdx.x];
   if (first) {
     *reinterpret_cast<f32x4*>(ddown + at) = s;
   } else {
@@ -821,7 +822,7 @@ int backward(const void* dY, int64_t ldy, const void* A, int64_t lda, const void
   else if (rt <= 4) hipLaunchKernelGGL((adapter_outer_kernel<DT, 4>), grid, dim3(256), 0, st, oa);
   else hipLaunchKernelGGL((adapter_outer_kernel<DT, 8>), grid, dim3(256), 0, st, oa);
   MIMO_LAUNCH_CHECK();
-  const int64_t total = (int64_t)n * r * (N + K), nwg = (total / 4 + 255) / 256;
+  const int64_t total = (int64_t)n * r * (N + K), nwg = (total / 4 + 31) / 32;
   if (nwg > 0x7fffffff) return MIMO_EINVAL;
   hipLaunchKernelGGL(adapter_join_kernel, dim3((unsigned)nwg), dim3(256), 0, st, p0, p1, ddown, dup, n, r, K, N,
                      b.parts);
