@@ -5,7 +5,7 @@
 //
 // Two kernels, both recompute P from lse (no score is ever stored):
 //   xattn_dq_kernel   S^T = K.Q^T and dP^T = V.dO^T: a lane owns a query, dS^T packed is the operand of dQ^T = K^T.dS^T.  Keys
-//                     resident in LDS as in the forward, or streamed; also leaves delta.
+//                     resident in LDS as in the forward, or streamed; also leaves delta (few keys: sum_k P dP instead of dO.O).
 //   xattn_dkv_kernel  S = Q.K^T and dP = dO.V^T: a lane owns a key, a wave 32 of them with K and V in registers; the block's waves
 //                     share the query tiles that pass through LDS, P and dS packed are the operands of dV^T = dO^T.P and
 //                     dK^T = Q^T.dS.  The flat rows are cut into parts (gridDim.y) when the keys do not fill the chip; their
@@ -16,11 +16,6 @@
 
 namespace mimo_xattn {
 namespace {
-
-template <int V>
-struct IC {
-  static constexpr int value = V;
-};
 
 constexpr int stream_keys(int ks) { return ks >= 6 ? 32 : 64; }  // keys per streamed buffer of dq
 
@@ -49,6 +44,21 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
   const int step = a.nb * NW;
   int t = j * NW + wave;
   const int rounds = (T - j * NW + step - 1) / step;
+
+  // delta from the rounded output is off by u |dO||O|: nothing beside dS where many keys share the row, but half of dQ's error where
+  // two do (relative l2 of dQ at 2, 8, 32 keys of width 40 in fp16: 4.7, 3.2, 3.05e-4; from P and dP 2.9, 3.0, 2.96e-4).  Up to 32
+  // keys that count are gathered into one tile for it, lane i (of each half) taking the i-th of them.
+  int n_few = 0, mine = 0;
+  for (int k = 0; k < len && n_few <= 32; k += 64) {
+    const bool on = k + lane < len && (!a.mask || a.mask[(int64_t)e * a.smb + min(k + lane, len - 1)] != 0);
+    const unsigned long long b = __builtin_amdgcn_ballot_w64(on);
+    const int rank = n_few + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, 0u));
+    const int got = __builtin_amdgcn_ds_permute(4 * (on && rank < 32 ? rank : 63), on ? k + lane + 1 : 0);  // (lane 63 keeps the rest)
+    if (lane < 32 && got > 0) mine = got - 1;
+    n_few += __builtin_popcountll(b);
+  }
+  const bool few = n_few <= 32;
+  mine = __shfl(mine, li, 64);
 
   struct Row {
     uint4 q[KS], d[KS], o[KS];
@@ -98,6 +108,29 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
       delta += __shfl_xor(delta, 32, 64);
     }
     if (l2 == -INFINITY) l2 = INFINITY;  // a row without a key: P = exp2(0 - inf) = 0
+    if (few) {
+      const uint16_t* kp = a.k + (int64_t)e * a.skb + (int64_t)mine * a.skr + (int64_t)g * a.d;
+      const uint16_t* vp = a.v + (int64_t)e * a.svb + (int64_t)mine * a.svr + (int64_t)g * a.d;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        const int kk = 16 * i + 8 * h2;
+        uint4 x = make_uint4(0, 0, 0, 0), y = x;
+        if (li < n_few && kk < a.d) {
+          x = *reinterpret_cast<const uint4*>(kp + kk);
+          y = *reinterpret_cast<const uint4*>(vp + kk);
+        }
+        s = HT<DT>::mfma32(x, qf[i], s);
+        dp = HT<DT>::mfma32(y, df[i], dp);
+      }
+      delta = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + 4 * h2 + (r & 3) < n_few) delta = fmaf(fast_exp2(fmaf(s[r], a.c, -l2)), dp[r], delta);
+      delta += __shfl_xor(delta, 32, 64);
+    }
     const RowPlace out = row_place(a, e, g, min(t, T - 1), li, a.out, a.delta);
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, delta), out.table, t < T && h2 == 0 ? out.stat : 0xF0000000u, 0, 0);
     f32x16 acc[OT];
@@ -172,7 +205,6 @@ constexpr int dkv_buffers(int ks, int nw) { return 2 * (2 * qt_rows(ks, nw) * (1
 constexpr int dkv_share(int ks) { return ks >= 8 ? 2 : 1; }
 constexpr int dkv_lds(int ks, int nw) { return dkv_buffers(ks, nw) + (dkv_share(ks) == 2 ? nw * ks * 1024 : 0); }
 constexpr int dkv_occ(int ks) { return ks <= 2 ? 3 : 2; }    // waves per SIMD
-constexpr int dkv_depth(int ks) { return ks <= 4 || ks >= 8 ? 2 : 1; }  // row tiles on their way in registers, where there are some to spare
 
 // NW: key tiles of a block
 template <int DT, int KS, int NW>
@@ -223,12 +255,12 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
   // rows [QT t, QT t + QT) of q and dO, their lse (log2 units) and delta: requested (issue), written to a buffer (commit).  Rows
   // behind the last one repeat it with lse = inf: P = 0.  Where there are eight threads to a row they take its 16-byte chunks, else
   // the chunks of the tile are dealt to the threads one after another; threads without one repeat the last: no request is behind a
-  // branch, so a wait for the oldest tile leaves the younger ones on their way.  The channels behind the last one are zeroed once.
+  // branch.  The channels behind the last one are zeroed once.
   constexpr bool BY_ROW = THREADS >= 8 * QT && KS > 4;
-  constexpr int NC = BY_ROW ? (2 * KS + 7) / 8 : (QT * 2 * KS + THREADS - 1) / THREADS, DEPTH = dkv_depth(KS);
+  constexpr int NC = BY_ROW ? (2 * KS + 7) / 8 : (QT * 2 * KS + THREADS - 1) / THREADS;
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-  u32x4 xr[DEPTH][NC], yr[DEPTH][NC];
-  float lr[DEPTH], dr[DEPTH];
+  u32x4 xr[NC], yr[NC];
+  float lr, dr;
   int place[NC];  // row << 8 | channel of this thread's chunks
   {
     const int dc = a.d >> 3;
@@ -242,8 +274,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       *reinterpret_cast<uint4*>(smem + (row >= 2 * QT ? BUF - 2 * QT * P * 2 : 0) + row * P * 2 + col * 16) = make_uint4(0, 0, 0, 0);
     }
   }
-  auto issue = [&](int t, auto w_c) __attribute__((always_inline)) {
-    constexpr int w = decltype(w_c)::value;
+  auto issue = [&](int t) __attribute__((always_inline)) {
     const uint16_t *qp = nullptr, *dp = nullptr;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -256,18 +287,17 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
         qp = a.q + bb * a.sqb + (int64_t)qi * a.sqr + col;
         dp = a.dout + bb * a.sdb + (int64_t)qi * a.sdr + col;
       }
-      xr[w][i] = *reinterpret_cast<const u32x4*>(qp + (at & 255));
-      yr[w][i] = *reinterpret_cast<const u32x4*>(dp + (at & 255));
+      xr[i] = *reinterpret_cast<const u32x4*>(qp + (at & 255));
+      yr[i] = *reinterpret_cast<const u32x4*>(dp + (at & 255));
     }
     static_assert(QT <= THREADS, "a thread per row");
     int img, qi, hh;
     flat_row(a, min(t * QT + (tid & (QT - 1)), a.R - 1), img, qi, hh);
     const int64_t stat = (((int64_t)e * a.G + img) * a.kvh * a.hg + g * a.hg + hh) * a.Nq + qi;
-    lr[w] = a.lse_in[stat];
-    dr[w] = a.delta[stat];
+    lr = a.lse_in[stat];
+    dr = a.delta[stat];
   };
-  auto commit = [&](int t, int b, auto w_c) __attribute__((always_inline)) {
-    constexpr int w = decltype(w_c)::value;
+  auto commit = [&](int t, int b) __attribute__((always_inline)) {
     uint16_t* qs = reinterpret_cast<uint16_t*>(smem + b * BUF);
     float* l2 = reinterpret_cast<float*>(smem + b * BUF + 2 * QT * P * 2 + 64);
 #pragma unroll
@@ -275,28 +305,25 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       int at = place[i];
       asm volatile("" : "+v"(at));
       uint16_t* to = qs + (at >> 8) * P + (at & 255);
-      *reinterpret_cast<u32x4*>(to) = xr[w][i];
-      *reinterpret_cast<u32x4*>(to + QT * P) = yr[w][i];
+      *reinterpret_cast<u32x4*>(to) = xr[i];
+      *reinterpret_cast<u32x4*>(to + QT * P) = yr[i];
     }
-    float l = lr[w];
+    float l = lr;
     asm volatile("" : "+v"(l));  // (not earlier: what is made of it would wait for the requests)
     if (tid < QT) {
-      l2[tid] = l == -INFINITY || t * QT + tid >= a.R || t >= t_hi ? INFINITY : l * LOG2E;
-      l2[QT + tid] = dr[w];
+      l2[tid] = l == -INFINITY || t * QT + tid >= a.R ? INFINITY : l * LOG2E;
+      l2[QT + tid] = dr;
     }
   };
-  // row tile t is in buffer (t - t_lo) & 1; t + 1 .. t + DEPTH are on their way, t + 1 + k in registers (t + k - t_lo) % DEPTH
+  // row tile t is in buffer (t - t_lo) & 1, t + 1 on its way
   if (t_lo < t_hi) {
-    issue(t_lo, IC<0>{});
-    commit(t_lo, 0, IC<0>{});
+    issue(t_lo);
+    commit(t_lo, 0);
     settle<KS>(kf);
     if constexpr (SHARE == 1) settle<KS>(vf);
-    issue(min(t_lo + 1, t_hi - 1), IC<0>{});
-    __builtin_amdgcn_sched_barrier(0);  // in the order in which the loop takes them
-    if (DEPTH == 2) issue(min(t_lo + 2, t_hi - 1), IC<DEPTH - 1>{});
-    __builtin_amdgcn_sched_barrier(0);
+    issue(min(t_lo + 1, t_hi - 1));
   }
-  auto body = [&](int t, auto w_c) __attribute__((always_inline)) {
+  for (int t = t_lo; t < t_hi; ++t) {
     const int b = (t - t_lo) & 1;
     lds_barrier();
     const uint16_t* qs = reinterpret_cast<const uint16_t*>(smem + b * BUF);
@@ -336,13 +363,9 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       }
     }
     }
-    commit(t + 1, b ^ 1, w_c);  // (read last in the previous round, which every wave has left)
-    issue(min(t + 1 + DEPTH, t_hi - 1), w_c);
-  };
-  // (a tile behind the last one repeats it with P = 0: a way around a body would have its rows waited for at once)
-  for (int t = t_lo; t < t_hi; t += DEPTH) {
-    body(t, IC<0>{});
-    if (DEPTH == 2) body(t + 1, IC<DEPTH - 1>{});
+    // (read last in the previous round, which every wave has left; behind the last tile it is not read, but nothing leads around a request)
+    commit(t + 1, b ^ 1);
+    issue(min(t + 2, t_hi - 1));
   }
   if (key >= a.Nk) return;
   const int64_t C = (int64_t)a.kvh * a.d, at = ((int64_t)e * a.Nk + key) * C + (int64_t)g * a.d, plane = (int64_t)a.Be * a.Nk * C;

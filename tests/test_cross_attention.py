@@ -5,7 +5,7 @@ With u = eps / 2 of the operand type: out = (sum_k half(p) v) / l rounds every p
 |error| <= u (sum_k p |v| / l + |out|); lse, delta and every sum are fp32, whose errors enter through the scores:
 ds = d 2^-24 scale max sum_c |q_c k_c| (a dot product of d terms), i.e. a factor 1 +- 2 ds on every p.  Values of p or dS below
 the normal range of fp16 are off by at most 2^-25 absolutely.  The gradients likewise: dS rounds once, delta is taken from the
-rounded output (|d delta| <= u sum |dO o|), the result rounds once."""
+rounded output (|d delta| <= u sum |dO o|) unless few keys count, the result rounds once."""
 import ctypes
 
 import pytest
@@ -175,6 +175,40 @@ def test_strided_and_broadcast_operands(dev, dtype):
         val, bnd = reference(q, kv[..., :C], kv[..., C:], heads, heads, keep, 0.3, dout)
         for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + grads):
             within(name, got, val[name], bnd[name])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Nq,Nk,heads,kvh,d,live", [(600, 2, 4, 4, 40, 2), (600, 77, 4, 2, 40, 3), (300, 257, 4, 4, 160, 5), (500, 64, 4, 4, 64, 20),
+                                                    (300, 300, 2, 2, 160, 30)])
+def test_gradients_of_few_keys(dev, dtype, Nq, Nk, heads, kvh, d, live):
+    """Where few keys share a row dS is a small difference of P dP and P delta, and a delta taken from the rounded output would double
+    dQ's error.  What is left are two roundings, dS's and the result's, each uniform within half a step: 0.425 u of the value in the
+    mean square (1 / sqrt(3), mantissas spread evenly in their logarithm), independent of each other; 15 % for the sample."""
+    from mimo_amd import ops
+    q, kv = rnd((2, Nq, heads * d), dev, dtype, 11), rnd((2, Nk, 2 * kvh * d), dev, dtype, 12)
+    k, v, dout = kv[..., :kvh * d], kv[..., kvh * d:], rnd((2, Nq, heads * d), dev, dtype, 13)
+    kv_len = mask = None
+    keep = torch.zeros((2, Nk), dtype=torch.bool, device=dev)
+    if live < Nk:   # row 0: anywhere, by the mask; row 1: in front, by the mask
+        keep[0, torch.randperm(Nk, generator=torch.Generator().manual_seed(4))[:live].to(dev)] = True
+        keep[1, :live] = True
+        mask = keep
+    else:
+        keep[:] = True
+    out, lse = ops.cross_attention(q, k, v, heads, kv_heads=kvh, mask=mask, want_lse=True)
+    val, _ = reference(q, k, v, heads, kvh, keep, d ** -0.5, dout)
+    u, tiny, hg = torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype == torch.float16 else 0.0, heads // kvh
+    split = lambda x, n: x.double().reshape(2, -1, n, d).transpose(1, 2)
+    Q, G, K, V = split(q, heads), split(dout, heads), split(k, kvh).repeat_interleave(hg, 1), split(v, kvh).repeat_interleave(hg, 1)
+    P = (Q @ K.transpose(2, 3) * d ** -0.5).masked_fill(~keep[:, None, None, :], float("-inf")).softmax(-1)
+    dP = G @ V.transpose(2, 3)
+    dS2 = (P * (dP - (P * dP).sum(-1, keepdim=True))).square() * (0.425 * u) ** 2 + tiny ** 2 * keep[:, None, None, :]
+    for name, got, from_dS in zip(("dq", "dk"), ops.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_heads=kvh, mask=mask),
+                                  (dS2 @ K.square(), dS2.transpose(2, 3) @ Q.square())):
+        left = float((from_dS.sum() / d + val[name].square().sum() * (0.425 * u) ** 2 + tiny ** 2 * got.numel()).sqrt())
+        off = float((got.double() - val[name]).norm())
+        assert off <= 1.15 * left, (name, off, left)
 
 
 @gpu
