@@ -88,7 +88,8 @@ __device__ __forceinline__ float scale_of(const LowArgs& a, int ad) { return ad 
 // pieces of 64 channels: eight neighbouring lanes read 128 bytes of a row of X (of down), the piece passes through the wave's own
 // LDS patch into fragments, the next piece is on its way meanwhile — fragments straight from memory (a row per lane) cost the
 // address path a look-up per lane.  KSPLIT: the block's waves share 32 rows and take pieces in turn, joined in LDS in wave order —
-// few rows; else each of four waves has 32 rows of its own.  Bound by the stream of X; down comes from L2.
+// few rows; else each of four waves has 32 rows of its own.  Bound by the stream of X, down comes from L2: M = 196608, K = 320 in
+// 22.5 us where X is in the last-level cache (5.6 TB/s), 40 us from HBM behind other traffic.
 constexpr int low_waves(int rt, bool ksplit) { return ksplit && rt < 8 ? 8 : 4; }
 template <int DT, int RT, bool KSPLIT>
 __global__ __launch_bounds__(64 * low_waves(RT, KSPLIT)) void adapter_low_kernel(const LowArgs a) {
@@ -256,6 +257,7 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(const TransposeA
 // A block owns 128 columns of x and all ranks; tiles of 64 rows pass through LDS row-major, both operands are read transposed
 // (a row that is not this adapter's is staged as zeros on BOTH sides); the planes of low meet the same columns (fp16: the remainder
 // plane has accumulators of its own, its scale comes off at the end).  Rows: only [first, last] of the adapter, cut into gridDim.z parts.
+// Bound by the streams of a and dy: 49152 rows of 640 + 640, r = 32 in 38 us (3.4 TB/s).
 struct OuterArgs {
   const uint16_t *x[2], *low[2];
   float* part[2];  // [parts][n][r][C]
@@ -334,13 +336,12 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     struct Piece {
       u32x4 x[NX], l[NL];
       int raw;
-      int64_t end;  // rows of it that exist, or more
+      int64_t m0;
     };
     auto fetch = [&](Piece& q, int64_t t) {
       int id0 = tid;
       asm volatile("" : "+v"(id0));
-      const int64_t m0 = m_lo + (t < t_hi ? t : t_hi - 1) * MR;
-      q.end = t < t_hi ? m_hi - m0 : 0;
+      const int64_t m0 = q.m0 = m_lo + t * MR;
       const int left = (int)(m_hi - m0 < MR ? m_hi - m0 : MR) - 1;
       const int c = c0 + (id0 & 15) * 8;
       const uint16_t* x = a.x[z] + m0 * a.ldx[z] + (c < C ? c : 0);
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
     auto use = [&](const Piece& q) {
       int id0 = tid;
       asm volatile("" : "+v"(id0));
-      const unsigned long long live = __builtin_amdgcn_ballot_w64(q.raw == who && lane < q.end);
+      const unsigned long long live = __builtin_amdgcn_ballot_w64(q.raw == who && q.m0 + lane < m_hi);
       lds_barrier();
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
@@ -389,22 +390,15 @@ __global__ __launch_bounds__(256) void adapter_outer_kernel(const OuterArgs a) {
         }
       }
     };
-    // two tiles ahead of the products (the largest ranks have registers for one).  A tile behind the last one repeats it and has no
-    // live rows: no way leads around a request or a step, so a tile is waited for while the younger one stays on its way
+    // the next tile on its way while this one's products run (two ahead were no faster: 121.9 against 117.5 us for the whole backward
+    // at M = 49152, N = K = 640, r = 32, 48.7 against 47.3 us at 5003 x 640 x 1280, r = 24)
     if (t_lo < t_hi) {
-      constexpr int AHEAD = RT <= 4 ? 2 : 1;
-      Piece q[AHEAD];
-      fetch(q[0], t_lo);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (AHEAD == 2) fetch(q[1], t_lo + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      for (int64_t t = t_lo; t < t_hi; t += AHEAD) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          use(q[i]);
-          fetch(q[i], t + i + AHEAD);
-          products();
-        }
+      Piece q;
+      fetch(q, t_lo);
+      for (int64_t t = t_lo; t < t_hi; ++t) {
+        use(q);
+        fetch(q, t + 1 < t_hi ? t + 1 : t);  // (the last one again rather than a way around the request)
+        products();
       }
     }
   }
@@ -455,7 +449,8 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(const float* p0, cons
 }
 
 // A few rows (M <= 16 MG) against the whole weight: a block of eight waves takes 16 columns, the waves share K (every eighth
-// k-step) and meet in LDS in wave order.  Bound by latency: one trip to W, one to the adapters.  RT > 0 (MG = 1): u is computed
+// k-step) and meet in LDS in wave order.  Bound by latency: one trip to W, one to the adapters (8 rows, N = K = 1280: 6.0 us, and 5.9
+// for u in front of it).  RT > 0 (MG = 1): u is computed
 // here too, by every block for itself — the rows' down weights come from L2 and a launch is saved; RT = 0: u is given.
 struct SkinnyArgs {
   const uint16_t *X, *W, *down, *up;
@@ -615,15 +610,19 @@ __global__ __launch_bounds__(512) void adapter_skinny_kernel(const SkinnyArgs a)
 // ---- host side --------------------------------------------------------------------------------------------------------------
 template <int DT>
 int launch_low(const LowArgs& a, hipStream_t st) {
-  // few rows with an adapter each: a matrix tile would run once per row, a block per row reads what the row needs
-  if (a.rows.rpi == 1 && a.rows.M <= 256 && a.rows.n > 1) {
+  // up to 1024 rows with an index each: a matrix tile would run once per adapter in it, a block per row reads what the row needs (whole
+  // call, N = K = 1280, r = 16, 1024 rows: of 64 adapters in turn 46 us against 95, of 8 in turn 31 against 39, of 8 in runs 26 against
+  // 21; 2048 rows of 8: 36 against 42 and 31 against 24)
+  if (a.rows.rpi == 1 && a.rows.M <= 1024 && a.rows.n > 1) {
     hipLaunchKernelGGL((adapter_low_row_kernel<DT>), dim3((unsigned)a.rows.M), dim3(256), 0, st, a);
     MIMO_LAUNCH_CHECK();
     return MIMO_OK;
   }
   const int rt = (a.r + 15) / 16;
   const int64_t m32 = (a.rows.M + 31) / 32;
-  const bool ksplit = m32 < 4 * (int64_t)cu_count();  // one wave per 32 rows would leave SIMDs empty
+  // one wave per 32 rows would leave SIMDs empty (whole call, N = K = 640, r = 16: 29.9 us split, 32.5 not, at M = 16384; 69.3 and 66.4
+  // at M = 49152)
+  const bool ksplit = m32 < 4 * (int64_t)cu_count();
   const int64_t nwg = ksplit ? m32 : (m32 + 3) / 4;
   if (nwg > 0x7fffffff) return MIMO_EINVAL;
 #define LOW(RT)                                                                                                                  \
@@ -694,7 +693,9 @@ int launch_gemm(GemmArgs g, hipStream_t st) {
     c.a_bytes = (unsigned)(((c.M - 1) * c.lda + c.K) * 2);
     const int64_t tn8 = (c.N + 255) / 256, nt8 = ((c.M + 255) / 256) * tn8;
     int rc;
-    if ((c.K % 64) == 0 && tn8 * 256 - c.N <= c.N / 12 && nt8 >= 128 && nt8 <= 0x7fffffff) {
+    // (256 x 256 tiles once they fill three quarters of the chip: 85.8 us against 91.5 for the other tiles at 245 of them, M = 12321,
+    // N = K = 1280, r = 64, fp32 out; 45.0 against 40.5 at 160, M = 8192, r = 16)
+    if ((c.K % 64) == 0 && tn8 * 256 - c.N <= c.N / 12 && 4 * nt8 >= 3 * (int64_t)cu_count() && nt8 <= 0x7fffffff) {
       c.tiles_n = (int)tn8;
       c.ntiles = (unsigned)G8_GM;
       hipLaunchKernelGGL((gemm8_kernel<DT, 3>), dim3((unsigned)nt8), dim3(512), 0, st, c);
@@ -737,14 +738,16 @@ GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t
   return g;
 }
 
-// Up to 64 rows: the skinny kernel; u inside it for one or two rows (it takes their adapters one after another).
+// Up to 64 rows: the skinny kernel (N = K = 1280, r = 16: 19.7 us for 8 rows, 20.5 for 64, by the tiles 24.5 and 26.2; N = K = 320, 64
+// rows: 19.7 against 20.0); u inside it for up to four rows, whose adapters it takes one after another (17.2 us against 20.1 with a
+// launch for u; eight rows of different adapters 20.9 against 19.7).
 template <int DT>
 int launch_skinny(const GemmArgs& g, const LowArgs& la, bool give_low, hipStream_t st) {
   SkinnyArgs a{g.A, g.W, la.down, g.ad_up, la.scale, g.bias, g.res, g.out, give_low ? la.low : nullptr, g.lda, g.ldo, g.ldr, la.rows,
                g.N, g.K, la.r, la.planes, g.ad_cols, g.flags};
   const dim3 grid((unsigned)((g.N + 15) / 16));
   const int rt = (la.r + 15) / 16, mg = (int)((g.M + 15) / 16);
-  if (g.M <= 2 && rt <= 4) {
+  if (g.M <= 4 && rt <= 4) {
     if (rt == 1) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 1>), grid, dim3(512), 0, st, a);
     else if (rt == 2) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 2>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 4>), grid, dim3(512), 0, st, a);

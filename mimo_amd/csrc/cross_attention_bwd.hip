@@ -6,12 +6,16 @@
 // Two kernels, both recompute P from lse (no score is ever stored):
 //   xattn_dq_kernel   S^T = K.Q^T and dP^T = V.dO^T: a lane owns a query, dS^T packed is the operand of dQ^T = K^T.dS^T.  Keys
 //                     resident in LDS as in the forward, or streamed; also leaves delta (few keys: sum_k P dP instead of dO.O).
+//                     What bounds it: the rows of q, dO, O and dQ, a piece of 2 d bytes per head and row: 55 us for 16 x 4096 queries,
+//                     8 heads of 40, 77 keys (3.1 TB/s); for 24 x 255 queries, 8 heads of 160, 257 streamed keys the exponentials and
+//                     LDS reads between the products of two waves per SIMD (39 us).
 //   xattn_dkv_kernel  S = Q.K^T and dP = dO.V^T: a lane owns a key, a wave 32 of them with K and V in registers; the block's waves
 //                     share the query tiles that pass through LDS, P and dS packed are the operands of dV^T = dO^T.P and
 //                     dK^T = Q^T.dS.  The flat rows are cut into parts (gridDim.y) when the keys do not fill the chip; their
 //                     fp32 sums are joined in a fixed order by xattn_dkv_join_kernel: no atomics, the same bits every time.
 // P and dS are rounded to the operand type for the last products (one rounding each of the size of the results' own); sums, lse
-// and delta are fp32.
+// and delta are fp32.  What bounds dk / dv: products (22 % of the time), LDS (32 %) and vector instructions (34 %) hardly overlap at
+// two waves per SIMD: 49 us at the last of these shapes, 44 us at the first.
 #include "cross_attention.hip.h"
 
 namespace mimo_xattn {
@@ -200,8 +204,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
 constexpr int qt_rows(int ks, int nw) { return ks <= 4 && nw > 2 ? 64 : 32; }
 constexpr int dkv_buffers(int ks, int nw) { return 2 * (2 * qt_rows(ks, nw) * (16 * ks + 8) * 2 + 2 * qt_rows(ks, nw) * 4 + 64); }
 // waves that share a key tile: dK and dV of a wide head do not fit one wave's registers beside its K and V, so two waves form the
-// same P and dS and each takes half of the channels
-// (and V's fragments are in LDS)
+// same P and dS and each takes half of the channels (and V's fragments are in LDS): two waves per SIMD without spills, 55 us against
+// 94 with one wave of 500 registers (24 x 255 queries, 8 heads of 160, 257 keys)
 constexpr int dkv_share(int ks) { return ks >= 8 ? 2 : 1; }
 constexpr int dkv_lds(int ks, int nw) { return dkv_buffers(ks, nw) + (dkv_share(ks) == 2 ? nw * ks * 1024 : 0); }
 constexpr int dkv_occ(int ks) { return ks <= 2 ? 3 : 2; }    // waves per SIMD
@@ -417,11 +421,13 @@ struct Plan {
   int dq_nw, lds, nb;      // dq
   int nw, groups, nsplit;  // dk / dv
 };
-// key tiles per block: heads whose tiles take two waves have 2; from 80 channels on one wave alone could not hold the rows on their way
-constexpr int least_tiles(int ks) { return ks >= 5 ? 2 : 1; }
+// key tiles per block: heads whose tiles take two waves have 2
+constexpr int least_tiles = 2;
 constexpr int most_tiles(int ks) { return dkv_share(ks) == 2 ? 2 : 4; }
-// dq: as the forward.  dk / dv: the number of key tiles per block (up to four) that leaves the fewest waves without one; the rows are
-// cut into as many parts as fill the chip once with resident blocks, a part keeping at least four row tiles.
+// dq: as the forward (resident 105 us, streamed 108 for the whole backward of 16 x 4096 queries, 8 heads of 40, 77 keys).  dk / dv: the
+// number of key tiles per block (two to four) that leaves the fewest waves without one (same queries, 64 keys: 98 us, four of them
+// always 102; a block of one wave for 32 keys 116 against 108); the rows are cut into as many parts as fill the chip once with
+// resident blocks, a part keeping at least four row tiles (forward and backward 152 us; twice the parts 155, a third 170).
 Plan plan(const Args& a) {
   Plan p{};
   const int ks = k_steps(a.d), cus = cu_count(), eg = a.Be * a.kvh;
@@ -434,7 +440,7 @@ Plan plan(const Args& a) {
   if (p.nb > most) p.nb = most;
   const int tiles = a.Nk > 0 ? (a.Nk + 31) / 32 : 1;  // (without keys there is no dk / dv launch)
   p.nw = most_tiles(ks);
-  for (int w = p.nw - 1; w >= least_tiles(ks); --w)
+  for (int w = p.nw - 1; w >= least_tiles; --w)
     if ((tiles + w - 1) / w * w < (tiles + p.nw - 1) / p.nw * p.nw) p.nw = w;
   p.groups = (tiles + p.nw - 1) / p.nw;
   const int T = (a.R + qt_rows(ks, p.nw) - 1) / qt_rows(ks, p.nw);
@@ -468,8 +474,6 @@ int launch(Args& a, const Plan& p, hipStream_t st) {
   if constexpr (dkv_share(KS) == 2) {
     hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(256), shm, st, a);
   } else {
-    if constexpr (least_tiles(KS) == 1)
-      if (p.nw == 1) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 1>), grid, dim3(64), shm, st, a);
     if (p.nw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 2>), grid, dim3(128), shm, st, a);
     if (p.nw == 3) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 3>), grid, dim3(192), shm, st, a);
     if (p.nw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<DT, KS, 4>), grid, dim3(256), shm, st, a);
