@@ -141,7 +141,7 @@ int mimo_gemm_ext(int dtype, const void* A, int64_t lda, const void* W, void* ou
  *   out[m] = A[m].W^T + bias + residual[m] + u[m].up[i]^T,   u[m] = scale[i] A[m].down[i]^T,   i = index[m / rows_per_index]
  *   A: half16 [M, lda]; W: half16 [N, K]; out: half16 or (MIMO_EPI_OUT_F32) fp32 [M, ldo]; bias fp32 [N], residual half16 or
  *   (MIMO_EPI_RES_F32) fp32 [M, ldr], both nullable; flags: those two only.  N % 8 == 0, K % 8 == 0, N K < 2^30,
- *   N, K < 2^23, M < 2^31.
+ *   N, K < 2^20, lda, ldo, ldr, ldy, ldda <= 2^20, M < 2^31.
  *   down: half16 [count, rank, K], up: half16 [count, N, rank], rank % 8 == 0, rank <= 128 (pad a smaller one with zeros);
  *   scale: fp32 [count] or NULL (1); index: int32 device array of ceil(M / rows_per_index) entries, in any order and number; an
  *   entry outside [0, count) means no adapter.

@@ -712,7 +712,7 @@ int launch_gemm(GemmArgs g, hipStream_t st) {
 // checks shared by both entries
 int check(const mimo_adapter_params* p, int64_t M, int N, int K) {
   if (!p || M <= 0 || M >= 0x7fffffffLL || N <= 0 || K <= 0 || (N & 7) || (K & 7) || (int64_t)N * K >= 0x40000000LL ||
-      N >= 0x800000 || K >= 0x800000)
+      N >= 0x100000 || K >= 0x100000)
     return MIMO_EINVAL;
   if (!p->down || !p->up || !p->index || p->count <= 0 || p->rank <= 0 || p->rank > 128 || (p->rank & 7) || p->rows_per_index <= 0)
     return MIMO_EINVAL;
@@ -840,7 +840,7 @@ extern "C" int mimo_adapter_gemm(int dtype, const void* A, int64_t lda, const vo
                                  void* low, int low_split, void* stream) {
   if (const int rc = check(p, M, N, K)) return rc;
   if (!A || !W || !out || !low || (lda & 7) || (ldo & 3) || (residual && (ldr & 3)) || !aligned16(A) || !aligned16(W) || !aligned16(out) ||
-      !aligned16(low) || lda < 0 || lda > 0x100000)
+      !aligned16(low) || lda < 0 || lda > 0x100000 || ldo < 0 || ldo > 0x100000 || (residual && (ldr < 0 || ldr > 0x100000)))
     return MIMO_EINVAL;
   if (flags & ~(MIMO_EPI_OUT_F32 | MIMO_EPI_RES_F32)) return MIMO_EINVAL;
   const bool of32 = flags & MIMO_EPI_OUT_F32;
@@ -865,6 +865,7 @@ extern "C" int mimo_adapter_gemm_backward(int dtype, const void* dY, int64_t ldy
                                           float* ddown, float* dup, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = check(p, M, N, K)) return rc;
   if (!dY || !A || !low || !ddown || !dup || !workspace || (dA && !Wt) || (ldy & 7) || (lda & 7) || (ldda & 3) || lda < 0 || ldy < 0 || ldy > 0x100000 ||
+      ldda < 0 || ldda > 0x100000 ||
       !aligned16(dY) || !aligned16(A) || !aligned16(Wt) || !aligned16(dA) || !aligned16(low) || !aligned16(ddown) || !aligned16(dup) ||
       !aligned16(workspace) || workspace_bytes < backward_plan(dtype, p, M, N, K).total)
     return MIMO_EINVAL;

@@ -365,6 +365,12 @@ def _rows_ok(t, name):
         raise L.MimoHipError(f"{name}: 16-byte aligned rows (strides {st})")
 
 
+def _pitch_ok(t, name):
+    """Rows no further apart than the tile kernels' 32-bit offsets reach."""
+    if t.shape[0] > 1 and t.stride(0) > 1 << 20:
+        raise L.MimoHipError(f"{name}: rows {t.stride(0)} elements apart, at most {1 << 20}")
+
+
 def _same(ref, **tensors):
     """Operands of one call: one type, one device."""
     dt, dev = ref.dtype, ref.device
@@ -385,13 +391,14 @@ def _adapter_params(a, w, down, up, index, rows_per_index, scale, transposed=Fal
         raise L.MimoHipError(f"a {tuple(a.shape)}, w {tuple(w.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)} do not fit together")
     if S <= 0 or not 0 < r <= 128 or r & 7:
         raise L.MimoHipError(f"{S} adapters of rank {r}: ranks are multiples of 8 up to 128 (packing.pack_adapters pads)")
-    if N <= 0 or K <= 0 or (N | K) & 7 or N * K >= 1 << 30 or S > 65535 or M >= (1 << 31) - 1:
+    if N <= 0 or K <= 0 or (N | K) & 7 or N * K >= 1 << 30 or N >= 1 << 20 or K >= 1 << 20 or S > 65535 or M >= (1 << 31) - 1:
         raise L.MimoHipError(f"{M} rows, widths {N} and {K} (multiples of 8), {S} adapters: beyond what the kernels address")
     _same(a, w=w, down=down, up=up)
     for t, name in ((w, "w"), (down, "down"), (up, "up")):
         if not t.is_contiguous() or t.data_ptr() & 15:
             raise L.MimoHipError(f"{name}: contiguous, 16-byte aligned")
     _rows_ok(a, "a")
+    _pitch_ok(a, "a")
     if rows_per_index < 1:
         raise L.MimoHipError(f"rows_per_index {rows_per_index}")
     if index.dim() != 1 or index.dtype != torch.int32 or index.device != a.device or not index.is_contiguous() or \
@@ -425,6 +432,7 @@ def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=No
         if residual.shape != (M, N) or residual.device != a.device or residual.dtype not in (torch.float32, a.dtype):
             raise L.MimoHipError(f"residual: fp32 or {a.dtype} [{M}, {N}] on {a.device}")
         _rows_ok(residual, "residual")
+        _pitch_ok(residual, "residual")
     split = bool(want_low or out_f32)
     with _on_device(a.device):
         out = torch.empty((M, N), device=a.device, dtype=torch.float32 if out_f32 else a.dtype)
@@ -454,6 +462,7 @@ def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=
                              "(want_low=True)")
     _same(a, dout=dout, low=low)
     _rows_ok(dout, "dout")
+    _pitch_ok(dout, "dout")
     if not low.is_contiguous() or low.data_ptr() & 15:
         raise L.MimoHipError("low: contiguous, 16-byte aligned")
     with _on_device(a.device):
@@ -982,7 +991,7 @@ def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
         raise L.MimoHipError(f"k {tuple(k.shape)}, v {tuple(v.shape)}: [encoder rows, keys, {kv_heads * d}]")
     if Be <= 0 or B % Be:
         raise L.MimoHipError(f"{B} images over {Be} encoder rows")
-    if B // Be * Nq * (heads // kv_heads) >= 1 << 30 or Be * kv_heads >= 1 << 16 or Nk >= 1 << 30 or heads * Nq >= 1 << 27 or heads >= 1 << 16:
+    if B >= 1 << 31 or B // Be * Nq * (heads // kv_heads) >= 1 << 30 or Be * kv_heads >= 1 << 16 or Nk >= 1 << 30 or heads * Nq >= 1 << 27 or heads >= 1 << 16:
         raise L.MimoHipError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: beyond what the kernels address")
     _same(q, k=k, v=v)
     _rows_ok(q, "q")

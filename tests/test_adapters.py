@@ -351,6 +351,33 @@ def test_c_entry_refuses_what_it_cannot_run():
     assert bwd(ws=None) == -1 and bwd(nb=64) == -1 and bwd(Wt=None) == -1 and bwd(ldy=4) == -1
 
 
+def test_refuses_rows_and_widths_behind_32_bit_offsets():
+    from mimo_amd import lib, ops
+    x = dict(a=torch.zeros(6, 16, dtype=H), w=torch.zeros(24, 16, dtype=H), down=torch.zeros(2, 8, 16, dtype=H),
+             up=torch.zeros(2, 24, 8, dtype=H), index=torch.zeros(6, dtype=torch.int32))
+    far = lambda n, dt=H: torch.empty_strided((6, n), ((1 << 20) + 8, 1), dtype=dt)
+    with pytest.raises(lib.MimoHipError, match="elements apart"):
+        ops.adapter_gemm(**{**x, "a": far(16)})
+    for t in (far(24), far(24, torch.float32)):
+        with pytest.raises(lib.MimoHipError, match="elements apart"):
+            ops._pitch_ok(t, "residual")
+    ops._pitch_ok(far(24)[:1], "residual")
+    n = 1 << 20
+    wide = dict(a=torch.zeros(6, 8, dtype=H), w=torch.zeros(n, 8, dtype=H), down=torch.zeros(1, 8, 8, dtype=H), up=torch.zeros(1, n, 8, dtype=H),
+                index=x["index"])
+    with pytest.raises(lib.MimoHipError, match="beyond what"):
+        ops.adapter_gemm(**wide)
+    L = lib.load()
+    p = lib.AdapterParams(4096, 4096, None, 4096, 1, 2, 16)
+    call = lambda N=64, K=64, lda=64, ldo=64, res=None, ldr=64: L.mimo_adapter_gemm(
+        lib.F16, 4096, lda, 4096, 4096, ldo, 8, N, K, None, res, ldr, 0, ctypes.byref(p), 4096, 1, None)
+    back = lambda ldy=64, ldda=64: L.mimo_adapter_gemm_backward(lib.F16, 4096, ldy, 4096, 64, 4096, 4096, ldda, 8, 64, 64, ctypes.byref(p), 4096,
+                                                                4096, 4096, 4096, 1 << 30, None)
+    far = (1 << 20) + 8
+    assert call(N=n, ldo=n) == call(K=n, lda=n) == call(lda=far) == call(ldo=far) == call(ldo=-8) == call(res=4096, ldr=far) == -1
+    assert call(res=4096, ldr=-8) == back(ldy=far) == back(ldda=far) == back(ldda=-8) == -1
+
+
 def test_pack_adapters_pads_and_stacks():
     from mimo_amd.packing import pack_adapters
     g = torch.Generator().manual_seed(0)
