@@ -738,8 +738,8 @@ GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t
   return g;
 }
 
-// Up to 64 rows: the skinny kernel (N = K = 1280, r = 16: 19.7 us for 8 rows, 20.5 for 64, by the tiles 24.5 and 26.2; N = K = 320, 64
-// rows: 19.7 against 20.0); u inside it for up to four rows, whose adapters it takes one after another (17.2 us against 20.1 with a
+// Up to 64 rows: the skinny kernel (whole call, N = K = 1280, r = 16: 19.7 us for 8 rows, 20.5 for 64, by the tiles 24.5 and 26.2; N = K =
+// 320, 64 rows: 19.7 against 20.0); u inside it for up to four rows, whose adapters it takes one after another (17.2 us against 20.1 with a
 // launch for u; eight rows of different adapters 20.9 against 19.7).
 template <int DT>
 int launch_skinny(const GemmArgs& g, const LowArgs& la, bool give_low, hipStream_t st) {
