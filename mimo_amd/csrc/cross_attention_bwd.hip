@@ -13,7 +13,8 @@
 //                     share the query tiles that pass through LDS, P and dS packed are the operands of dV^T = dO^T.P and
 //                     dK^T = Q^T.dS.  The flat rows are cut into parts (gridDim.y) when the keys do not fill the chip; their
 //                     fp32 sums are joined in a fixed order by xattn_dkv_join_kernel: no atomics, the same bits every time.
-// P and dS are rounded to the operand type for the last products (one rounding each of the size of the results' own); sums, lse
+// P and dS are rounded to the operand type for the last products (one rounding each of the size of the results' own; dQ of heads up to
+// 32 wide takes dS's remainder as well); sums, lse
 // and delta are fp32.  What bounds dk / dv: products (22 % of the time), LDS (32 %) and vector instructions (34 %) hardly overlap at
 // two waves per SIMD: 49 us at the last of these shapes, 44 us at the first.
 #include "cross_attention.hip.h"
@@ -167,6 +168,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
         const uint4 ds = pack_k<DT>(s, u);
 #pragma unroll
         for (int i = 0; i < OT; ++i) acc[i] = HT<DT>::mfma32(read_tr(ks, P, kr + 16 * u, 32 * i, lane), ds, acc[i]);
+        if constexpr (KS == 2) {  // what dS lost, too: a narrow head's dQ is a sum that largely cancels (relative l2 at width 8, 77 keys
+          float hi[8];            // in fp16: 3.3e-4 with dS rounded, 2.35e-4 with its remainder, the result's own rounding 2.1e-4)
+          unpack8<DT>(ds, hi);
+          const uint4 lo = make_uint4(pack2<DT>(s[8 * u] - hi[0], s[8 * u + 1] - hi[1]), pack2<DT>(s[8 * u + 2] - hi[2], s[8 * u + 3] - hi[3]),
+                                      pack2<DT>(s[8 * u + 4] - hi[4], s[8 * u + 5] - hi[5]), pack2<DT>(s[8 * u + 6] - hi[6], s[8 * u + 7] - hi[7]));
+          acc[0] = HT<DT>::mfma32(read_tr(ks, P, kr + 16 * u, 0, lane), lo, acc[0]);
+        }
       }
     };
     if constexpr (RESIDENT) {
