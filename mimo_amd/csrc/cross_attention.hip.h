@@ -19,6 +19,7 @@ struct Args {
   uint16_t *out, *dk, *dv;       // out: the forward's output, or dq
   float *lse, *delta;            // [B, heads, Nq]
   float* ws;                     // partial results of a split launch
+  int* tops;                     // backward, fp16: [Be kvh][slots] exponents of bounds of |dS|, one per wave of dq, for dk / dv
   const int* kv_len;             // [Be] or null
   const uint8_t* mask;           // [Be, Nk] or null
   int64_t sqb, sqr, skb, skr, svb, svr, sob, sor, sdb, sdr, smb;  // element strides: batch, row (o / dout: sob.., sdb..)
@@ -27,6 +28,7 @@ struct Args {
   float c;                       // scale * log2(e): scores leave the matrix unit unscaled
   float scale, lag;
   int nb;                        // blocks per (e, g)
+  int slots;                     // waves of dq per (e, g)
   int nsplit;                    // parts the keys (forward, dq) or the flat rows (dk / dv) are cut into
 };
 
@@ -133,17 +135,29 @@ __device__ __forceinline__ void settle(uint4 (&f)[KS]) {
 constexpr int lanes_of(int ks) { return ks <= 2 ? 4 : 8; }
 constexpr int chunks_of(int ks) { return (2 * ks + lanes_of(ks) - 1) / lanes_of(ks); }
 
+// the larger magnitudes of two running fp16 maxima (bits without sign: they order like integers, NaN on top) and of eight halfs
+__device__ __forceinline__ uint32_t top_of(uint32_t top, uint4 y) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = __builtin_bit_cast(u16x2, top);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, (i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w) & 0x7fff7fffu));
+  return __builtin_bit_cast(uint32_t, m);
+}
+
 // Key and value rows [key0, key0 + N) of (e, g) on their way into row-major LDS tiles of pitch 16 KS + 8 halfs (an odd number of
 // 16-byte units: a 16-lane group of b128 row reads covers all banks).  issue() requests the rows, commit() writes them: between
 // the two a block computes on other rows.  Only keys below len are read; what the mask drops, rows behind len and channels
 // >= d are ZERO in LDS whatever memory holds there (NaN included), and bias[i] = 0 or -inf is added to their scores.
 // ones: V's channel d, which pads the last 32-channel tile, is 1 — the product with P then also leaves the sum of P in that row.
+// TOP (fp16): top collects the largest |v| of what is written, as bits, two maxima in one word.
 template <int KS, int THREADS, int N>
 struct Stager {
   static constexpr int P = 16 * KS + 8, LPR = lanes_of(KS), CH = chunks_of(KS), RP = THREADS / LPR, NC = (N + RP - 1) / RP;
   uint4 kr[NC][CH], vr[NC][CH];
   uint8_t keep;  // the mask's byte of key key0 + lane
   int left;      // keys of this piece
+  uint32_t top = 0u;
   const uint16_t *kb, *vb;
   __device__ __forceinline__ void open(const Args& a, int e, int g) {
     kb = a.k + (int64_t)e * a.skb + (int64_t)g * a.d;
@@ -169,7 +183,7 @@ struct Stager {
     keep = 1;
     if (a.mask) keep = a.mask[(int64_t)e * a.smb + key0 + min(tid & 63, left - 1)];
   }
-  template <int DT>
+  template <int DT, bool TOP = false>
   __device__ __forceinline__ void commit(const Args& a, uint16_t* ks, uint16_t* vs, float* bias, bool ones, int tid) {
     asm volatile("" : "+v"(tid));
     const int row0 = tid / LPR, cc = (tid & (LPR - 1)) * 8;
@@ -185,6 +199,7 @@ struct Stager {
         if (col < 16 * KS && (N % RP == 0 || row < N)) {
           const bool ok = alive && col < a.d;
           uint4 x = ok ? kr[i][c] : make_uint4(0, 0, 0, 0), y = ok ? vr[i][c] : make_uint4(0, 0, 0, 0);
+          if constexpr (TOP) top = top_of(top, y);
           if (ones && col == a.d) y.x = HT<DT>::from_f(1.f);
           *reinterpret_cast<uint4*>(ks + row * P + col) = x;
           *reinterpret_cast<uint4*>(vs + row * P + col) = y;
@@ -198,10 +213,11 @@ struct Stager {
   }
 };
 
-// all keys of (e, g), 96 at a time on their way
-template <int DT, int KS, int THREADS>
-__device__ __forceinline__ void stage_all(const Args& a, int e, int g, int len, uint16_t* ks, uint16_t* vs, float* bias, bool ones, int tid) {
+// all keys of (e, g), 96 at a time on their way; the thread's top (0 without TOP)
+template <int DT, int KS, int THREADS, bool TOP = false>
+__device__ __forceinline__ uint32_t stage_all(const Args& a, int e, int g, int len, uint16_t* ks, uint16_t* vs, float* bias, bool ones, int tid) {
   constexpr int P = 16 * KS + 8;
+  uint32_t top = 0u;
   for (int k0 = 0; k0 < len; k0 += 96) {
     Stager<KS, THREADS, 32> s[3];
 #pragma unroll
@@ -212,9 +228,13 @@ __device__ __forceinline__ void stage_all(const Args& a, int e, int g, int len, 
       }
 #pragma unroll
     for (int u = 0; u < 3; ++u)
-      if (k0 + 32 * u < len)
-        s[u].template commit<DT>(a, ks + (k0 + 32 * u) * P, vs + (k0 + 32 * u) * P, bias + k0 + 32 * u, ones, tid);
+      if (k0 + 32 * u < len) {
+        s[u].top = top;
+        s[u].template commit<DT, TOP>(a, ks + (k0 + 32 * u) * P, vs + (k0 + 32 * u) * P, bias + k0 + 32 * u, ones, tid);
+        top = s[u].top;
+      }
   }
+  return top;
 }
 
 // bytes of LDS that n staged keys take (+ the transposed reads of the last row's last tile, which run up to 16 halfs past it)

@@ -13,9 +13,9 @@
 //                     share the query tiles that pass through LDS, P and dS packed are the operands of dV^T = dO^T.P and
 //                     dK^T = Q^T.dS.  The flat rows are cut into parts (gridDim.y) when the keys do not fill the chip; their
 //                     fp32 sums are joined in a fixed order by xattn_dkv_join_kernel: no atomics, the same bits every time.
-// P and dS are rounded to the operand type for the last products (one rounding each of the size of the results' own; dQ of heads up to
-// 32 wide takes dS's remainder as well); sums, lse
-// and delta are fp32.  What bounds dk / dv: products (22 % of the time), LDS (32 %) and vector instructions (34 %) hardly overlap at
+// P and dS are rounded to the operand type for the last products (one rounding each, relative to the value, of the size of the results'
+// own; dQ of heads up to 32 wide takes dS's remainder as well); sums, lse and delta are fp32.  In fp16 dS is lifted by a power of two
+// first (lift_of), so that neither a small nor a large dO takes it out of that type's 30 binades.  What bounds dk / dv: products (22 % of the time), LDS (32 %) and vector instructions (34 %) hardly overlap at
 // two waves per SIMD: 49 us at the last of these shapes, 44 us at the first.
 #include "cross_attention.hip.h"
 
@@ -24,10 +24,40 @@ namespace {
 
 constexpr int stream_keys(int ks) { return ks >= 6 ? 32 : 64; }  // keys per streamed buffer of dq
 
+// dS in fp16.  dS follows dO, which may be anything from 1e-6 (a mean over many rows) to the loss scale of its user, and P, which is about
+// 1 / keys: unscaled it loses its bits below 2^-14 and is infinite above 65504, where dQ and dK, sums of it, still fit (512 rows, 1024
+// keys, dO of 1e-3: dQ off by 1.7e-3 relative l2 instead of 6.5e-4).  |dP| <= d max|V| max|dO| and P <= 1, so f dS with f = 2^(15 - e), e the
+// exponent of d max|V| max|dO| + |delta|, is always finite; a typical dP lies some seven binades below that bound, which leaves P 2^8 down
+// to 2^-14.  dq takes f per query (its lane's), dk / dv one for all rows of a key head, from the largest e that dq's waves left; f comes
+// off the fp32 sums exactly.  Price: max|V| while the keys are staged, max|dO| beside delta; nothing per pair of query and key (dQ with
+// resident keys 55.5 us with and without, 16 x 4096 queries, 8 heads of 40, 77 keys; streamed 83 -> 89, 16 rows of 4097 keys of width 64,
+// and 40 -> 44.5, 24 x 255 queries, 8 heads of 160, 257 keys; a running maximum of |dS| in both kernels' inner loops took 10 us of the
+// first shape's 139).
+constexpr int NO_ROW = -1000;  // e of a wave without rows
+__device__ __forceinline__ float lift_of(int e) { return ldexpf(1.f, 15 - e); }
+// the largest of the wave's two packed maxima, left for the block in one of eight words behind the value rows, which no read of this
+// file's kernels reaches (lane exchanges by DPP: through LDS they took 0.3 us per streamed chunk)
+__device__ __forceinline__ void put_top(uint32_t top, uint32_t* slots, int lane, int wave) {
+  uint32_t m = max(top & 0xffffu, top >> 16);
+#define STEP(ctrl) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, ctrl, 0xf, 0xf, false))
+  STEP(0x111); STEP(0x112); STEP(0x114); STEP(0x118);  // row_shr 1 2 4 8
+  STEP(0x142); STEP(0x143);                            // row_bcast 15 31
+#undef STEP
+  if (lane == 63) slots[wave] = m;
+}
+template <int NW>
+__device__ __forceinline__ float get_top(const uint32_t* slots) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m = max(m, slots[w]);
+  return HT<MIMO_F16>::to_f((uint16_t)__builtin_amdgcn_readfirstlane((int)m));
+}
+
 // RESIDENT: NW = 4 or 8 waves per block as in the forward; streamed: 4
 template <int DT, int KS, bool RESIDENT, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_kernel(const Args a) {
   constexpr int OT = (KS + 1) / 2, P = 16 * KS + 8, THREADS = 64 * NW, CH = stream_keys(KS);
+  constexpr bool LIFT = DT == MIMO_F16;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h2 = lane >> 5, li = lane & 31;
@@ -40,15 +70,23 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
   auto ks_of = [&](int b) { return reinterpret_cast<uint16_t*>(smem + b * stride); };
   auto vs_of = [&](int b) { return reinterpret_cast<uint16_t*>(smem + b * stride) + npad * P; };
   auto bias_of = [&](int b) { return reinterpret_cast<float*>(smem + b * stride + 2 * npad * P * 2 + 64); };
+  auto tops_of = [&](int b) { return reinterpret_cast<uint32_t*>(smem + b * stride + 2 * npad * P * 2); };
   Stager<KS, THREADS, CH> stager;
   stager.open(a, e, g);
   if constexpr (RESIDENT) {
-    stage_all<DT, KS, THREADS>(a, e, g, len, ks_of(0), vs_of(0), bias_of(0), false, tid);
+    const uint32_t top = stage_all<DT, KS, THREADS, LIFT>(a, e, g, len, ks_of(0), vs_of(0), bias_of(0), false, tid);
+    if constexpr (LIFT) put_top(top, tops_of(0), lane, wave);
     lds_barrier();
   }
+  auto commit = [&](int b) {
+    stager.top = 0u;
+    stager.template commit<DT, LIFT>(a, ks_of(b), vs_of(b), bias_of(b), false, tid);
+    if constexpr (LIFT) put_top(stager.top, tops_of(b), lane, wave);
+  };
   const int step = a.nb * NW;
   int t = j * NW + wave;
   const int rounds = (T - j * NW + step - 1) / step;
+  [[maybe_unused]] int most = NO_ROW;  // the largest e of the wave's rows (uniform)
 
   // delta from the rounded output is off by u |dO||O|: nothing beside dS where many keys share the row, but half of dQ's error where
   // two do (relative l2 of dQ at 2, 8, 32 keys of width 40 in fp16: 4.7, 3.2, 3.05e-4; from P and dP 2.9, 3.0, 2.96e-4).  Up to 32
@@ -93,6 +131,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
   for (int round = 0; RESIDENT ? t < T : round < rounds; t += step, ++round) {
     uint4 qf[KS], df[KS];
     float delta = 0.f, l2;
+    [[maybe_unused]] float size = 0.f;  // max |dO|
     {
       if constexpr (!AHEAD) request(min(t, T - 1), nx);
 #pragma unroll
@@ -105,12 +144,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
 #pragma unroll
         for (int i = 0; i < 8; ++i) p = fmaf(x[i], y[i], p);
         delta += kk < a.d ? p : 0.f;
+        if constexpr (LIFT) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) size = fmaxf(size, __builtin_fabsf(y[i]));  // (channels behind the last one repeat the first)
+        }
         qf[s] = nx.q[s];
         df[s] = nx.d[s];
       }
       l2 = nx.lse * LOG2E;
       if (AHEAD && t + step < T) request(t + step, nx);
       delta += __shfl_xor(delta, 32, 64);
+      if constexpr (LIFT) size = fmaxf(size, __shfl_xor(size, 32, 64));
     }
     if (l2 == -INFINITY) l2 = INFINITY;  // a row without a key: P = exp2(0 - inf) = 0
     if (few) {
@@ -143,6 +187,26 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
     for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    // e, f and f delta for values up to v_top; a streamed chunk that holds larger ones brings f, and the sums so far, down
+    [[maybe_unused]] float v_top = -1.f;
+    [[maybe_unused]] int ex = 15;
+    float f = 1.f, off = delta;
+    auto raise = [&](float top) {
+      v_top = top;
+      const float d1 = ldexpf(off, ex - 15);
+      const int to = __builtin_amdgcn_frexp_expf(fmaf(size * (float)a.d, top, __builtin_fabsf(d1)));
+      if constexpr (!RESIDENT) {
+        const float by = ldexpf(1.f, ex - to);
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] *= by;
+      }
+      ex = to;
+      f = lift_of(to);
+      off = d1 * f;
+    };
+    if constexpr (LIFT && RESIDENT) raise(get_top<NW>(tops_of(0)));
 
     auto tile = [&](const uint16_t* ks, const uint16_t* vs, const float* bias, int kr, bool masked) {
       f32x16 s, dp;
@@ -162,7 +226,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
         }
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], a.c, -l2)) * (dp[r] - delta);
+      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], a.c, -l2)) * (LIFT ? fmaf(dp[r], f, -off) : dp[r] - off);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const uint4 ds = pack_k<DT>(s, u);
@@ -184,7 +248,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
       if (chunks > 0) {
         stager.issue(a, e, len, 0, tid);
         if (round > 0) lds_barrier();
-        stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), false, tid);
+        commit(0);
         settle<KS>(qf);
         settle<KS>(df);
         if (chunks > 1) stager.issue(a, e, len, CH, tid);
@@ -192,19 +256,30 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
       for (int i = 0; i < chunks; ++i) {
         lds_barrier();
         const int bf = i & 1;
+        if constexpr (LIFT) {
+          const float top = get_top<NW>(tops_of(bf));
+          if (top > v_top) raise(top);
+        }
         if (t < T) {
           tile(ks_of(bf), vs_of(bf), bias_of(bf), 0, a.mask || i * CH + 32 > len);
           if (CH > 32 && i * CH + 32 < len) tile(ks_of(bf), vs_of(bf), bias_of(bf), 32, a.mask || i * CH + 64 > len);
         }
         if (i + 1 < chunks) {
-          stager.template commit<DT>(a, ks_of(bf ^ 1), vs_of(bf ^ 1), bias_of(bf ^ 1), false, tid);
+          commit(bf ^ 1);
           if (i + 2 < chunks) stager.issue(a, e, len, (i + 2) * CH, tid);
         }
       }
     }
     if (t >= T) continue;
+    if constexpr (LIFT) {
+      for (unsigned long long b = __builtin_amdgcn_ballot_w64(ex > most); b != 0ull; b = __builtin_amdgcn_ballot_w64(ex > most))
+        most = __builtin_amdgcn_readlane(ex, (int)__builtin_ctzll(b));
+    }
 #pragma unroll
-    for (int i = 0; i < OT; ++i) store_tile<DT>(acc[i], a.scale, out, i, a.d, h2);
+    for (int i = 0; i < OT; ++i) store_tile<DT>(acc[i], LIFT ? ldexpf(a.scale, ex - 15) : a.scale, out, i, a.d, h2);
+  }
+  if constexpr (LIFT) {
+    if (a.tops && lane == 0) a.tops[((int64_t)e * a.kvh + g) * a.slots + j * NW + wave] = most;
   }
 }
 
@@ -286,6 +361,17 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       *reinterpret_cast<uint4*>(smem + (row >= 2 * QT ? BUF - 2 * QT * P * 2 : 0) + row * P * 2 + col * 16) = make_uint4(0, 0, 0, 0);
     }
   }
+  // f of dS, from the largest e of this key head's rows
+  float f = 1.f;
+  if constexpr (DT == MIMO_F16) {
+    const int* tops = a.tops + ((int64_t)e * a.kvh + g) * a.slots;
+    int m = NO_ROW;
+#pragma unroll 4
+    for (int i = lane; i < a.slots; i += 64) m = max(m, tops[i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
+    f = lift_of(m);
+  }
   auto issue = [&](int t) __attribute__((always_inline)) {
     const uint16_t *qp = nullptr, *dp = nullptr;
 #pragma unroll
@@ -324,7 +410,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     asm volatile("" : "+v"(l));  // (not earlier: what is made of it would wait for the requests)
     if (tid < QT) {
       l2[tid] = l == -INFINITY || t * QT + tid >= a.R ? INFINITY : l * LOG2E;
-      l2[QT + tid] = dr;
+      l2[QT + tid] = dr * f;
     }
   };
   // row tile t is in buffer (t - t_lo) & 1, t + 1 on its way
@@ -360,7 +446,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
         for (int r = 0; r < 4; ++r) {
           const float p = fast_exp2(fmaf(s[4 * c + r], a.c, -l[r]));
           s[4 * c + r] = p;
-          dp[4 * c + r] = p * (dp[4 * c + r] - dl[r]);
+          dp[4 * c + r] = p * (DT == MIMO_F16 ? fmaf(dp[4 * c + r], f, -dl[r]) : dp[4 * c + r] - dl[r]);
         }
       }
 #pragma unroll
@@ -380,6 +466,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     issue(min(t + 2, t_hi - 1));
   }
   if (key >= a.Nk) return;
+  const float unlift = a.scale / f;
   const int64_t C = (int64_t)a.kvh * a.d, at = ((int64_t)e * a.Nk + key) * C + (int64_t)g * a.d, plane = (int64_t)a.Be * a.Nk * C;
 #pragma unroll
   for (int i = 0; i < OW; ++i)
@@ -390,7 +477,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       f32x4 x, y;  // a key that the mask drops has no gradient (its columns hold what zeros gave)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[r] = valid ? dk[i][4 * c + r] * a.scale : 0.f;
+        x[r] = valid ? dk[i][4 * c + r] * unlift : 0.f;
         y[r] = valid ? dv[i][4 * c + r] : 0.f;
       }
       if (a.nsplit > 1) {
@@ -460,17 +547,18 @@ Plan plan(const Args& a) {
   return p;
 }
 
-// workspace: delta [B, heads, Nq], then the parts' dk / dv
+// workspace: delta [B, heads, Nq], the exponents that dq leaves for dk / dv, then the parts' dk / dv
 int64_t delta_floats(const Args& a) { return ((int64_t)a.Be * a.kvh * a.R + 3) / 4 * 4; }
+int64_t top_floats(const Args& a, const Plan& p) { return a.Nk > 0 ? ((int64_t)a.Be * a.kvh * p.nb * p.dq_nw + 3) / 4 * 4 : 0; }
 size_t ws_bytes(const Args& a, const Plan& p) {
   const int64_t parts = p.nsplit > 1 ? (int64_t)p.nsplit * 2 * a.Be * a.Nk * a.kvh * a.d : 0;
-  return (size_t)(delta_floats(a) + parts) * sizeof(float);
+  return (size_t)(delta_floats(a) + top_floats(a, p) + parts) * sizeof(float);
 }
 
 template <int DT, int KS>
 int launch(Args& a, const Plan& p, hipStream_t st) {
   const unsigned eg = (unsigned)(a.Be * a.kvh);
-  a.nb = p.nb; a.nsplit = 1;
+  a.nb = p.nb; a.nsplit = 1; a.slots = p.nb * p.dq_nw;
   if (p.resident && p.dq_nw == 8) hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, true, 8>), dim3(eg * (unsigned)p.nb), dim3(512), p.lds, st, a);
   else if (p.resident) hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, true, 4>), dim3(eg * (unsigned)p.nb), dim3(256), p.lds, st, a);
   else hipLaunchKernelGGL((xattn_dq_kernel<DT, KS, false, 4>), dim3(eg * (unsigned)p.nb), dim3(256), p.lds, st, a);
@@ -532,7 +620,8 @@ extern "C" int mimo_cross_attention_backward(int dtype, const void* dout, const 
   const Plan pl = plan(a);
   if (workspace_bytes < ws_bytes(a, pl)) return MIMO_EINVAL;
   a.delta = (float*)workspace;
-  a.ws = (float*)workspace + delta_floats(a);
+  a.tops = a.Nk > 0 ? (int*)workspace + delta_floats(a) : nullptr;
+  a.ws = (float*)workspace + delta_floats(a) + top_floats(a, pl);
   if (dtype == MIMO_F16) return dispatch<MIMO_F16>(a, pl, (hipStream_t)stream);
   if (dtype == MIMO_BF16) return dispatch<MIMO_BF16>(a, pl, (hipStream_t)stream);
   return MIMO_EDTYPE;
