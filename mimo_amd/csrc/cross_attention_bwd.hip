@@ -361,7 +361,9 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
       *reinterpret_cast<uint4*>(smem + (row >= 2 * QT ? BUF - 2 * QT * P * 2 : 0) + row * P * 2 + col * 16) = make_uint4(0, 0, 0, 0);
     }
   }
-  // f of dS, from the largest e of this key head's rows
+  // f of dS, from the largest e of this key head's rows; in fp16 P itself is held as 2^14 P, f is what dS needs beyond that: a key among
+  // 16384 has P below fp16's normal range (64 queries, 60000 keys: dV off by 6.8e-4 relative l2 instead of 3e-4)
+  constexpr int UP = DT == MIMO_F16 ? 14 : 0;
   float f = 1.f;
   if constexpr (DT == MIMO_F16) {
     const int* tops = a.tops + ((int64_t)e * a.kvh + g) * a.slots;
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     for (int i = lane; i < a.slots; i += 64) m = max(m, tops[i]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o, 64));
-    f = lift_of(m);
+    f = lift_of(m + UP);
   }
   auto issue = [&](int t) __attribute__((always_inline)) {
     const uint16_t *qp = nullptr, *dp = nullptr;
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     float l = lr;
     asm volatile("" : "+v"(l));  // (not earlier: what is made of it would wait for the requests)
     if (tid < QT) {
-      l2[tid] = l == -INFINITY || t * QT + tid >= a.R ? INFINITY : l * LOG2E;
+      l2[tid] = l == -INFINITY || t * QT + tid >= a.R ? INFINITY : fmaf(l, LOG2E, (float)-UP);
       l2[QT + tid] = dr * f;
     }
   };
@@ -466,7 +468,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
     issue(min(t + 2, t_hi - 1));
   }
   if (key >= a.Nk) return;
-  const float unlift = a.scale / f;
+  const float drop = ldexpf(1.f, -UP), unlift = a.scale * drop / f;
   const int64_t C = (int64_t)a.kvh * a.d, at = ((int64_t)e * a.Nk + key) * C + (int64_t)g * a.d, plane = (int64_t)a.Be * a.Nk * C;
 #pragma unroll
   for (int i = 0; i < OW; ++i)
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(64 * NW * dkv_share(KS), dkv_occ(KS)) void xattn_dk
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         x[r] = valid ? dk[i][4 * c + r] * unlift : 0.f;
-        y[r] = valid ? dv[i][4 * c + r] : 0.f;
+        y[r] = valid ? dv[i][4 * c + r] * drop : 0.f;
       }
       if (a.nsplit > 1) {
         float* w = a.ws + (int64_t)blockIdx.y * 2 * plane + at + d0;
