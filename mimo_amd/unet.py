@@ -179,6 +179,9 @@ class UNetBase(HipModule):
                   if isinstance(m, SpatialTransformerBlock)]
         return sorted(blocks, key=lambda b: -b.dim)
 
+    def spatial_transformers(self):
+        return [m for part in (*self.down_blocks, self.mid_block, *self.up_blocks) for m in getattr(part, "attentions", None) or ()]
+
     def _pack(self, dt):
         dev = self.device
         h = lambda w: w.detach().to(dt).contiguous()
@@ -280,8 +283,10 @@ class UNetBase(HipModule):
         attentions collapse); pose_tok: [b*F, h, w, C0] (fp32|half) or None.
         Returns fp32 tokens [b*F, h, w, Cout_pad4] (or the last hidden state when there is no output head).
         precision "split": x_tok may be fp32 (then nothing of the input is rounded); see mimo_amd.precise."""
-        if (attn2 is not None or self.precision == "split") and (ehs_mask is not None or _several_tokens(ehs)):
-            raise ValueError("several or masked encoder tokens: precision \"half\", without the tables of clip_tables()")
+        if (ehs_mask is not None or _several_tokens(ehs)) and (
+                attn2 is not None or any(getattr(m, "precision", "half") == "split" for m in [self] + self.spatial_transformers())):
+            raise ValueError("several or masked encoder tokens: precision \"half\" of the model and its spatial transformers, without the "
+                             "tables of clip_tables()")
         if self.precision == "split":
             from . import precise
             return precise.run_tokens(self, x_tok, timestep, ehs, b, F, pose_tok, ctx, temb, attn2)

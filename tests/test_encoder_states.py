@@ -87,6 +87,27 @@ def test_refusals_of_several_tokens():
     assert ctx.tokens.dtype == torch.float16 and ctx.tokens_mask.dtype == torch.uint8
 
 
+def test_refusal_of_several_tokens_with_a_split_module():
+    """A single spatial transformer on split operands takes the collapsed form only: refused before anything has run (no bank is
+    written).  One token runs as before, and so does a split module of another kind."""
+    from mimo_amd.modules import SpatialTransformer
+    _, _, p3, p2 = build_pair_unets(torch.float16, torch.device("cpu"))
+    many, one = torch.randn(2, 7, 768), torch.randn(2, 1, 768)
+    keep = torch.ones(2, 7, dtype=torch.bool)
+    for u in (p3, p2):
+        all_of_it = [m for m in u.modules() if isinstance(m, SpatialTransformer)]
+        assert len(all_of_it) == 16
+        for m in all_of_it:
+            m.precision = "split"
+            for kw in (dict(ehs=many), dict(ehs=many, ehs_mask=keep), dict(ehs=one, ehs_mask=keep[:, :1])):
+                with pytest.raises(ValueError, match="spatial transformers"):
+                    u.run_tokens(None, 0, b=2, F=1, **kw)
+            del m.precision
+        u.up_blocks[-1].resnets[-1].precision = "split"
+        with pytest.raises(ValueError, match="encoder_"):   # (past the refusal: the shape is looked at next)
+            u.run_tokens(None, 0, many[:1], 2, 1)
+
+
 def test_packed_projections_follow_the_weights():
     _, _, p3, _ = build_pair_unets(torch.float16, torch.device("cpu"))
     blk = p3.spatial_blocks()[0]
