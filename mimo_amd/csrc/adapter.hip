@@ -555,7 +555,7 @@ __global__ __launch_bounds__(512) void adapter_skinny_kernel(const SkinnyArgs a)
         v *= scale_of(la, ad[0]);
         if (ad[0] < 0) v = (f32x4){0.f, 0.f, 0.f, 0.f};
         store_planes<DT>(la, us + li * ULP + j, v);
-        if (blockIdx.x == 0 && a.low && li < a.rows.M) store_planes<DT>(la, a.low + (int64_t)li * a.planes * a.r + j, v);
+        if (blockIdx.x == 0 && li < a.rows.M) store_planes<DT>(la, a.low + (int64_t)li * a.planes * a.r + j, v);
       }
     }
     lds_barrier();
@@ -742,8 +742,8 @@ GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t
 // 320, 64 rows: 19.7 against 20.0); u inside it for up to four rows, whose adapters it takes one after another (17.2 us against 20.1 with a
 // launch for u; eight rows of different adapters 20.9 against 19.7).
 template <int DT>
-int launch_skinny(const GemmArgs& g, const LowArgs& la, bool give_low, hipStream_t st) {
-  SkinnyArgs a{g.A, g.W, la.down, g.ad_up, la.scale, g.bias, g.res, g.out, give_low ? la.low : nullptr, g.lda, g.ldo, g.ldr, la.rows,
+int launch_skinny(const GemmArgs& g, const LowArgs& la, hipStream_t st) {
+  SkinnyArgs a{g.A, g.W, la.down, g.ad_up, la.scale, g.bias, g.res, g.out, la.low, g.lda, g.ldo, g.ldr, la.rows,
                g.N, g.K, la.r, la.planes, g.ad_cols, g.flags};
   const dim3 grid((unsigned)((g.N + 15) / 16));
   const int rt = (la.r + 15) / 16, mg = (int)((g.M + 15) / 16);
@@ -755,7 +755,6 @@ int launch_skinny(const GemmArgs& g, const LowArgs& la, bool give_low, hipStream
     return MIMO_OK;
   }
   if (const int rc = launch_low<DT>(la, st)) return rc;
-  a.low = la.low;
   if (mg == 1) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 1, 0>), grid, dim3(512), 0, st, a);
   else if (mg == 2) hipLaunchKernelGGL((adapter_skinny_kernel<DT, 2, 0>), grid, dim3(512), 0, st, a);
   else hipLaunchKernelGGL((adapter_skinny_kernel<DT, 4, 0>), grid, dim3(512), 0, st, a);
@@ -765,7 +764,7 @@ int launch_skinny(const GemmArgs& g, const LowArgs& la, bool give_low, hipStream
 
 template <int DT>
 int forward(const GemmArgs& g, const LowArgs& la, hipStream_t st) {
-  if (g.M <= 64) return launch_skinny<DT>(g, la, la.planes > 1, st);
+  if (g.M <= 64) return launch_skinny<DT>(g, la, st);
   if (const int rc = launch_low<DT>(la, st)) return rc;
   return launch_gemm<DT>(g, st);
 }

@@ -217,6 +217,33 @@ def test_requests_do_not_touch_each_other(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("M,r", [(1, 8), (3, 40), (4, 64), (4, 128), (9, 16), (70, 16), (2100, 16)])
+def test_low_holds_the_low_rank_values_afterwards(dev, dtype, split, M, r):
+    """What the C entry promises of `low`, whichever kernel the number of rows and the rank select: the rows' values rounded once, or
+    value and remainders, and zeros for a row without an adapter."""
+    from mimo_amd import lib, ops
+    K, N, S = 96, 80, 3
+    a, w = rnd((M, K), dev, dtype, 1), rnd((N, K), dev, dtype, 2, 0.1)
+    down, up, scale = rnd((S, r, K), dev, dtype, 3, 0.1), rnd((S, N, r), dev, dtype, 4, 0.1), rnd((S,), dev, torch.float32, 5).abs() + 0.5
+    index, per, who = layout("rows", M, S, dev)
+    planes = ops.LOW_PLANES[dtype] if split else 1
+    low, out = torch.full((M, planes * r), float("nan"), device=dev, dtype=dtype), torch.empty((M, N), device=dev, dtype=dtype)
+    p = lib.AdapterParams(down.data_ptr(), up.data_ptr(), scale.data_ptr(), index.data_ptr(), per, S, r)
+    lib.call("mimo_adapter_gemm", lib.F16 if dtype == torch.float16 else lib.BF16, a.data_ptr(), K, w.data_ptr(), out.data_ptr(), N, M, N, K,
+             None, None, 0, 0, ctypes.byref(p), low.data_ptr(), split, torch.cuda.current_stream().cuda_stream)
+    val, size = (torch.zeros((M, r), dtype=torch.float64, device=dev) for _ in range(2))
+    for i in range(S):
+        at = who == i
+        val[at] = float(scale[i]) * a[at].double() @ down[i].double().t()
+        size[at] = float(scale[i]) * a[at].double().abs() @ down[i].double().abs().t()
+    u, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -25 if dtype == torch.float16 else 0.0
+    got = low.double().reshape(M, planes, r).sum(1)
+    within("low", got, val, acc(K) * size + (u ** planes if split else u) * val.abs() * 1.01 + tiny)
+
+
+@gpu
 def test_gradient_against_differences(dev):
     """The directional derivative of sum(out g) along a step of a, down and up: the formula is bilinear in down and up and linear in
     a, so one central difference in 64 bits is exact."""
