@@ -422,7 +422,7 @@ int mimo_attention_fp8qk(int dtype, const void* q, int64_t ldq, const void* k, i
  *   half16 contiguous: dk / dv are summed over the images and query heads that share a key, in a fixed order (no atomics).
  *   workspace: 16-byte aligned scratch of at least the size that the *_workspace call returns for the same params (0: none
  *   needed); it holds nothing between calls.  Nq >= 1, Nk >= 0, B / Be * Nq * (heads / kv_heads) < 2^30, Be * kv_heads < 2^16,
- *   heads * Nq < 2^27.
+ *   heads * Nq < 2^27, 2^-126 <= scale <= 2^126.
  * --------------------------------------------------------------------------------- */
 typedef struct mimo_cross_attention_params {
   int B, Be, Nq, Nk, heads, kv_heads, d;

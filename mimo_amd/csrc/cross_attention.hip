@@ -21,7 +21,7 @@ namespace mimo_xattn {
 
 int fill(Args& a, const mimo_cross_attention_params* p) {
   if (!p || p->B <= 0 || p->Be <= 0 || p->B % p->Be || p->Nq <= 0 || p->Nk < 0 || p->heads <= 0 || p->kv_heads <= 0 ||
-      p->heads % p->kv_heads || p->d <= 0 || p->d > 160 || (p->d & 7) || !(p->scale > 0.f))
+      p->heads % p->kv_heads || p->d <= 0 || p->d > 160 || (p->d & 7) || !(p->scale >= 0x1p-126f && p->scale <= 0x1p126f))
     return MIMO_EINVAL;
   if ((p->q_batch & 7) || (p->q_row & 7) || (p->k_batch & 7) || (p->k_row & 7) || (p->v_batch & 7) || (p->v_row & 7)) return MIMO_EINVAL;
   a.Be = p->Be; a.G = p->B / p->Be; a.Nq = p->Nq; a.Nk = p->Nk; a.kvh = p->kv_heads; a.hg = p->heads / p->kv_heads; a.d = p->d;

@@ -1006,8 +1006,8 @@ def _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale):
     _rows_ok(k, "k")
     _rows_ok(v, "v")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise L.MimoHipError(f"scale {scale}")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:   # (what fp32 holds, log2(e) times it too)
+        raise L.MimoHipError(f"scale {scale}: positive, within 2^-126 .. 2^126")
     sq, sk, sv = q.stride(), k.stride(), v.stride()
     p = L.CrossAttentionParams(B, Be, Nq, Nk, heads, kv_heads, d, scale, sq[0] if B > 1 else 0, sq[1] if Nq > 1 else 0,
                                sk[0] if Be > 1 else 0, sk[1] if Nk > 1 else 0, sv[0] if Be > 1 else 0, sv[1] if Nk > 1 else 0)

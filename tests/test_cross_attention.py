@@ -379,6 +379,18 @@ def test_refusals(change, why):
         ops.cross_attention_backward(a["q"], a.pop("q"), a.pop("k"), a.pop("v"), a.pop("out"), torch.zeros(4, 2, 6), a.pop("heads"), **a)
 
 
+@pytest.mark.parametrize("scale", [1e39, 3e38, float("inf"), 1e-46, 1e-38, -1.0])
+def test_refuses_a_scale_outside_fp32(scale):
+    """A scale that fp32 turns into infinity, zero or a value whose log2(e)-fold is infinite would give NaN or the mean of the values."""
+    from mimo_amd import lib, ops
+    with pytest.raises(lib.MimoHipError, match="2\\^126"):
+        ops.cross_attention(**_host(scale=scale))
+    p = lib.CrossAttentionParams(4, 2, 6, 5, 2, 2, 32, scale, 384, 64, 320, 64, 320, 64)
+    L = lib.load()
+    assert L.mimo_cross_attention(lib.F16, 4096, 4096, 4096, 4096, None, ctypes.byref(p), None, 0, None) == -1
+    assert L.mimo_cross_attention_workspace(ctypes.byref(p)) == L.mimo_cross_attention_backward_workspace(ctypes.byref(p)) == 0
+
+
 def test_c_entry_refuses_what_it_cannot_run():
     """The C-ABI itself (no device is touched: every one of these returns before a launch)."""
     from mimo_amd import lib
