@@ -87,8 +87,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
   }
   const int step = a.nb * NW;
   int t = j * NW + wave;
-  // a streamed block's waves share its key buffers: all of them walk the same number of tiles
-  const int rounds = (T - j * NW + step - 1) / step;
 
   uint4 qf[KS], qn[RESIDENT ? KS : 1];
   auto query = [&](int tt, auto& f) {
@@ -100,7 +98,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
     if (t < T) query(t, qn);
   }
 
-  for (int round = 0; RESIDENT ? t < T : round < rounds; t += step, ++round) {
+  // (a streamed block has one tile per wave; its waves share the key buffers, so one without a tile goes through the chunks as well)
+  for (bool more = !RESIDENT || t < T; more; t += step, more = RESIDENT && t < T) {
     if constexpr (RESIDENT) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[s] = qn[s];
@@ -186,7 +185,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
       const int chunks = (k_hi - k_lo + CHK - 1) / CHK;
       if (chunks > 0) {
         stager.issue(a, e, k_hi, k_lo, tid);
-        if (round > 0) lds_barrier();  // the previous round's last chunk is read
         stager.template commit<DT>(a, ks_of(0), vs_of(0), bias_of(0), ones, tid);
         settle<KS>(qf);
         if (chunks > 1) stager.issue(a, e, k_hi, k_lo + CHK, tid);

@@ -29,7 +29,7 @@ struct Args {
   float scale, lag;
   int nb;                        // blocks per (e, g)
   int slots;                     // waves of dq per (e, g)
-  int nsplit;                    // parts the keys (forward, dq) or the flat rows (dk / dv) are cut into
+  int nsplit;                    // parts the keys (forward) or the flat rows (dk / dv) are cut into; dq takes all keys in one
 };
 
 // (image, token, head) of a flat row

@@ -85,7 +85,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
   };
   const int step = a.nb * NW;
   int t = j * NW + wave;
-  const int rounds = (T - j * NW + step - 1) / step;
   [[maybe_unused]] int most = NO_ROW;  // the largest e of the wave's rows (uniform)
 
   // delta from the rounded output is off by u |dO||O|: nothing beside dS where many keys share the row, but half of dQ's error where
@@ -128,7 +127,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
   Row nx;
   if (AHEAD && t < T) request(t, nx);
 
-  for (int round = 0; RESIDENT ? t < T : round < rounds; t += step, ++round) {
+  // (streamed: one tile per wave, as in the forward)
+  for (bool more = !RESIDENT || t < T; more; t += step, more = RESIDENT && t < T) {
     uint4 qf[KS], df[KS];
     float delta = 0.f, l2;
     [[maybe_unused]] float size = 0.f;  // max |dO|
@@ -247,7 +247,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
       const int chunks = (len + CH - 1) / CH;
       if (chunks > 0) {
         stager.issue(a, e, len, 0, tid);
-        if (round > 0) lds_barrier();
         commit(0);
         settle<KS>(qf);
         settle<KS>(df);
