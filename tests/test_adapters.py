@@ -218,6 +218,66 @@ def test_requests_do_not_touch_each_other(dev, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N,r,per", [
+    (3, 128, 160, 16, 1),          # the low-rank values inside the kernel for few rows
+    (40, 128, 160, 16, 1),         # in front of it
+    (61, 128, 160, 40, 7),         # ... by matrix tiles that several requests share
+    (200, 128, 160, 16, 24),       # boundaries inside a tile of 32 rows and of 64
+    (3000, 64, 320, 8, 100),
+    (10300, 64, 1280, 16, 333),    # 256 x 256 tiles
+    (33000, 64, 96, 24, 500),      # a wave per 32 rows
+])
+def test_requests_do_not_touch_each_other_in_any_kernel(dev, dtype, M, K, N, r, per):
+    """As above, for each of the kernels that sizes select: a zero operand in place of a selection would let NaN through."""
+    from mimo_amd import ops
+    S = 3
+    a, w = rnd((M, K), dev, dtype, 1), rnd((N, K), dev, dtype, 2, 0.1)
+    down, up = rnd((S, r, K), dev, dtype, 3, 0.1), rnd((S, N, r), dev, dtype, 4, 0.2)
+    dout = rnd((M, N), dev, dtype, 5)
+    index = torch.tensor([(0, 1, 2, 1, -1)[i % 5] for i in range((M + per - 1) // per)], dtype=torch.int32, device=dev)
+    mine = index.repeat_interleave(per)[:M] != 1
+    wt = w.t().contiguous()
+    d2, u2, a2, g2 = down.clone(), up.clone(), a.clone(), dout.clone()
+    d2[1, 0, 0], u2[1, 5, 3], a2[~mine], g2[~mine] = float("nan"), float("inf"), float("nan"), float("-inf")
+    for f32 in (False, True):
+        out, low = ops.adapter_gemm(a, w, down, up, index, rows_per_index=per, want_low=True, out_f32=f32)
+        out2, low2 = ops.adapter_gemm(a2, w, d2, u2, index, rows_per_index=per, want_low=True, out_f32=f32)
+        assert torch.equal(out[mine], out2[mine]) and torch.equal(low[mine], low2[mine]), f32
+    grads = ops.adapter_gemm_backward(dout, a, wt, down, up, index, low, rows_per_index=per)
+    grads2 = ops.adapter_gemm_backward(g2, a2, wt, d2, u2, index, low2, rows_per_index=per)
+    assert torch.equal(grads[0][mine], grads2[0][mine])
+    for i in (0, 2):
+        assert torch.equal(grads[1][i], grads2[1][i]) and torch.equal(grads[2][i], grads2[2][i])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,N,extras", [("ragged", 96, "bias"), ("groups", 160, "residual")])
+def test_rows_so_far_apart_that_launches_are_cut(dev, dtype, kind, N, extras):
+    """Rows 2^20 elements apart: 32-bit offsets reach 768 of them, so the tiles of 1100 rows go in two launches, the second with the
+    index, the low-rank values, the result and the residual moved on."""
+    from mimo_amd import ops
+    M, K, S, r, far = 1100, 128, 4, 16, 1 << 20
+    buf = torch.empty((M * far,), device=dev, dtype=dtype)
+    a, dout = torch.as_strided(buf, (M, K), (far, 1), 0), torch.as_strided(buf, (M, N), (far, 1), 512)
+    a.copy_(rnd((M, K), dev, dtype, 1)), dout.copy_(rnd((M, N), dev, dtype, 5))
+    w, down, up = rnd((N, K), dev, dtype, 2, K ** -0.5), rnd((S, r, K), dev, dtype, 3, K ** -0.5), rnd((S, N, r), dev, dtype, 4, r ** -0.5)
+    scale = rnd((S,), dev, torch.float32, 6).abs() + 0.5
+    bias = rnd((N,), dev, torch.float32, 7) if extras == "bias" else None
+    res = rnd((M, N), dev, torch.float32, 8) if extras == "residual" else None
+    index, per, who = layout(kind, M, S, dev)
+    kw = dict(rows_per_index=per, scale=scale)
+    for f32 in (False, True):
+        out, low = ops.adapter_gemm(a, w, down, up, index, bias=bias, residual=res, out_f32=f32, want_low=True, **kw)
+        val, bnd = reference(a, w, down, up, who, scale, bias, res, f32, None if f32 else dout)
+        within("out", out, val["out"], bnd["out"])
+        if not f32:
+            for name, got in zip(("da", "ddown", "dup"), ops.adapter_gemm_backward(dout, a, w.t().contiguous(), down, up, index, low, **kw)):
+                within(name, got, val[name], bnd[name])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("split", [0, 1])
 @pytest.mark.parametrize("M,r", [(1, 8), (3, 40), (4, 64), (4, 128), (9, 16), (70, 16), (2100, 16)])
 def test_low_holds_the_low_rank_values_afterwards(dev, dtype, split, M, r):
