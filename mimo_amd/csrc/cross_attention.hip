@@ -99,7 +99,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NW == 1 && KS >= 8 ? 1 : (KS
   }
 
   // (a streamed block has one tile per wave; its waves share the key buffers, so one without a tile goes through the chunks as well)
-  for (bool more = !RESIDENT || t < T; more; t += step, more = RESIDENT && t < T) {
+  for (bool first = true; RESIDENT ? t < T : first; t += step, first = false) {
     if constexpr (RESIDENT) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[s] = qn[s];

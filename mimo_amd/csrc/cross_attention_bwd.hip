@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && KS <= 3 ? 3 : 2) void xattn_dq_
   if (AHEAD && t < T) request(t, nx);
 
   // (streamed: one tile per wave, as in the forward)
-  for (bool more = !RESIDENT || t < T; more; t += step, more = RESIDENT && t < T) {
+  for (bool first = true; RESIDENT ? t < T : first; t += step, first = false) {
     uint4 qf[KS], df[KS];
     float delta = 0.f, l2;
     [[maybe_unused]] float size = 0.f;  // max |dO|
