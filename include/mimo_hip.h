@@ -146,7 +146,8 @@ int mimo_gemm_ext(int dtype, const void* A, int64_t lda, const void* W, void* ou
  *   scale: fp32 [count] or NULL (1); index: int32 device array of ceil(M / rows_per_index) entries, in any order and number; an
  *   entry outside [0, count) means no adapter.
  *   low: caller's half16 [M, rank] (low_split = 0) or [M, P rank] (low_split != 0: u as P = 2 (fp16) | 3 (bf16) planes, value and
- *   remainders, needed for a fp32 result and for the backward); it is written by the call and holds u afterwards.
+ *   remainders, needed for a fp32 result and for the backward); it is written by the call and holds u afterwards.  u, and t in the
+ *   backward, have the operands' range: in fp16 a value beyond 65504 makes the row's out or dA, and ddown, infinite or NaN.
  *   backward, W frozen: dA [M, ldda] half16 (nullable: not wanted) = dY.W + t.down with t = scale dY.up, from Wt = W^T, half16 [K, N];
  *   ddown fp32 [count, rank, K] = sum_m t[m]^T A[m], dup fp32 [count, N, rank] = sum_m dY[m]^T u[m], summed in a fixed order (no
  *   atomics; zeros for an adapter without rows).  low: the forward's split form.  workspace: 16-byte aligned, the size the

@@ -8,7 +8,11 @@
 // its rows, usually one; a row never takes part in another row's adapter (values are selected, not multiplied by zero, so a NaN
 // in one adapter stays in its requests).
 // u is kept as one rounded 16-bit value where the result is 16 bit, and as PLANES of 16-bit values (value | remainder: fp16 2, bf16
-// 3, i.e. at least 22 mantissa bits) where the result is fp32 or gradients are to be taken: [M, planes rank].
+// 3, i.e. at least 22 mantissa bits) where the result is fp32 or gradients are to be taken: [M, planes rank].  A 16-bit result takes the
+// value plane alone, da that of t: one rounding of the low-rank part, which is usually the smaller one, beside the result's own (out and
+// da 2.27e-4 relative l2 in fp16, the result's rounding 2.08e-4; bf16 1.82e-3 and 1.66e-3; where the low-rank part is
+// nearly all of it 2.94e-4).  In fp16 u and t end at 65504: beyond it the row's out or da, and the adapter's gradient, are infinite or NaN, as they are
+// for any 16-bit value between two products.
 //
 // Backward of the same call, W frozen: t[m] = scale[i] dy[m].up[i];  da = dy.W + t.down (the same kernels on W^T and transposed
 // adapters);  ddown[i] = sum_m t[m]^T a[m];  dup[i] = sum_m dy[m]^T u[m] (adapter_outer_kernel: rows stream through LDS, both
@@ -29,7 +33,9 @@ inline int cu_count() {
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int planes_of(int dt) { return dt == MIMO_F16 ? 2 : 3; }
-constexpr float T_SCALE = 2048.f;  // on the remainder plane of t in fp16: gradients are small, 2^-25 is not small beside them
+// on the remainder plane of t in fp16: gradients are small, 2^-25 is not small beside them (dO of 1e-5: ddown off by 4e-7; da, which takes
+// the value alone, 1.58e-3, its own rounding 1.54e-3)
+constexpr float T_SCALE = 2048.f;
 
 // which adapter a row has
 struct Rows {
@@ -257,7 +263,10 @@ __global__ __launch_bounds__(256) void adapter_transpose_kernel(const TransposeA
 // A block owns 128 columns of x and all ranks; tiles of 64 rows pass through LDS row-major, both operands are read transposed
 // (a row that is not this adapter's is staged as zeros on BOTH sides); the planes of low meet the same columns (fp16: the remainder
 // plane has accumulators of its own, its scale comes off at the end).  Rows: only [first, last] of the adapter, cut into gridDim.z parts.
-// Bound by the streams of a and dy: 49152 rows of 640 + 640, r = 32 in 33 us (3.8 TB/s).
+// Where an adapter's rows lie together it is bound by the streams of a and dy: 49152 rows of 640 + 640, r = 32 in 33 us (3.8 TB/s).
+// Every row BETWEEN an adapter's first and last passes, its own or not, so adapters in turn read them again for each (the whole backward
+// of the same rows, eight adapters: in runs of 6144 rows 115 us, 1024 rows of each in turn 228, an adapter per row in turn 339, in
+// runs 132: with an index per row each block walks all of it first, 255 us against 194 at 200000 rows of 320 + 320).
 struct OuterArgs {
   const uint16_t *x[2], *low[2];
   float* part[2];  // [parts][n][r][C]
@@ -449,8 +458,8 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(const float* p0, cons
 }
 
 // A few rows (M <= 16 MG) against the whole weight: a block of eight waves takes 16 columns, the waves share K (every eighth
-// k-step) and meet in LDS in wave order.  Bound by latency: one trip to W, one to the adapters (8 rows, N = K = 1280: 6.0 us, and 5.9
-// for u in front of it).  RT > 0 (MG = 1): u is computed
+// k-step) and meet in LDS in wave order.  Bound by latency: one trip to W, one to the adapters (8 rows, N = K = 1280: 7.0 us, and 7.5
+// for u in front of it, operands in no cache).  RT > 0 (MG = 1): u is computed
 // here too, by every block for itself — the rows' down weights come from L2 and a launch is saved; RT = 0: u is given.
 struct SkinnyArgs {
   const uint16_t *X, *W, *down, *up;
@@ -610,9 +619,14 @@ __global__ __launch_bounds__(512) void adapter_skinny_kernel(const SkinnyArgs a)
 // ---- host side --------------------------------------------------------------------------------------------------------------
 template <int DT>
 int launch_low(const LowArgs& a, hipStream_t st) {
-  // up to 1024 rows with an index each: a matrix tile would run once per adapter in it, a block per row reads what the row needs (whole
-  // call, N = K = 1280, r = 16, 1024 rows: of 64 adapters in turn 46 us against 95, of 8 in turn 31 against 39, of 8 in runs 26 against
-  // 21; 2048 rows of 8: 36 against 42 and 31 against 24)
+  // up to 1024 rows with an index each: a matrix tile would run once per adapter in it, a block per row reads what the row needs.  The
+  // order of the rows is not known here: the rule keeps the worst one in bounds and pays for it where requests lie in runs.  Whole call,
+  // N = K = 1280, 1024 rows, by rows | by tiles, us:
+  //            64 adapters in turn    8 in turn     8 in runs    64 in runs
+  //   r = 16       47 |  97            32 | 40       27 | 22       29 | 24
+  //   r = 64       90 | 164            59 | 60       49 | 24       56 | 30
+  //   r = 128     150 | 356            98 | 115      79 | 30       92 | 44
+  // (512 rows alike; 128 rows of 64 adapters in runs 36 | 58, 70 | 93, 116 | 186)
   if (a.rows.rpi == 1 && a.rows.M <= 1024 && a.rows.n > 1) {
     hipLaunchKernelGGL((adapter_low_row_kernel<DT>), dim3((unsigned)a.rows.M), dim3(256), 0, st, a);
     MIMO_LAUNCH_CHECK();
@@ -620,7 +634,7 @@ int launch_low(const LowArgs& a, hipStream_t st) {
   }
   const int rt = (a.r + 15) / 16;
   const int64_t m32 = (a.rows.M + 31) / 32;
-  // one wave per 32 rows would leave SIMDs empty (whole call, N = K = 640, r = 16: 29.9 us split, 32.5 not, at M = 16384; 69.3 and 66.4
+  // one wave per 32 rows would leave SIMDs empty (whole call, N = K = 640, r = 16: 30.5 us split, 33.1 not, at M = 16384; 69.7 and 67.7
   // at M = 49152)
   const bool ksplit = m32 < 4 * (int64_t)cu_count();
   const int64_t nwg = ksplit ? m32 : (m32 + 3) / 4;
@@ -693,8 +707,8 @@ int launch_gemm(GemmArgs g, hipStream_t st) {
     c.a_bytes = (unsigned)(((c.M - 1) * c.lda + c.K) * 2);
     const int64_t tn8 = (c.N + 255) / 256, nt8 = ((c.M + 255) / 256) * tn8;
     int rc;
-    // (256 x 256 tiles once they fill three quarters of the chip: 85.8 us against 91.5 for the other tiles at 245 of them, M = 12321,
-    // N = K = 1280, r = 64, fp32 out; 45.0 against 40.5 at 160, M = 8192, r = 16)
+    // (256 x 256 tiles once they fill three quarters of the chip: the whole call 104 us against 112 with the other tiles at 245 of them,
+    // M = 12321, N = K = 1280, r = 64, fp32 out, sixteen requests, and 80 against 90 with one; 44.8 against 39.3 at 160, M = 8192, r = 16)
     if ((c.K % 64) == 0 && tn8 * 256 - c.N <= c.N / 12 && 4 * nt8 >= 3 * (int64_t)cu_count() && nt8 <= 0x7fffffff) {
       c.tiles_n = (int)tn8;
       c.ntiles = (unsigned)G8_GM;
@@ -738,9 +752,9 @@ GemmArgs gemm_args(const void* A, int64_t lda, const void* W, void* out, int64_t
   return g;
 }
 
-// Up to 64 rows: the skinny kernel (whole call, N = K = 1280, r = 16: 19.7 us for 8 rows, 20.5 for 64, by the tiles 24.5 and 26.2; N = K =
-// 320, 64 rows: 19.7 against 20.0); u inside it for up to four rows, whose adapters it takes one after another (17.2 us against 20.1 with a
-// launch for u; eight rows of different adapters 20.9 against 19.7).
+// Up to 64 rows: the skinny kernel (whole call, N = K = 1280, r = 16: 21.3 us for 8 rows and for 64, by the tiles 23.9 and 30.0; N = K =
+// 320, 64 rows: 21.2 against 21.7); u inside it for up to four rows, whose adapters it takes one after another (four rows 18.7 us against
+// 21.4 with a launch for u; eight rows of different adapters: one kernel of 20.1 us, two of 14.5 together).
 template <int DT>
 int launch_skinny(const GemmArgs& g, const LowArgs& la, hipStream_t st) {
   SkinnyArgs a{g.A, g.W, la.down, g.ad_up, la.scale, g.bias, g.res, g.out, la.low, g.lda, g.ldo, g.ldr, la.rows,

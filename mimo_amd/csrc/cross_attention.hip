@@ -11,8 +11,8 @@
 // (xattn_kernel<RESIDENT>): no barrier after the first, the next tile's queries requested before this one's products.
 // Measured: 48 x 4096 queries, 8 heads of 40, 77 keys in 95 us (2.6 TB/s).  Neither the products (14 % of it) nor the vector
 // instructions (50 %) bound that but the 80-byte piece that a head has of a row: a copy of such pieces, a row per lane, takes 90 to
-// 103 us, of 320-byte pieces 53, of whole rows 36 to 41.  48 x 1024 queries, 8 heads of 80, 257 keys in 60 us: products and
-// exponentials in turn.
+// 103 us, of 320-byte pieces 53, of whole rows 36 to 41.  48 x 1024 queries, 8 heads of 80, 257 keys in 54 us, 60 with a mask: products
+// and exponentials in turn.
 // Longer key sequences stream through two LDS buffers of 64 keys that four query tiles share (RESIDENT = false), and when the
 // query tiles are too few to fill the chip the keys are cut into parts (gridDim.y) joined by xattn_join_kernel in a fixed order.
 #include "cross_attention.hip.h"
@@ -51,7 +51,7 @@ struct IC {
 // keys per streamed buffer: what a thread can hold on its way
 constexpr int stream_keys(int ks, int nw) { return ks >= 8 || (nw == 1 && ks > 4) ? 32 : 64; }
 
-constexpr float LAG = 8.f;  // log2 units by which a row's maximum may pass its reference before the row is rescaled (95.9 us, with 0 99.6)
+constexpr float LAG = 8.f;  // log2 units by which a row's maximum may pass its reference before the row is rescaled (48 x 1024 queries, 8 heads of 80, 257 keys: 54.2 us, with 0 56.4)
 
 // RESIDENT: all keys of (e, g) staged once; NW = 4 (two or more blocks per CU) or 8 (one).  Else: streamed in chunks of CHK keys
 // through two buffers, NW = 4 or 1 waves that share them.
@@ -298,11 +298,11 @@ struct Plan {
   int nw, chk, nb, nsplit, lds;
 };
 // Resident keys while two blocks of them fit a CU (4 waves), or one block of 8 waves when there are query tiles for them: 48 x 4096
-// queries, 8 heads of 40, 77 keys 97 us, streamed 122; 48 x 1024 queries, 8 heads of 80, 257 keys 56 against 86, 48 x 256 26 against 28.
+// queries, 8 heads of 40, 77 keys 98 us, streamed 102; 48 x 1024 queries, 8 heads of 80, 257 keys 54 against 74, 48 x 256 24 against 21.
 // The blocks are as many as are resident at once.  Streamed with one wave per block when one tile holds all queries (64 x 1 query, 16
-// heads of 64 on 2 key heads, 4097 keys: 32 us, four waves of which three wait 48), else four.  The keys are cut into parts while not
-// even half the chip has a block, a part keeping at least 256 keys (the same call uncut: 128 us; 2 x 1024 queries, 8 heads of 40, 4097
-// keys: 53 against 89; twice the parts 36 instead of 34).
+// heads of 64 on 2 key heads, 4097 keys: 36 us, four waves of which three wait 55), else four.  The keys are cut into parts while not
+// even half the chip has a block, a part keeping at least 256 keys (the same call uncut 141 us, with twice the parts 42, with half of
+// them 48; 2 x 1024 queries, 8 heads of 40, 4097 keys: 51, uncut 84, with twice the parts 39).
 Plan plan(const Args& a) {
   Plan p{};
   const int ks = k_steps(a.d), cus = cu_count(), eg = a.Be * a.kvh;

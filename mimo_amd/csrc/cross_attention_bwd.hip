@@ -8,15 +8,16 @@
 //                     resident in LDS as in the forward, or streamed; also leaves delta (few keys: sum_k P dP instead of dO.O).
 //                     What bounds it: the rows of q, dO, O and dQ, a piece of 2 d bytes per head and row: 55 us for 16 x 4096 queries,
 //                     8 heads of 40, 77 keys (3.1 TB/s); for 24 x 255 queries, 8 heads of 160, 257 streamed keys the exponentials and
-//                     LDS reads between the products of two waves per SIMD (39 us).
+//                     LDS reads between the products (35 us; a third of its blocks have no key there, so about one wave per SIMD).
 //   xattn_dkv_kernel  S = Q.K^T and dP = dO.V^T: a lane owns a key, a wave 32 of them with K and V in registers; the block's waves
 //                     share the query tiles that pass through LDS, P and dS packed are the operands of dV^T = dO^T.P and
 //                     dK^T = Q^T.dS.  The flat rows are cut into parts (gridDim.y) when the keys do not fill the chip; their
 //                     fp32 sums are joined in a fixed order by xattn_dkv_join_kernel: no atomics, the same bits every time.
 // P and dS are rounded to the operand type for the last products (one rounding each, relative to the value, of the size of the results'
 // own; dQ of heads up to 32 wide takes dS's remainder as well); sums, lse and delta are fp32.  In fp16 dS is lifted by a power of two
-// first (lift_of), so that neither a small nor a large dO takes it out of that type's 30 binades.  What bounds dk / dv: products (22 % of the time), LDS (32 %) and vector instructions (34 %) hardly overlap at
-// two waves per SIMD: 49 us at the last of these shapes, 44 us at the first.
+// first (lift_of), so that neither a small nor a large dO takes it out of that type's 30 binades.
+// What bounds dk / dv: products (22 % of the time), LDS (32 %) and vector instructions (34 %) hardly overlap at two waves per SIMD: 47 to
+// 49 us at the last of these shapes, 44 us at the first.
 #include "cross_attention.hip.h"
 
 namespace mimo_xattn {
@@ -520,10 +521,10 @@ struct Plan {
 // key tiles per block: heads whose tiles take two waves have 2
 constexpr int least_tiles = 2;
 constexpr int most_tiles(int ks) { return dkv_share(ks) == 2 ? 2 : 4; }
-// dq: as the forward (resident 105 us, streamed 108 for the whole backward of 16 x 4096 queries, 8 heads of 40, 77 keys).  dk / dv: the
-// number of key tiles per block (two to four) that leaves the fewest waves without one (same queries, 64 keys: 98 us, four of them
-// always 102; a block of one wave for 32 keys 116 against 108); the rows are cut into as many parts as fill the chip once with
-// resident blocks, a part keeping at least four row tiles (forward and backward 152 us; twice the parts 155, a third 170).
+// dq: as the forward, but all keys in one part (forward and backward of 16 x 4096 queries, 8 heads of 40, 77 keys: resident 136.5 us,
+// streamed 134.7).  dk / dv: the number of key tiles per block (two to four) that leaves the fewest waves without one (same queries, 64
+// keys: 124.5 us, four of them always 128.4; a block of one wave for 32 keys 116 against 108); the rows are cut into as many parts as
+// fill the chip once with resident blocks, a part keeping at least four row tiles (77 keys: twice the parts 143 us, a third 170).
 Plan plan(const Args& a) {
   Plan p{};
   const int ks = k_steps(a.d), cus = cu_count(), eg = a.Be * a.kvh;

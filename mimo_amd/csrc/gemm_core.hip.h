@@ -1,6 +1,6 @@
 // gemm_core.hip.h — the tile kernels of the dense GEMM and the implicit-GEMM convolution (see gemm_conv.hip, which instantiates
 // and launches them) with their epilogues; adapter.hip instantiates the dense ones with EPI = 3, whose epilogue is preceded by
-// the low-rank product of each row's adapter (tile_adapter, defined there).
+// the low-rank product of each row's adapter (tile_adapter).
 #pragma once
 #include "common.hip.h"
 
@@ -780,8 +780,8 @@ __device__ __forceinline__ void tile_epilogue_ln(const GemmArgs& g, f32x4 (&acc)
 // ---- EPI 3: out += low . up^T, every row with the adapter of its request ----
 // Where all rows of a tile have one adapter (most tiles: requests are longer than tiles) the low-rank product is the tile's last
 // K-tiles: the same ring, the operands come from `low` and from that adapter's `up`, nothing waits.  A tile with several adapters
-// takes tile_adapter behind the K loop instead (M = 12321, N = K = 1280, r = 64, fp32 out, the whole call: 75 us with one adapter in
-// every tile, 95 with sixteen runs of rows; without adapters 50).
+// takes tile_adapter behind the K loop instead (M = 12321, N = K = 1280, r = 64, fp32 out and residual, the whole call: 80 us with one
+// adapter, 104 with sixteen runs of rows; mimo_gemm without adapters 62).
 // adapters of rows M0 + lane, M0 + 64 + lane, ... (rows that do not exist: -2, no adapter: -1)
 template <int N>
 __device__ __forceinline__ void adapter_rows(const GemmArgs& g, const int64_t M0, const int lane, int (&ad)[N]) {

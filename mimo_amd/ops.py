@@ -430,7 +430,9 @@ def adapter_gemm(a, w, down, up, index, *, rows_per_index=1, scale=None, bias=No
     packing.pack_adapters pads and stacks checkpoints of any rank); index: int32 device tensor, one entry per rows_per_index
     consecutive rows, in any order; an entry outside [0, S) (use -1) means no adapter.  scale: fp32 [S] (None: 1); bias: fp32 [N];
     residual: fp32 or half [M, N].  Returns half, or fp32 with out_f32.
-    want_low: returns (out, low), low half [M, LOW_PLANES r] = the rows' scaled low-rank values, value and remainders, for the backward."""
+    want_low: returns (out, low), low half [M, LOW_PLANES r] = the rows' scaled low-rank values, value and remainders, for the backward.
+    The low-rank values are held in the type of `a`: in fp16 one beyond 65504 makes its row's result infinite or NaN.  Like every function
+    here it records no autograd graph: adapter_gemm_backward is the gradient."""
     p = _adapter_params(a, w, down, up, index, rows_per_index, scale)
     M, K = a.shape
     N, r = w.shape[0], p.rank
@@ -461,7 +463,9 @@ def adapter_gemm_backward(dout, a, w_t, down, up, index, low, *, rows_per_index=
     """(da, ddown, dup) of adapter_gemm with w frozen, from the gradient dout half [M, N] of its result (row-strided allowed), its
     operands, w_t = the transposed weight [K, N] (contiguous, laid out once) and its low (want_low=True).  da: half [M, K] (None
     with want_da=False); ddown fp32 [S, r, K] and dup fp32 [S, N, r] are summed over the rows of each adapter in a fixed order:
-    the same bits on every run, zeros for an adapter without rows.  (The residual's gradient is dout, the bias's its column sum.)"""
+    the same bits on every run, zeros for an adapter without rows.  (The residual's gradient is dout, the bias's its column sum.)
+    scale dout @ up is held in the type of `a`: in fp16 a value beyond 65504 makes its row of da and its adapter's ddown infinite or NaN
+    (a sign to lower the loss scale), whatever they would sum to."""
     p = _adapter_params(a, w_t, down, up, index, rows_per_index, scale, transposed=True)
     M, K = a.shape
     N, r, S = up.shape[1], p.rank, p.count
@@ -1032,7 +1036,8 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, kv_len=None, mask=None, sc
     key head h // (heads // kv_heads).  d a multiple of 8 up to 160; Nq = 1 and long Nk split the keys over the chip.
     kv_len: int32 [Be] device tensor, only keys below it count; mask: bool / uint8 [Be, Nk], only nonzero keys count (both may be
     given; what k and v hold elsewhere, NaN included, has no effect).  A query without any key gives zeros.
-    want_lse: returns (out, lse), lse fp32 [B, heads, Nq] = ln sum exp(scale q.k) (-inf without a key), for the backward."""
+    want_lse: returns (out, lse), lse fp32 [B, heads, Nq] = ln sum exp(scale q.k) (-inf without a key), for the backward.  Like every
+    function here it records no autograd graph: cross_attention_backward is the gradient."""
     p = _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale)
     with _on_device(q.device):
         out = q.new_empty(q.shape)
@@ -1051,7 +1056,8 @@ def cross_attention(q, k, v, heads, *, kv_heads=None, kv_len=None, mask=None, sc
 def cross_attention_backward(dout, q, k, v, out, lse, heads, *, kv_heads=None, kv_len=None, mask=None, scale=None):
     """(dq, dk, dv) of cross_attention, half and contiguous, from its operands, its output and its lse (want_lse=True) and the
     gradient dout [B, Nq, heads d] (any strides of whole 16-byte chunks).  dk and dv are summed over the images and query heads that
-    share a key, in a fixed order: the same bits on every run.  Keys that do not count get zeros."""
+    share a key, in a fixed order: the same bits on every run.  Keys that do not count get zeros.  dout may be of any size that its type
+    holds: what is rounded on the way is rounded relative to its value."""
     p = _cross_params(q, k, v, heads, kv_heads, kv_len, mask, scale)
     if dout.shape != q.shape or out.shape != q.shape:
         raise L.MimoHipError(f"dout {tuple(dout.shape)}, out {tuple(out.shape)}: as q {tuple(q.shape)}")

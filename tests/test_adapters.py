@@ -277,6 +277,38 @@ def test_rows_so_far_apart_that_launches_are_cut(dev, dtype, kind, N, extras):
 
 
 @gpu
+@pytest.mark.parametrize("M", [3, 40, 900])
+def test_low_rank_values_up_to_the_largest_fp16_and_beyond(dev, M):
+    """u and t up to 65504: right.  Beyond it: the rows concerned are infinite or NaN and the others are right; no finite number is wrong."""
+    from mimo_amd import ops
+    K, N, r = 64, 96, 8
+    w, wt = torch.zeros((N, K), device=dev, dtype=H), torch.zeros((K, N), device=dev, dtype=H)
+    a, dout = (torch.ones((M, n), device=dev, dtype=H) for n in (K, N))
+    down, up = torch.full((1, r, K), 2.0 ** -10, device=dev, dtype=H), torch.full((1, N, r), 2.0 ** -10, device=dev, dtype=H)
+    index = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def run(size, back):   # every u is `size`, every t is `back`
+        out, low = ops.adapter_gemm(size * 2.0 ** 4 * a, w, down, up, index, rows_per_index=M, want_low=True)
+        return out, low, *ops.adapter_gemm_backward(back * (2.0 ** 10 / N) * dout, a, wt, down, up, index, low, rows_per_index=M)
+    out, low, da, ddown, dup = run(4094.0, 384.0)   # (inputs within fp16 too)
+    assert torch.equal(out, torch.full_like(out, 4094.0 * r * 2.0 ** -10)) and torch.isfinite(ddown).all() and torch.isfinite(dup).all()
+    big = 2.0 ** 5      # the same with weights and adapters 2^5 larger: u = 131008, t = 12288
+    down, up = down * big, up * big
+    out, low, da, ddown, dup = run(4094.0, 384.0)
+    assert not torch.isfinite(out).any() and torch.isfinite(ddown).all()
+    a2, a3 = a.clone(), 4094.0 * 2.0 ** 4 * a
+    a3[1:] = a2[1:]
+    out, low = ops.adapter_gemm(a3, w, down, up, index, rows_per_index=M, want_low=True)
+    assert not torch.isfinite(out[0]).any() and torch.equal(out[1:], torch.full_like(out[1:], K * 2.0 ** -5 * r * 2.0 ** -5))
+    g = dout.clone()
+    g[0] = 384.0 * 2.0 ** 10 / N * 8    # t = 98304 in row 0, 3 elsewhere
+    _, low = ops.adapter_gemm(a, w, down, up, index, rows_per_index=M, want_low=True)
+    da, ddown, dup = ops.adapter_gemm_backward(g, a, wt, down, up, index, low, rows_per_index=M)
+    assert not torch.isfinite(da[0]).any() and torch.equal(da[1:], torch.full_like(da[1:], N * 2.0 ** -5 * r * 2.0 ** -5))
+    assert not torch.isfinite(ddown).any() and torch.isfinite(dup).all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("split", [0, 1])
 @pytest.mark.parametrize("M,r", [(1, 8), (3, 40), (4, 64), (4, 128), (9, 16), (70, 16), (2100, 16)])
