@@ -111,3 +111,27 @@ def test_value_gradient_of_keys_that_are_hardly_seen(dev, dtype, case):
     for name, got in zip(("dq", "dk", "dv"), grads):
         off = float((got.double() - val[name]).norm())
         assert off <= 1.15 * left[name], (name, off, left[name], float(val[name].norm()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Nk,d,heads", [(70, 40, 1), (64, 160, 1), (33, 16, 2), (300, 160, 1), (900, 128, 1), (1500, 24, 1), (257, 80, 1)])
+def test_one_large_value_anywhere(dev, dtype, Nk, d, heads):
+    """dS is held relative to a bound that contains the largest |v|: one value of 6e4 among others of 1e-3, at another key and channel in
+    each of 192 encoder rows, so that every lane and wave that looks for it has it once.  Missed, dS would be infinite.  A key that
+    does not count may hold anything."""
+    from mimo_amd import ops
+    E, Nq = 192, 33
+    q, k, v, dout = (x.to(dev) for x in operands((E, E, Nq, Nk, heads, heads, d, (1, 1, 1e-3, 1e-2)), dtype))
+    at = torch.randperm((Nk - 1) * heads * d, generator=torch.Generator().manual_seed(3))[:E].to(dev)
+    v.view(E, -1)[torch.arange(E, device=dev), at] = 6e4
+    v[:, -1], k[:, -1] = 65504.0, float("nan")
+    kv_len = torch.full((E,), Nk - 1, dtype=torch.int32, device=dev)
+    out, lse = ops.cross_attention(q, k, v, heads, kv_len=kv_len, want_lse=True)
+    grads = ops.cross_attention_backward(dout, q, k, v, out, lse, heads, kv_len=kv_len)
+    val, left = expected((E, E, Nq, Nk - 1, heads, heads, d, None), q, k[:, :-1], v[:, :-1], dout)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        assert torch.isfinite(got).all(), name
+        got = got if name == "dq" else got[:, :-1]
+        off = float((got.double() - val[name]).norm())
+        assert off <= 1.15 * left[name], (name, off, left[name], float(val[name].norm()))
