@@ -99,7 +99,7 @@ __device__ __forceinline__ float silu_f(float x) { return x / (1.0f + __expf(-x)
 // Q(u) = erfc(u / sqrt 2) / 2 = 2^P(u).  P = log2 Q is smooth; a degree-7 polynomial fitted for the absolute error of
 // u Q(u) on [0, 6] (beyond 6 the tail is below 1e-9: u is clamped) leaves |gelu error| <= 2.9e-7 evaluated in fp32 — tighter
 // than the Abramowitz-Stegun 7.1.26 erf it replaces (4.7e-7) — for ONE transcendental (v_exp) instead of two (v_rcp + v_exp)
-// and 7 FMAs that pair up as v_pk_fma_f32.  The GEGLU epilogues are VALU-bound on exactly this.
+// and 7 FMAs.  The GEGLU epilogues are VALU-bound on exactly this.
 constexpr float GELU_P[8] = {-0.9999997019767761f, -1.1511194705963135f, -0.4590896666049957f, -0.05285593867301941f,
                              0.007583224214613438f, -0.0005337183247320354f, -2.2708369215251878e-05f, 5.1834608711942565e-06f};
 __device__ __forceinline__ f32x2_t gelu_erf_2(f32x2_t x) {

@@ -32,8 +32,8 @@ constexpr int stream_keys(int ks) { return ks >= 6 ? 32 : 64; }  // keys per str
 // to 2^-14.  dq takes f per query (its lane's), dk / dv one for all rows of a key head, from the largest e that dq's waves left; f comes
 // off the fp32 sums exactly.  Price: max|V| while the keys are staged, max|dO| beside delta; nothing per pair of query and key (dQ with
 // resident keys 55.5 us with and without, 16 x 4096 queries, 8 heads of 40, 77 keys; streamed 83 -> 89, 16 rows of 4097 keys of width 64,
-// and 40 -> 44.5, 24 x 255 queries, 8 heads of 160, 257 keys; a running maximum of |dS| in both kernels' inner loops took 10 us of the
-// first shape's 139).
+// and 36.5 where bf16 takes 33.5, 24 x 255 queries, 8 heads of 160, 257 keys; a running maximum of |dS| in both kernels' inner loops
+// added 10 us to the first shape's 139).
 constexpr int NO_ROW = -1000;  // e of a wave without rows
 __device__ __forceinline__ float lift_of(int e) { return ldexpf(1.f, 15 - e); }
 // the largest of the wave's two packed maxima, left for the block in one of eight words behind the value rows, which no read of this
